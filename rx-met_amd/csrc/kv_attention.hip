@@ -1,0 +1,418 @@
+// kv_attention.hip — attention over the paged int8 cache.
+//
+// Mathematics.  For a query row q of head g (cache head g / (q_heads / heads)) and the cached
+// tokens t that it sees: s_t = (q . k_t) * ks * scale, out = sum_t softmax(s)_t * vs * v_t, with the codes k_t, v_t and
+// their pages' scales ks, vs.  One pass over the tokens keeps the running maximum m, the sum l of
+// 2^(s - m) (log2 e is part of the scale) and the weighted sum of the value codes; m, l and the
+// sums are fp32.
+//
+// Precision.  An int8 code is exact in fp16, so both products run on the fp16 matrix instruction
+// with the codes themselves and the scales stay outside.  A query row is brought to [-2, 2) by a power
+// of two, which keeps all of its bits.  The weights are rounded to fp16 (11 bits) once, as p * vs / R:
+// R is a running reference near the scales of the pages at hand (within a factor of 8 above the
+// largest of each 64 tokens), so that pages of any scale keep their bits; the sums are in units of R.
+//
+// Layout.  With mfma 16x16x32 (lane = (col, g), col = lane % 16, g = lane / 16) the first product is
+// taken as S^T = K Q^T on 64 tokens: row i of tile t stands for token 16 * (i / 4) + 4 t + i % 4, so that
+// lane (col, g) gets the scores of query col for the 16 consecutive tokens 16 g..16 g + 15.  The second
+// product is O^T = V^T P^T; its operand from P is what the lane holds already, and its operand
+// from V is 16 consecutive bytes, as values lie dimension by dimension.  Nothing crosses lanes but the row maximum.
+#include "kv_cache.h"
+#include <type_traits>
+
+#include "mfma_frag.h"
+
+namespace rxmet {
+namespace dec {
+namespace {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+constexpr int kRows = 16;   // query rows of a workgroup: one column of the matrix instruction each
+constexpr int kGroup = 64;  // tokens that a wave takes at a time
+constexpr int kWaves = 4;
+
+struct AttnArgs {
+  Pages g;
+  const int32_t *lengths, *cu;
+  int64_t queries;
+  const void *q;
+  int64_t stride_t, stride_h;
+  int q_heads, group;  // group = q_heads / heads
+  float scale;         // with log2 e
+  int causal;
+  int64_t window, chunk;
+  int splits, row_tiles;
+  void *out;
+  float *part, *stats;  // [splits, queries * q_heads, D] and [.., 2]: used where splits > 1
+};
+
+// Eight codes (two words) as fp16: 0x6400 | u is 1024 + u, and u is the code + 128.
+__device__ __forceinline__ v8h codes_f16(unsigned w0, unsigned w1) {
+  union {
+    unsigned u[4];
+    v2h h[4];
+    v8h v;
+  } r;
+  w0 ^= 0x80808080u;
+  w1 ^= 0x80808080u;
+  r.u[0] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04010400u);
+  r.u[1] = __builtin_amdgcn_perm(0x64646464u, w0, 0x04030402u);
+  r.u[2] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04010400u);
+  r.u[3] = __builtin_amdgcn_perm(0x64646464u, w1, 0x04030402u);
+  const v2h bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r.h[k] -= bias;
+  return r.v;
+}
+
+__device__ __forceinline__ v4f mfma_f16(v8h a, v8h b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Over the four lanes that share a column.
+__device__ __forceinline__ float col_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, kWave));
+  return fmaxf(v, __shfl_xor(v, 32, kWave));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  v += __shfl_xor(v, 16, kWave);
+  return v + __shfl_xor(v, 32, kWave);
+}
+
+// Tokens [lo, hi) that query i of n sees.
+struct Seen {
+  int64_t lo, hi;
+};
+__device__ __forceinline__ Seen seen_by(const AttnArgs &a, int64_t length, int64_t n, int64_t i) {
+  const int64_t pos = length - n + i;
+  Seen s{0, length};
+  if (a.causal && pos + 1 < s.hi) s.hi = pos + 1;
+  if (a.window > 0 && pos - a.window + 1 > 0) s.lo = pos - a.window + 1;
+  return s;
+}
+
+// The row's values as the matrix instruction's operands, brought to [-2, 2) by 2^-e; e returned.
+template <typename T, int D>
+__device__ __forceinline__ int load_query(const T *q, bool valid, int g, v8h (&out)[D / 64][2]) {
+  float f[D / 64][2][8];
+  float top = 0.0f;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (valid) {
+        load8(q + 64 * c + 16 * g + 8 * k, f[c][k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[c][k][e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[c][k][e]));
+    }
+  top = col_max(top);
+  const bool plain = top > 0.0f && top <= 3.402823466e38f;
+  const int e2 = plain ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        out[c][k][e] = static_cast<_Float16>(__builtin_amdgcn_ldexpf(f[c][k][e], -e2));
+  return e2;
+}
+
+// Sixteen query rows of one cache head, one chunk of their tokens.  The waves take groups of 64
+// tokens in turn and join their sums in LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
+  constexpr int NC = D / 64, NU = D / 16, pitch = D + 4;
+  __shared__ float s_acc[kWaves][kRows][pitch];
+  __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int col = lane % 16, g = lane / 16;
+  const int split = blockIdx.x % a.splits, head = blockIdx.y, b = blockIdx.z;
+  const int P = a.g.c.page_size, shift = __builtin_ctz(P), H = a.g.c.heads, G = a.group;
+  const int64_t length = a.lengths[b];
+  const int64_t q0 = a.cu ? a.cu[b] : b;
+  int64_t n = a.cu ? a.cu[b + 1] - q0 : 1;
+  if (q0 < 0) return;
+  if (n > a.queries - q0) n = a.queries - q0;
+  if (n <= 0) return;
+  const int64_t rows = n * G;
+  for (int64_t rt = blockIdx.x / a.splits; rt * kRows < rows; rt += a.row_tiles) {
+    const int64_t row = rt * kRows + col;
+    const bool valid = row < rows;
+    const Seen me = seen_by(a, length, n, valid ? row / G : n - 1);
+    const Seen top = seen_by(a, length, n, rt * kRows / G);  // the tile's first and last query
+    const int64_t last = rt * kRows + kRows - 1 < rows ? rt * kRows + kRows - 1 : rows - 1;
+    const Seen bot = seen_by(a, length, n, last / G);
+    const int64_t begin = (top.lo & ~static_cast<int64_t>(kGroup - 1)) + split * a.chunk;
+    const int64_t end =
+        split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
+
+    v8h q[NC][2];
+    const T *qp = static_cast<const T *>(a.q) + (q0 + (valid ? row / G : 0)) * a.stride_t +
+                  (head * static_cast<int64_t>(G) + (valid ? row % G : 0)) * a.stride_h;
+    const int e2 = load_query<T, D>(qp, valid, g, q);
+    const float q_scale = __builtin_amdgcn_ldexpf(a.scale, e2);
+
+    v4f acc[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) acc[u] = v4f{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f, ref = 1.0f, inv_ref = 1.0f;
+
+    for (int64_t t0 = begin + wave * kGroup; t0 < end; t0 += kWaves * kGroup) {
+      // the pages of this lane's key rows and of its sixteen tokens; past the end: any page
+      const int64_t tk = t0 + 16 * (col >> 2), tv = t0 + 16 * g;
+      const int64_t pk = tk < bot.hi ? page_of(a.g, b, tk >> shift) : 0;
+      const int64_t pv = tv < bot.hi ? page_of(a.g, b, tv >> shift) : 0;
+      const int64_t kat = (pk < 0 ? 0 : pk) * H + head, vat = (pv < 0 ? 0 : pv) * H + head;
+      const int8_t *kp = a.g.c.k + kat * P * D + ((tk & (P - 1)) + (col & 3)) * D + 16 * g;
+      const int8_t *vp = a.g.c.v + vat * P * D + static_cast<int64_t>(col) * P + (tv & (P - 1));
+      uint4 kw[4][NC], vw[NU];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          kw[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) vw[u] = *reinterpret_cast<const uint4 *>(vp + 16 * u * P);
+      float ks = 0.0f, vs = 0.0f;
+      if (tv < bot.hi) {
+        ks = pv < 0 ? nanf32() : a.g.c.k_scale[vat];
+        vs = pv < 0 ? nanf32() : a.g.c.v_scale[vat];
+      }
+
+      v4f s[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        s[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          s[t] = mfma_f16(codes_f16(kw[t][c].x, kw[t][c].y), q[c][0], s[t]);
+          s[t] = mfma_f16(codes_f16(kw[t][c].z, kw[t][c].w), q[c][1], s[t]);
+        }
+      }
+      const float f = ks * q_scale;
+      const bool whole = t0 >= bot.lo && t0 + kGroup <= top.hi;  // every row sees all 64
+      unsigned hidden = 0;  // bit 4 t + r: this row does not see the token
+      float high = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[t][r] *= f;
+          if (!whole) {
+            const int64_t tok = tv + 4 * t + r;
+            if (tok < me.lo || tok >= me.hi) {
+              s[t][r] = -INFINITY;
+              hidden |= 1u << (4 * t + r);
+            }
+          }
+          high = fmaxf(high, s[t][r]);
+        }
+      high = fmaxf(m, col_max(high));
+      const float base = high == -INFINITY ? 0.0f : high;
+      const float alpha = exp2f(m - base);
+      m = high;
+      // reference of the weights' rounding
+      const float big = col_max(vs == vs ? vs : 0.0f);
+      float fix = alpha;
+      if (big > 0.0f && (big > ref || big * 8.0f < ref)) {
+        fix *= ref / big;
+        ref = big;
+        inv_ref = 1.0f / big;
+      }
+      if (__any(fix != 1.0f)) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[u][r] *= fix;
+      }
+      l *= alpha;
+      const float ratio = vs * inv_ref;
+      v8h p[2];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = exp2f(s[t][r] - base);
+          l += e;
+          const bool gone = hidden >> (4 * t + r) & 1;
+          p[t / 2][4 * (t % 2) + r] = gone ? static_cast<_Float16>(0.0f)
+                                           : static_cast<_Float16>(e * ratio);
+        }
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        acc[u] = mfma_f16(codes_f16(vw[u].x, vw[u].y), p[0], acc[u]);
+        acc[u] = mfma_f16(codes_f16(vw[u].z, vw[u].w), p[1], acc[u]);
+      }
+    }
+
+    // the four waves' sums on one maximum
+    l = col_sum(l);
+    if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
+    __syncthreads();
+    float all = s_m[0][col];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) all = fmaxf(all, s_m[w][col]);
+    const float mine = exp2f(m - (all == -INFINITY ? 0.0f : all)) * ref;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = acc[u] * mine;
+    __syncthreads();
+    constexpr int per = D / 16;  // elements of a thread: 16 threads a row
+    const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * per;
+    const int64_t orow = rt * kRows + r;
+    if (orow < rows) {
+      float best = s_m[0][r], total = 0.0f;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) best = fmaxf(best, s_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w)
+        total += s_l[w][r] * exp2f(s_m[w][r] - (best == -INFINITY ? 0.0f : best));
+      const int64_t place = (q0 + orow / G) * a.q_heads + head * static_cast<int64_t>(G) + orow % G;
+      float o[per];
+#pragma unroll
+      for (int e = 0; e < per; ++e)
+        o[e] = s_acc[0][r][d0 + e] + s_acc[1][r][d0 + e] + s_acc[2][r][d0 + e] +
+               s_acc[3][r][d0 + e];
+      if (a.splits == 1) {
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        T *out = static_cast<T *>(a.out) + place * D + d0;
+#pragma unroll
+        for (int e = 0; e < per; ++e) out[e] = static_cast<T>(o[e] * inv);
+      } else {
+        const int64_t at = split * a.queries * a.q_heads + place;
+        if (d0 == 0) a.stats[2 * at] = best, a.stats[2 * at + 1] = total;
+        if (begin < end) {
+          float *part = a.part + at * D + d0;
+#pragma unroll
+          for (int e = 0; e < per; ++e) part[e] = o[e];
+        }
+      }
+    }
+    __syncthreads();  // the next tile writes the LDS again
+  }
+}
+
+// Joins the chunks of a row: one wave each, in the chunks' order.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t rows = a.queries * a.q_heads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
+  if (row >= rows) return;
+  float best = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) best = fmaxf(best, a.stats[2 * (s * rows + row)]);
+  const float base = best == -INFINITY ? 0.0f : best;
+  float total = 0.0f, o[D / 64] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = s * rows + row;
+    const float l = a.stats[2 * at + 1], f = exp2f(a.stats[2 * at] - base);
+    if (l == 0.0f) continue;  // the chunk held nothing that the row sees (NaN is not 0)
+    total += l * f;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] += a.part[at * D + 64 * e + lane] * f;
+  }
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  T *out = static_cast<T *>(a.out) + row * D + lane;
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) out[64 * e] = static_cast<T>(o[e] * inv);
+}
+
+struct Plan {
+  int64_t row_tiles, chunk;
+  int splits;
+};
+
+// Chunks of the token axis: enough workgroups to fill the GPU (four for each of 256 CUs), each
+// with at least 512 tokens, eight groups, so that its start and its sums' join stay small beside them.
+Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t max_query, int64_t max_length,
+              int64_t window) {
+  Plan p;
+  p.row_tiles = cdiv((max_query < 1 ? 1 : max_query) * group, kRows);
+  int64_t span = max_length;
+  if (window > 0 && window + max_query + kGroup < span) span = window + max_query + kGroup;
+  const int64_t tiles = p.row_tiles * heads * seqs;
+  int64_t splits = cdiv(1024, tiles < 1 ? 1 : tiles);
+  if (splits > cdiv(span, 512)) splits = cdiv(span, 512);
+  if (splits < 1) splits = 1;
+  p.chunk = cdiv(cdiv(span, splits), kWaves * kGroup) * (kWaves * kGroup);
+  if (p.chunk < 1) p.chunk = kWaves * kGroup;
+  p.splits = static_cast<int>(span < 1 ? 1 : cdiv(span, p.chunk));
+  return p;
+}
+
+}  // namespace
+}  // namespace dec
+}  // namespace rxmet
+
+using namespace rxmet;
+using namespace rxmet::dec;
+
+extern "C" int64_t rxmet_kv_attention_workspace_bytes(const rxmet_kv_cache *cache, int32_t seqs,
+                                                      int64_t queries, int32_t q_heads,
+                                                      int64_t max_query, int64_t max_length,
+                                                      int64_t window) {
+  if (!cache || cache->heads < 1 || q_heads < cache->heads || queries <= 0 || seqs <= 0) return 0;
+  const Plan p = plan_for(cache->heads, seqs, q_heads / cache->heads, max_query, max_length, window);
+  return p.splits == 1 ? 0 : p.splits * queries * q_heads * (cache->dim + 2) * 4;
+}
+
+extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_table *table,
+                                  const int32_t *lengths, const int32_t *cu_query, int64_t queries,
+                                  int64_t max_query, int64_t max_length, const void *query,
+                                  int64_t query_stride_t, int64_t query_stride_h, int32_t q_heads,
+                                  float scale, int32_t causal, int64_t window, void *out,
+                                  int32_t dtype, void *workspace, void *stream) {
+  if (int rc = check_cache(cache, table)) return rc;
+  RXMET_CHECK_ARG(dtype == RXMET_QDQ_F16 || dtype == RXMET_QDQ_BF16,
+                  "queries must be fp16 or bf16");
+  RXMET_CHECK_ARG(q_heads >= cache->heads && q_heads % cache->heads == 0,
+                  "query heads must be a multiple of the cache's heads");
+  RXMET_CHECK_ARG(queries >= 0 && max_query >= 0 && max_length >= 0 && window >= 0,
+                  "queries, max_query, max_length and window must be >= 0");
+  RXMET_CHECK_ARG(max_query <= INT32_MAX && max_length <= INT32_MAX && queries <= INT32_MAX,
+                  "lengths must be below 2^31");
+  RXMET_CHECK_ARG(cu_query || queries == table->seqs,
+                  "without cu_query there is one query a sequence");
+  if (queries == 0 || table->seqs == 0) return 0;
+  RXMET_CHECK_ARG(lengths && query && out, "lengths, query and out are needed");
+  const int group = q_heads / cache->heads;
+  const Plan p = plan_for(cache->heads, table->seqs, group, max_query, max_length, window);
+  RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
+  RXMET_CHECK_ARG(p.row_tiles * p.splits <= INT32_MAX, "too many query rows for one call");
+  const int64_t rows = queries * q_heads;
+  float *part = static_cast<float *>(workspace);
+  const AttnArgs a{{*cache, *table}, lengths, cu_query, queries, query, query_stride_t,
+                   query_stride_h, q_heads, group, scale * 1.44269504088896340736f, causal, window,
+                   p.chunk, p.splits, static_cast<int>(p.row_tiles), out, part,
+                   part ? part + p.splits * rows * cache->dim : nullptr};
+  auto st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(p.row_tiles * p.splits), cache->heads, table->seqs);
+  prof::Scope scope("kv_attention", st);
+  auto launch = [&](auto t, auto dim) {
+    using T = decltype(t);
+    attn_rows<T, dim.value><<<grid, 256, 0, st>>>(a);
+    if (p.splits > 1)
+      attn_join<T, dim.value><<<static_cast<unsigned>(cdiv(rows, kWaves)), 256, 0, st>>>(a);
+  };
+  auto with_dim = [&](auto t) {
+    switch (cache->dim) {
+      case 64: launch(t, std::integral_constant<int, 64>{}); break;
+      case 128: launch(t, std::integral_constant<int, 128>{}); break;
+      case 192: launch(t, std::integral_constant<int, 192>{}); break;
+      default: launch(t, std::integral_constant<int, 256>{}); break;
+    }
+  };
+  if (dtype == RXMET_QDQ_F16)
+    with_dim(f16{});
+  else
+    with_dim(bf16{});
+  RXMET_CHECK_LAUNCH();
+  return 0;
+}

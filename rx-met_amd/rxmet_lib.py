@@ -55,11 +55,29 @@ class BlockJob(ctypes.Structure):
 
 BLOCK_JOBS = 16  # RXMET_BLOCK_JOBS
 
+
+class KvCache(ctypes.Structure):
+    """rxmet_kv_cache (include/rxmet_decoder.h): int8 pages of keys and values, their scales."""
+    _fields_ = [("k", c_ptr), ("v", c_ptr), ("k_scale", c_ptr), ("v_scale", c_ptr),
+                ("pages", c_i64), ("heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("dim", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class KvTable(ctypes.Structure):
+    """rxmet_kv_table: the pages of each sequence."""
+    _fields_ = [("ids", c_ptr), ("stride", c_i64), ("seqs", ctypes.c_int32),
+                ("cols", ctypes.c_int32)]
+
+
 _LAY = ctypes.POINTER(QdqLayout)
 _MME = ctypes.POINTER(QdqMinMaxEnc)
 _NUM = ctypes.POINTER(QdqNumerics)
+_KVC = ctypes.POINTER(KvCache)
+_KVT = ctypes.POINTER(KvTable)
+_i32 = ctypes.c_int32
 
-# name -> (restype, argtypes); mirrors include/rxmet_qdq.h and include/rxmet_gru.h
+# name -> (restype, argtypes); mirrors include/rxmet_qdq.h, include/rxmet_decoder.h and the shared
+# entry points
 _SIGNATURES = {
     "rxmet_last_error": (ctypes.c_char_p, []),
     "rxmet_abi_version": (c_int, []),
@@ -106,6 +124,22 @@ _SIGNATURES = {
     "rxmet_prof_query": (c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
                                  ctypes.POINTER(c_i64)]),
     "rxmet_prof_names": (c_i64, [ctypes.c_char_p, c_i64]),
+    "rxmet_rms_quantize_forward": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, _i32, c_ptr, c_ptr,
+                                           c_ptr, c_ptr, c_ptr, c_i64, c_i64, _i32, c_float,
+                                           c_ptr]),
+    "rxmet_rms_quantize_backward_workspace_bytes": (c_i64, [c_i64, c_i64]),
+    "rxmet_rms_quantize_backward": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, _i32,
+                                            c_ptr, c_ptr, c_ptr, c_i64, c_i64, _i32, c_ptr,
+                                            c_ptr]),
+    "rxmet_linear_int8_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "rxmet_linear_int8": (c_int, [c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64,
+                                  c_ptr, c_i64, c_i64, c_i64, _i32, _i32, c_ptr, c_ptr]),
+    "rxmet_kv_append": (c_int, [_KVC, _KVT, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64,
+                                c_ptr, c_i64, c_i64, _i32, c_ptr]),
+    "rxmet_kv_read": (c_int, [_KVC, _KVT, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_ptr, _i32, c_ptr]),
+    "rxmet_kv_attention_workspace_bytes": (c_i64, [_KVC, _i32, c_i64, _i32, c_i64, c_i64, c_i64]),
+    "rxmet_kv_attention": (c_int, [_KVC, _KVT, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64,
+                                   c_i64, _i32, c_float, _i32, c_i64, c_ptr, _i32, c_ptr, c_ptr]),
 }
 
 
