@@ -93,34 +93,32 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs &a, int64_t length, int64
   return s;
 }
 
-// The row's values as the matrix instruction's operands, brought to [-2, 2) by 2^-e; e returned.
-template <typename T, int D>
-__device__ __forceinline__ int load_query(const T *q, bool valid, int g, v8h (&out)[D / 64][2]) {
-  float f[D / 64][2][8];
+// Pieces of a query row (eight elements each, `at(i)` the place of piece i) as operands of the
+// matrix instruction, brought to [-2, 2) by 2^-e; e returned.  A row with a NaN or an infinity is NaN throughout.
+// `join` takes the NaN-keeping maximum over the lanes that share the row.
+template <typename T, int N, typename At, typename Join>
+__device__ __forceinline__ int load_query(const T *q, bool valid, At at, Join join, v8h (&out)[N]) {
+  float f[N][8];
   float top = 0.0f;
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c)
+  for (int i = 0; i < N; ++i) {
+    if (valid) {
+      load8(q + at(i), f[i]);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (valid) {
-        load8(q + 64 * c + 16 * g + 8 * k, f[c][k]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[c][k][e] = 0.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[c][k][e]));
+      for (int e = 0; e < 8; ++e) f[i][e] = 0.0f;
     }
-  top = col_max(top);
-  const bool plain = top > 0.0f && top <= 3.402823466e38f;
-  const int e2 = plain ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c)
+    for (int e = 0; e < 8; ++e) top = nan_max(top, fabsf(f[i][e]));
+  }
+  top = join(top);
+  const bool good = top <= 3.402823466e38f;
+  const int e2 = good && top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 1 : 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        out[c][k][e] = static_cast<_Float16>(__builtin_amdgcn_ldexpf(f[c][k][e], -e2));
+    for (int e = 0; e < 8; ++e)
+      out[i][e] = static_cast<_Float16>(good ? __builtin_amdgcn_ldexpf(f[i][e], -e2) : nanf32());
   return e2;
 }
 
@@ -153,10 +151,16 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
     const int64_t end =
         split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
 
-    v8h q[NC][2];
+    v8h q[2 * NC];
     const T *qp = static_cast<const T *>(a.q) + (q0 + (valid ? row / G : 0)) * a.stride_t +
                   (head * static_cast<int64_t>(G) + (valid ? row % G : 0)) * a.stride_h;
-    const int e2 = load_query<T, D>(qp, valid, g, q);
+    const int e2 = load_query(
+        qp, valid, [&](int i) { return 64 * (i / 2) + 16 * g + 8 * (i % 2); },
+        [](float v) {
+          v = nan_max(v, __shfl_xor(v, 16, kWave));
+          return nan_max(v, __shfl_xor(v, 32, kWave));
+        },
+        q);
     const float q_scale = __builtin_amdgcn_ldexpf(a.scale, e2);
 
     v4f acc[NU];
@@ -192,8 +196,8 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
         s[t] = v4f{0, 0, 0, 0};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          s[t] = mfma_f16(codes_f16(kw[t][c].x, kw[t][c].y), q[c][0], s[t]);
-          s[t] = mfma_f16(codes_f16(kw[t][c].z, kw[t][c].w), q[c][1], s[t]);
+          s[t] = mfma_f16(codes_f16(kw[t][c].x, kw[t][c].y), q[2 * c], s[t]);
+          s[t] = mfma_f16(codes_f16(kw[t][c].z, kw[t][c].w), q[2 * c + 1], s[t]);
         }
       }
       const float f = ks * q_scale;
@@ -299,34 +303,298 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
   }
 }
 
-// Joins the chunks of a row: one wave each, in the chunks' order.
+// ---------------------------------------------------------------------------------------------
+// Many query rows: 128 rows of one cache head, 32 to a wave, on mfma 32x32x16 (lane = (col, h),
+// col = lane % 32, h = lane / 32).  The workgroup brings 64 tokens at a time into LDS as fp16, so that the
+// codes are converted once for all 128 rows, while the next 64 are on their way.  As above,
+// S^T = K Q^T with row i of tile t standing for token 32 t + 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4, so that a lane holds
+// 16 consecutive tokens of one page a tile, and the weights are the second product's operand
+// where they are.  The weights are 2^(s f - m + log2(vs / R)): vs / R costs nothing for each weight, and l takes it
+// out again once for 16 of them.  The reference m follows the maximum only when that is more than
+// 8 above it, which leaves weights below 2^8 and spares most rescalings of the sums.
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int kTileRows = 128;
+
+__device__ __forceinline__ v16f mfma32_f16(v8h a, v8h b, v16f c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
 template <typename T, int D>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArgs a) {
+  constexpr int KC = D / 16, NU = D / 32;   // steps of the first product, tiles of the second
+  constexpr int kp = kGroup + 1, vp = D + 1;  // pitches in units of 16 bytes
+  constexpr int pieces = D * kGroup / 16 / 256;  // of keys and of values for each thread
+  struct Stage {
+    uint4 k[D / 8 * kp];  // [8 dimensions][row of the tiles]
+    uint4 v[8 * vp];      // [8 tokens][dimension]
+    float ks[4], vs[4];   // of 16 tokens each
+  };
+  __shared__ Stage stage[2];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int col = lane % 32, h = lane / 32;
+  const int split = blockIdx.x % a.splits, head = blockIdx.y, b = blockIdx.z;
+  const int P = a.g.c.page_size, shift = __builtin_ctz(P), H = a.g.c.heads, G = a.group;
+  const int64_t length = a.lengths[b];
+  const int64_t q0 = a.cu ? a.cu[b] : b;
+  int64_t n = a.cu ? a.cu[b + 1] - q0 : 1;
+  if (q0 < 0) return;
+  if (n > a.queries - q0) n = a.queries - q0;
+  if (n <= 0) return;
+  const int64_t rows = n * G;
+  const int64_t slot = blockIdx.x / a.splits;
+  // the last rows see the most tokens: they go first
+  for (int64_t rt = a.row_tiles - 1 - slot; rt * kTileRows < rows; rt += a.row_tiles) {
+    const int64_t r0 = rt * kTileRows, w0 = r0 + wave * 32;
+    auto clip = [&](int64_t r) { return (r < rows ? r : rows - 1) / G; };
+    const Seen top = seen_by(a, length, n, r0 / G);
+    const Seen bot = seen_by(a, length, n, clip(r0 + kTileRows - 1));
+    const Seen wtop = seen_by(a, length, n, clip(w0)), wbot = seen_by(a, length, n, clip(w0 + 31));
+    const int64_t row = w0 + col;
+    const bool valid = row < rows;
+    const Seen me = seen_by(a, length, n, clip(row));
+    const int64_t begin = (top.lo & ~static_cast<int64_t>(kGroup - 1)) + split * a.chunk;
+    const int64_t end =
+        split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
+
+    v8h q[KC];
+    const T *qp = static_cast<const T *>(a.q) + (q0 + clip(row)) * a.stride_t +
+                  (head * static_cast<int64_t>(G) + (valid ? row % G : 0)) * a.stride_h;
+    const int e2 = load_query(
+        qp, valid, [&](int i) { return 16 * i + 8 * h; },
+        [](float v) { return nan_max(v, __shfl_xor(v, 32, kWave)); }, q);
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // the maximum is taken before the scale
+    const float q_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale), e2);
+
+    v16f acc[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f, ref = 1.0f;
+
+    uint4 kw[pieces], vw[pieces];
+    float ks = 0.0f, vs = 0.0f;
+    auto fetch = [&](int64_t t0) {
+#pragma unroll
+      for (int j = 0; j < pieces; ++j) {
+        const int i = tid + 256 * j;
+        {
+          const int64_t t = t0 + i / (D / 16);
+          const int64_t pg = t < bot.hi ? page_of(a.g, b, t >> shift) : 0;
+          kw[j] = *reinterpret_cast<const uint4 *>(
+              a.g.c.k + (((pg < 0 ? 0 : pg) * H + head) * P + (t & (P - 1))) * D + i % (D / 16) * 16);
+        }
+        {
+          const int64_t t = t0 + i % 4 * 16;
+          const int64_t pg = t < bot.hi ? page_of(a.g, b, t >> shift) : 0;
+          vw[j] = *reinterpret_cast<const uint4 *>(
+              a.g.c.v + (((pg < 0 ? 0 : pg) * H + head) * D + i / 4) * P + (t & (P - 1)));
+        }
+      }
+      if (tid < 4) {
+        const int64_t t = t0 + 16 * tid;
+        ks = vs = 0.0f;
+        if (t < bot.hi) {
+          const int64_t pg = page_of(a.g, b, t >> shift);
+          ks = pg < 0 ? nanf32() : a.g.c.k_scale[pg * H + head];
+          vs = pg < 0 ? nanf32() : a.g.c.v_scale[pg * H + head];
+        }
+      }
+    };
+    auto put = [&](Stage &s) {
+#pragma unroll
+      for (int j = 0; j < pieces; ++j) {
+        const int i = tid + 256 * j;
+        {
+          const int t = i / (D / 16), d = i % (D / 16) * 2;
+          const int r = (t & 32) + (t >> 4 & 1) * 4 + (t >> 2 & 3) * 8 + (t & 3);
+          s.k[d * kp + r] = __builtin_bit_cast(uint4, codes_f16(kw[j].x, kw[j].y));
+          s.k[(d + 1) * kp + r] = __builtin_bit_cast(uint4, codes_f16(kw[j].z, kw[j].w));
+        }
+        {
+          const int c = i % 4 * 2, d = i / 4;
+          s.v[c * vp + d] = __builtin_bit_cast(uint4, codes_f16(vw[j].x, vw[j].y));
+          s.v[(c + 1) * vp + d] = __builtin_bit_cast(uint4, codes_f16(vw[j].z, vw[j].w));
+        }
+      }
+      if (tid < 4) s.ks[tid] = ks, s.vs[tid] = vs;
+    };
+
+    if (begin < end) {
+      fetch(begin);
+      put(stage[0]);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t t0 = begin; t0 < end; t0 += kGroup, buf ^= 1) {
+      const bool more = t0 + kGroup < end;
+      if (more) fetch(t0 + kGroup);
+      if (t0 < wbot.hi && t0 + kGroup > wtop.lo && w0 < rows) {
+        const Stage &s = stage[buf];
+        v16f st[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) st[t][r] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < KC; ++c)
+            st[t] = mfma32_f16(
+                __builtin_bit_cast(v8h, s.k[(2 * c + h) * kp + 32 * t + col]), q[c], st[t]);
+        }
+        const bool whole = t0 >= wbot.lo && t0 + kGroup <= wtop.hi;
+        float f[2], high = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          f[t] = s.ks[2 * t + h] * q_scale;
+          if (!whole) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int64_t tok = t0 + 32 * t + 16 * h + r;
+              st[t][r] = tok >= me.lo && tok < me.hi ? sign * st[t][r] : -INFINITY;
+            }
+          } else if (sign < 0.0f) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[t][r] = -st[t][r];
+          }
+          float x = st[t][0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) x = fmaxf(x, st[t][r]);
+          if (x != -INFINITY) high = fmaxf(high, x * f[t]);
+        }
+        high = fmaxf(high, __shfl_xor(high, 32, kWave));
+        float big = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) big = fmaxf(big, s.vs[t]);
+        const bool turn = big > 0.0f && (big > ref || big * 8.0f < ref);
+        if (__any(high > m + 8.0f) || turn) {
+          const float was = m;
+          m = fmaxf(m, high);
+          float fix = exp2f(was - (m == -INFINITY ? 0.0f : m));
+          l *= fix;
+          if (turn) {
+            fix *= ref / big;
+            ref = big;
+          }
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[u][r] *= fix;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        v8h p[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float v = s.vs[2 * t + h];
+          const float ratio = v == v ? fmaxf(v / ref, 0x1p-40f) : v;  // below: rounds to 0 anyway
+          const float c = __log2f(ratio) - base;
+          float sum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float x = __builtin_fmaf(st[t][r], f[t], c);
+            if (!whole) x = st[t][r] == -INFINITY ? -INFINITY : x;
+            const float e = __builtin_amdgcn_exp2f(x);
+            sum += e;
+            p[2 * t + r / 8][r % 8] = static_cast<_Float16>(e);
+          }
+          l += sum == 0.0f ? 0.0f : sum / ratio;  // a NaN page counts where a token of it is seen
+        }
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            // weights c: tokens 32 (c / 2) + 16 h + 8 (c % 2) + 0..7
+            const int chunk = 4 * (c / 2) + 2 * h + c % 2;
+            acc[u] = mfma32_f16(__builtin_bit_cast(v8h, s.v[chunk * vp + 32 * u + col]), p[c], acc[u]);
+          }
+      }
+      if (more) put(stage[buf ^ 1]);
+      __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32, kWave);
+    if (valid) {
+      const int64_t place = (q0 + row / G) * a.q_heads + head * static_cast<int64_t>(G) + row % G;
+      const int64_t at = split * a.queries * a.q_heads + place;
+      const float f = a.splits > 1 ? ref : l == 0.0f ? 0.0f : ref / l;
+      if (a.splits > 1 && h == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
+      if (a.splits == 1 || begin < end) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int d = 32 * u + 8 * k + 4 * h;
+            struct {
+              T v[4];
+            } o;
+            v4f w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              w[e] = acc[u][4 * k + e] * f;
+              o.v[e] = static_cast<T>(w[e]);
+            }
+            if (a.splits > 1)
+              *reinterpret_cast<v4f *>(a.part + at * D + d) = w;
+            else
+              __builtin_memcpy(static_cast<T *>(a.out) + place * D + d, &o, sizeof(o));
+          }
+      }
+    }
+  }
+}
+
+// Joins the chunks of a row in the chunks' order: W waves take every W-th chunk, lane by lane of
+// the row.  A chunk in which the row sees nothing has l = 0 and its sums were never written.
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
-  const int lane = threadIdx.x % kWave;
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int64_t rows = a.queries * a.q_heads;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWave;
-  if (row >= rows) return;
-  float best = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) best = fmaxf(best, a.stats[2 * (s * rows + row)]);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWaves / W) + (W == 1 ? wave : 0);
+  if (row >= rows) return;  // whole workgroups where they meet at a barrier
+  float best = -INFINITY, total = 0.0f;
+  for (int s = lane; s < a.splits; s += kWave) best = fmaxf(best, a.stats[2 * (s * rows + row)]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) best = fmaxf(best, __shfl_xor(best, off, kWave));
   const float base = best == -INFINITY ? 0.0f : best;
-  float total = 0.0f, o[D / 64] = {};
-  for (int s = 0; s < a.splits; ++s) {
+  for (int s = lane; s < a.splits; s += kWave) {
+    const float *st = a.stats + 2 * (s * rows + row);
+    total += st[1] * exp2f(st[0] - base);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, kWave);
+  float o[E] = {};
+#pragma unroll 4
+  for (int s = W == 1 ? 0 : wave; s < a.splits; s += W) {
     const int64_t at = s * rows + row;
     const float l = a.stats[2 * at + 1], f = exp2f(a.stats[2 * at] - base);
-    if (l == 0.0f) continue;  // the chunk held nothing that the row sees (NaN is not 0)
-    total += l * f;
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] += a.part[at * D + 64 * e + lane] * f;
+    for (int e = 0; e < E; ++e) {
+      const float v = a.part[at * D + 64 * e + lane];
+      o[e] += l == 0.0f ? 0.0f : v * f;
+    }
+  }
+  if constexpr (W > 1) {
+    __shared__ float s_o[W][D];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_o[wave][64 * e + lane] = o[e];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int w = 1; w < W; ++w) o[e] += s_o[w][64 * e + lane];
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   T *out = static_cast<T *>(a.out) + row * D + lane;
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) out[64 * e] = static_cast<T>(o[e] * inv);
+  for (int e = 0; e < E; ++e) out[64 * e] = static_cast<T>(o[e] * inv);
 }
 
 struct Plan {
   int64_t row_tiles, chunk;
   int splits;
+  bool tile;  // attn_tile, else attn_rows
 };
 
 // Chunks of the token axis: enough workgroups to fill the GPU (four for each of 256 CUs), each
@@ -334,7 +602,9 @@ struct Plan {
 Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t max_query, int64_t max_length,
               int64_t window) {
   Plan p;
-  p.row_tiles = cdiv((max_query < 1 ? 1 : max_query) * group, kRows);
+  const int64_t rows = (max_query < 1 ? 1 : max_query) * group;
+  p.tile = rows >= 64;
+  p.row_tiles = cdiv(rows, p.tile ? kTileRows : kRows);
   int64_t span = max_length;
   if (window > 0 && window + max_query + kGroup < span) span = window + max_query + kGroup;
   const int64_t tiles = p.row_tiles * heads * seqs;
@@ -378,6 +648,7 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
                   "queries, max_query, max_length and window must be >= 0");
   RXMET_CHECK_ARG(max_query <= INT32_MAX && max_length <= INT32_MAX && queries <= INT32_MAX,
                   "lengths must be below 2^31");
+  RXMET_CHECK_ARG(queries * q_heads <= INT32_MAX, "too many query rows for one call");
   RXMET_CHECK_ARG(cu_query || queries == table->seqs,
                   "without cu_query there is one query a sequence");
   if (queries == 0 || table->seqs == 0) return 0;
@@ -397,9 +668,14 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
   prof::Scope scope("kv_attention", st);
   auto launch = [&](auto t, auto dim) {
     using T = decltype(t);
-    attn_rows<T, dim.value><<<grid, 256, 0, st>>>(a);
-    if (p.splits > 1)
-      attn_join<T, dim.value><<<static_cast<unsigned>(cdiv(rows, kWaves)), 256, 0, st>>>(a);
+    if (p.tile)
+      attn_tile<T, dim.value><<<grid, 256, 0, st>>>(a);
+    else
+      attn_rows<T, dim.value><<<grid, 256, 0, st>>>(a);
+    if (p.splits > 8)
+      attn_join<T, dim.value, kWaves><<<static_cast<unsigned>(rows), 256, 0, st>>>(a);
+    else if (p.splits > 1)
+      attn_join<T, dim.value, 1><<<static_cast<unsigned>(cdiv(rows, kWaves)), 256, 0, st>>>(a);
   };
   auto with_dim = [&](auto t) {
     switch (cache->dim) {
