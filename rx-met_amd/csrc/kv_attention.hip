@@ -36,14 +36,13 @@ constexpr int kWaves = 4;
 struct AttnArgs {
   Pages g;
   const int32_t *lengths, *cu;
-  int64_t queries;
+  int queries;
   const void *q;
   int64_t stride_t, stride_h;
   int q_heads, group;  // group = q_heads / heads
   float scale;         // with log2 e
   int causal;
-  int64_t window, chunk;
-  int splits, row_tiles;
+  int window, chunk, splits, row_tiles, cap;
   void *out;
   float *part, *stats;  // [splits, queries * q_heads, D] and [.., 2]: used where splits > 1
 };
@@ -71,6 +70,11 @@ __device__ __forceinline__ v4f mfma_f16(v8h a, v8h b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// The wave's number, known to be the same for all of its lanes.
+__device__ __forceinline__ int wave_id() {
+  return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+}
+
 // Over the four lanes that share a column.
 __device__ __forceinline__ float col_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, kWave));
@@ -81,16 +85,50 @@ __device__ __forceinline__ float col_sum(float v) {
   return v + __shfl_xor(v, 32, kWave);
 }
 
-// Tokens [lo, hi) that query i of n sees.
+// Most tokens of a sequence and most query rows of a call: sums of two of them stay in int32.
+constexpr int kMost = 1 << 29;
+
+// Tokens [lo, hi) that query i of n sees.  Of tokens past `cap` (the table's end) one is kept: it
+// has no page, and makes the row NaN.
 struct Seen {
-  int64_t lo, hi;
+  int lo, hi;
 };
-__device__ __forceinline__ Seen seen_by(const AttnArgs &a, int64_t length, int64_t n, int64_t i) {
-  const int64_t pos = length - n + i;
+__device__ __forceinline__ Seen seen_by(const AttnArgs &a, int length, int n, int i) {
+  const int pos = length - n + i;
   Seen s{0, length};
   if (a.causal && pos + 1 < s.hi) s.hi = pos + 1;
-  if (a.window > 0 && pos - a.window + 1 > 0) s.lo = pos - a.window + 1;
+  if (a.window > 0 && pos >= a.window) s.lo = pos - a.window + 1;
+  if (s.hi > a.cap + 1) {
+    if (s.lo > a.cap) s.lo = a.cap;
+    s.hi = a.cap + 1;
+  }
   return s;
+}
+
+// The sequence of a workgroup: its query rows (n queries of `group` heads) and its tokens.
+struct Sequence {
+  int length, q0, n, rows;
+};
+__device__ __forceinline__ Sequence sequence_of(const AttnArgs &a, int b) {
+  Sequence s;
+  s.length = a.lengths[b];
+  s.q0 = a.cu ? a.cu[b] : b;
+  s.n = a.cu ? a.cu[b + 1] - s.q0 : 1;
+  if (s.q0 < 0 || s.q0 >= a.queries) s.n = 0;
+  if (s.n > a.queries - s.q0) s.n = a.queries - s.q0;
+  s.rows = s.n > 0 ? s.n * a.group : 0;
+  return s;
+}
+
+// The id of the page that holds token t, as it stands in the table; -1 past the table, and 0 past
+// `end`, where nothing is seen and any page may be read.
+__device__ __forceinline__ int page_id(const AttnArgs &a, const int32_t *ids, int t, int end, int shift) {
+  if (t >= end) return 0;
+  const int p = t >> shift;
+  return p < a.g.t.cols ? ids[p] : -1;
+}
+__device__ __forceinline__ bool in_cache(const AttnArgs &a, int id) {
+  return static_cast<unsigned>(id) < static_cast<unsigned>(a.g.c.pages);
 }
 
 // Pieces of a query row (eight elements each, `at(i)` the place of piece i) as operands of the
@@ -129,31 +167,26 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
   constexpr int NC = D / 64, NU = D / 16, pitch = D + 4;
   __shared__ float s_acc[kWaves][kRows][pitch];
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = wave_id();
   const int col = lane % 16, g = lane / 16;
   const int split = blockIdx.x % a.splits, head = blockIdx.y, b = blockIdx.z;
   const int P = a.g.c.page_size, shift = __builtin_ctz(P), H = a.g.c.heads, G = a.group;
-  const int64_t length = a.lengths[b];
-  const int64_t q0 = a.cu ? a.cu[b] : b;
-  int64_t n = a.cu ? a.cu[b + 1] - q0 : 1;
-  if (q0 < 0) return;
-  if (n > a.queries - q0) n = a.queries - q0;
-  if (n <= 0) return;
-  const int64_t rows = n * G;
-  for (int64_t rt = blockIdx.x / a.splits; rt * kRows < rows; rt += a.row_tiles) {
-    const int64_t row = rt * kRows + col;
+  const Sequence seq = sequence_of(a, b);
+  const int rows = seq.rows;
+  const int32_t *ids = a.g.t.ids + b * a.g.t.stride;
+  for (int rt = blockIdx.x / a.splits; rt * kRows < rows; rt += a.row_tiles) {
+    const int row = rt * kRows + col;
     const bool valid = row < rows;
-    const Seen me = seen_by(a, length, n, valid ? row / G : n - 1);
-    const Seen top = seen_by(a, length, n, rt * kRows / G);  // the tile's first and last query
-    const int64_t last = rt * kRows + kRows - 1 < rows ? rt * kRows + kRows - 1 : rows - 1;
-    const Seen bot = seen_by(a, length, n, last / G);
-    const int64_t begin = (top.lo & ~static_cast<int64_t>(kGroup - 1)) + split * a.chunk;
-    const int64_t end =
-        split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
+    const Seen me = seen_by(a, seq.length, seq.n, valid ? row / G : seq.n - 1);
+    const Seen top = seen_by(a, seq.length, seq.n, rt * kRows / G);  // the tile's first and last query
+    const int last = rt * kRows + kRows - 1 < rows ? rt * kRows + kRows - 1 : rows - 1;
+    const Seen bot = seen_by(a, seq.length, seq.n, last / G);
+    const int begin = (top.lo & ~(kGroup - 1)) + split * a.chunk;
+    const int end = split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
 
     v8h q[2 * NC];
-    const T *qp = static_cast<const T *>(a.q) + (q0 + (valid ? row / G : 0)) * a.stride_t +
-                  (head * static_cast<int64_t>(G) + (valid ? row % G : 0)) * a.stride_h;
+    const T *qp = static_cast<const T *>(a.q) + (seq.q0 + (valid ? row / G : 0)) * a.stride_t +
+                  (head * G + (valid ? row % G : 0)) * a.stride_h;
     const int e2 = load_query(
         qp, valid, [&](int i) { return 64 * (i / 2) + 16 * g + 8 * (i % 2); },
         [](float v) {
@@ -168,27 +201,23 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
     for (int u = 0; u < NU; ++u) acc[u] = v4f{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f, ref = 1.0f, inv_ref = 1.0f;
 
-    for (int64_t t0 = begin + wave * kGroup; t0 < end; t0 += kWaves * kGroup) {
-      // the pages of this lane's key rows and of its sixteen tokens; past the end: any page
-      const int64_t tk = t0 + 16 * (col >> 2), tv = t0 + 16 * g;
-      const int64_t pk = tk < bot.hi ? page_of(a.g, b, tk >> shift) : 0;
-      const int64_t pv = tv < bot.hi ? page_of(a.g, b, tv >> shift) : 0;
-      const int64_t kat = (pk < 0 ? 0 : pk) * H + head, vat = (pv < 0 ? 0 : pv) * H + head;
+    auto step = [&](int t0, int ik, int iv) {  // one group of 64 tokens
+      const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * g;
+      const int64_t kat = static_cast<int64_t>(in_cache(a, ik) ? ik : 0) * H + head;
+      const int64_t vat = static_cast<int64_t>(in_cache(a, iv) ? iv : 0) * H + head;
       const int8_t *kp = a.g.c.k + kat * P * D + ((tk & (P - 1)) + (col & 3)) * D + 16 * g;
-      const int8_t *vp = a.g.c.v + vat * P * D + static_cast<int64_t>(col) * P + (tv & (P - 1));
+      const int8_t *vp = a.g.c.v + vat * P * D + col * P + (tv & (P - 1));
       uint4 kw[4][NC], vw[NU];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
           kw[t][c] = *reinterpret_cast<const uint4 *>(kp + 4 * t * D + 64 * c);
+      float ks = a.g.c.k_scale[vat], vs = a.g.c.v_scale[vat];
 #pragma unroll
       for (int u = 0; u < NU; ++u) vw[u] = *reinterpret_cast<const uint4 *>(vp + 16 * u * P);
-      float ks = 0.0f, vs = 0.0f;
-      if (tv < bot.hi) {
-        ks = pv < 0 ? nanf32() : a.g.c.k_scale[vat];
-        vs = pv < 0 ? nanf32() : a.g.c.v_scale[vat];
-      }
+      if (!in_cache(a, iv)) ks = vs = nanf32();
+      if (tv >= bot.hi) ks = vs = 0.0f;
 
       v4f s[4];
 #pragma unroll
@@ -201,30 +230,30 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
         }
       }
       const float f = ks * q_scale;
-      const bool whole = t0 >= bot.lo && t0 + kGroup <= top.hi;  // every row sees all 64
-      unsigned hidden = 0;  // bit 4 t + r: this row does not see the token
+      const float big = col_max(vs == vs ? vs : 0.0f);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) s[t] *= f;
+      if (t0 < bot.lo || t0 + kGroup > top.hi) {  // some row does not see all 64
+        asm volatile("");  // stays a branch: few groups need it
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int tok = tv + 4 * t + r;
+            s[t][r] = tok >= me.lo && tok < me.hi ? s[t][r] : -INFINITY;
+          }
+        if (tv + 16 <= me.lo || tv >= me.hi) vs = 0.0f;  // 0 times a hidden page's NaN is no 0
+      }
       float high = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[t][r] *= f;
-          if (!whole) {
-            const int64_t tok = tv + 4 * t + r;
-            if (tok < me.lo || tok >= me.hi) {
-              s[t][r] = -INFINITY;
-              hidden |= 1u << (4 * t + r);
-            }
-          }
-          high = fmaxf(high, s[t][r]);
-        }
+        for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][r]);
       high = fmaxf(m, col_max(high));
       const float base = high == -INFINITY ? 0.0f : high;
       const float alpha = exp2f(m - base);
       m = high;
-      // reference of the weights' rounding
-      const float big = col_max(vs == vs ? vs : 0.0f);
-      float fix = alpha;
+      float fix = alpha;  // and the reference of the weights' rounding
       if (big > 0.0f && (big > ref || big * 8.0f < ref)) {
         fix *= ref / big;
         ref = big;
@@ -243,17 +272,27 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = exp2f(s[t][r] - base);
+          const float e = __builtin_amdgcn_exp2f(s[t][r] - base);
           l += e;
-          const bool gone = hidden >> (4 * t + r) & 1;
-          p[t / 2][4 * (t % 2) + r] = gone ? static_cast<_Float16>(0.0f)
-                                           : static_cast<_Float16>(e * ratio);
+          p[t / 2][4 * (t % 2) + r] = static_cast<_Float16>(e * ratio);
         }
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         acc[u] = mfma_f16(codes_f16(vw[u].x, vw[u].y), p[0], acc[u]);
         acc[u] = mfma_f16(codes_f16(vw[u].z, vw[u].w), p[1], acc[u]);
       }
+    };
+    // the ids of a group's pages are on their way while the group before is computed
+    const int t_first = begin + wave * kGroup;
+    int ik = page_id(a, ids, t_first + 16 * (col >> 2), end, shift);
+    int iv = page_id(a, ids, t_first + 16 * g, end, shift);
+    for (int t0 = t_first; t0 < end; t0 += kWaves * kGroup) {
+      const int t1 = t0 + kWaves * kGroup;
+      const int nk = page_id(a, ids, t1 + 16 * (col >> 2), end, shift);
+      const int nv = page_id(a, ids, t1 + 16 * g, end, shift);
+      step(t0, ik, iv);
+      ik = nk;
+      iv = nv;
     }
 
     // the four waves' sums on one maximum
@@ -270,7 +309,7 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
     __syncthreads();
     constexpr int per = D / 16;  // elements of a thread: 16 threads a row
     const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * per;
-    const int64_t orow = rt * kRows + r;
+    const int orow = rt * kRows + r;
     if (orow < rows) {
       float best = s_m[0][r], total = 0.0f;
 #pragma unroll
@@ -278,7 +317,7 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w)
         total += s_l[w][r] * exp2f(s_m[w][r] - (best == -INFINITY ? 0.0f : best));
-      const int64_t place = (q0 + orow / G) * a.q_heads + head * static_cast<int64_t>(G) + orow % G;
+      const int64_t place = static_cast<int64_t>(seq.q0 + orow / G) * a.q_heads + head * G + orow % G;
       float o[per];
 #pragma unroll
       for (int e = 0; e < per; ++e)
@@ -290,7 +329,7 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
 #pragma unroll
         for (int e = 0; e < per; ++e) out[e] = static_cast<T>(o[e] * inv);
       } else {
-        const int64_t at = split * a.queries * a.q_heads + place;
+        const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;
         if (d0 == 0) a.stats[2 * at] = best, a.stats[2 * at + 1] = total;
         if (begin < end) {
           float *part = a.part + at * D + d0;
@@ -331,39 +370,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
     float ks[4], vs[4];   // of 16 tokens each
   };
   __shared__ Stage stage[2];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = wave_id();
   const int col = lane % 32, h = lane / 32;
   const int split = blockIdx.x % a.splits, head = blockIdx.y, b = blockIdx.z;
   const int P = a.g.c.page_size, shift = __builtin_ctz(P), H = a.g.c.heads, G = a.group;
-  const int64_t length = a.lengths[b];
-  const int64_t q0 = a.cu ? a.cu[b] : b;
-  int64_t n = a.cu ? a.cu[b + 1] - q0 : 1;
-  if (q0 < 0) return;
-  if (n > a.queries - q0) n = a.queries - q0;
-  if (n <= 0) return;
-  const int64_t rows = n * G;
-  const int64_t slot = blockIdx.x / a.splits;
+  const Sequence seq = sequence_of(a, b);
+  const int rows = seq.rows, slot = blockIdx.x / a.splits;
+  const int32_t *ids = a.g.t.ids + b * a.g.t.stride;
   // the last rows see the most tokens: they go first
-  for (int64_t rt = a.row_tiles - 1 - slot; rt * kTileRows < rows; rt += a.row_tiles) {
-    const int64_t r0 = rt * kTileRows, w0 = r0 + wave * 32;
-    auto clip = [&](int64_t r) { return (r < rows ? r : rows - 1) / G; };
-    const Seen top = seen_by(a, length, n, r0 / G);
-    const Seen bot = seen_by(a, length, n, clip(r0 + kTileRows - 1));
-    const Seen wtop = seen_by(a, length, n, clip(w0)), wbot = seen_by(a, length, n, clip(w0 + 31));
-    const int64_t row = w0 + col;
+  for (int rt = a.row_tiles - 1 - slot; rt * kTileRows < rows; rt += a.row_tiles) {
+    const int r0 = rt * kTileRows, w0 = r0 + wave * 32;
+    auto seen = [&](int r) { return seen_by(a, seq.length, seq.n, (r < rows ? r : rows - 1) / G); };
+    const Seen top = seen(r0), bot = seen(r0 + kTileRows - 1), wtop = seen(w0), wbot = seen(w0 + 31);
+    const int row = w0 + col;
     const bool valid = row < rows;
-    const Seen me = seen_by(a, length, n, clip(row));
-    const int64_t begin = (top.lo & ~static_cast<int64_t>(kGroup - 1)) + split * a.chunk;
-    const int64_t end =
-        split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
+    const Seen me = seen(row);
+    const int begin = (top.lo & ~(kGroup - 1)) + split * a.chunk;
+    const int end = split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
 
     v8h q[KC];
-    const T *qp = static_cast<const T *>(a.q) + (q0 + clip(row)) * a.stride_t +
-                  (head * static_cast<int64_t>(G) + (valid ? row % G : 0)) * a.stride_h;
+    const T *qp = static_cast<const T *>(a.q) + (seq.q0 + (valid ? row / G : 0)) * a.stride_t +
+                  (head * G + (valid ? row % G : 0)) * a.stride_h;
     const int e2 = load_query(
         qp, valid, [&](int i) { return 16 * i + 8 * h; },
         [](float v) { return nan_max(v, __shfl_xor(v, 32, kWave)); }, q);
-    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;  // the maximum is taken before the scale
+    if (a.scale < 0.0f) {  // the maximum is taken before the scale
+#pragma unroll
+      for (int c = 0; c < KC; ++c) q[c] = -q[c];
+    }
     const float q_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale), e2);
 
     v16f acc[NU];
@@ -371,35 +405,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f, ref = 1.0f;
+    float m = -INFINITY, l = 0.0f, ref = 1.0f, inv_ref = 1.0f;
 
+    // Staging.  Piece i = tid + 256 j: keys of token i / (D / 16), values of the 16 tokens i % 4.
     uint4 kw[pieces], vw[pieces];
     float ks = 0.0f, vs = 0.0f;
-    auto fetch = [&](int64_t t0) {
+    int ik[pieces], iv;
+    auto look_up = [&](int t0) {
+#pragma unroll
+      for (int j = 0; j < pieces; ++j)
+        ik[j] = page_id(a, ids, t0 + (tid + 256 * j) / (D / 16), end, shift);
+      iv = page_id(a, ids, t0 + tid % 4 * 16, end, shift);
+    };
+    auto fetch = [&](int t0) {
+      const int64_t vat = static_cast<int64_t>(in_cache(a, iv) ? iv : 0) * H + head;
+      const int tv = t0 + tid % 4 * 16;
 #pragma unroll
       for (int j = 0; j < pieces; ++j) {
-        const int i = tid + 256 * j;
-        {
-          const int64_t t = t0 + i / (D / 16);
-          const int64_t pg = t < bot.hi ? page_of(a.g, b, t >> shift) : 0;
-          kw[j] = *reinterpret_cast<const uint4 *>(
-              a.g.c.k + (((pg < 0 ? 0 : pg) * H + head) * P + (t & (P - 1))) * D + i % (D / 16) * 16);
-        }
-        {
-          const int64_t t = t0 + i % 4 * 16;
-          const int64_t pg = t < bot.hi ? page_of(a.g, b, t >> shift) : 0;
-          vw[j] = *reinterpret_cast<const uint4 *>(
-              a.g.c.v + (((pg < 0 ? 0 : pg) * H + head) * D + i / 4) * P + (t & (P - 1)));
-        }
+        const int i = tid + 256 * j, t = t0 + i / (D / 16);
+        const int64_t kat = static_cast<int64_t>(in_cache(a, ik[j]) ? ik[j] : 0) * H + head;
+        kw[j] = *reinterpret_cast<const uint4 *>(a.g.c.k + kat * P * D + (t & (P - 1)) * D +
+                                                 i % (D / 16) * 16);
+        vw[j] = *reinterpret_cast<const uint4 *>(a.g.c.v + vat * P * D + i / 4 * P + (tv & (P - 1)));
       }
       if (tid < 4) {
-        const int64_t t = t0 + 16 * tid;
-        ks = vs = 0.0f;
-        if (t < bot.hi) {
-          const int64_t pg = page_of(a.g, b, t >> shift);
-          ks = pg < 0 ? nanf32() : a.g.c.k_scale[pg * H + head];
-          vs = pg < 0 ? nanf32() : a.g.c.v_scale[pg * H + head];
-        }
+        ks = a.g.c.k_scale[vat];
+        vs = a.g.c.v_scale[vat];
+        if (!in_cache(a, iv)) ks = vs = nanf32();
+        if (tv >= end) ks = vs = 0.0f;
       }
     };
     auto put = [&](Stage &s) {
@@ -421,92 +454,104 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
       if (tid < 4) s.ks[tid] = ks, s.vs[tid] = vs;
     };
 
-    if (begin < end) {
-      fetch(begin);
-      put(stage[0]);
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int64_t t0 = begin; t0 < end; t0 += kGroup, buf ^= 1) {
-      const bool more = t0 + kGroup < end;
-      if (more) fetch(t0 + kGroup);
-      if (t0 < wbot.hi && t0 + kGroup > wtop.lo && w0 < rows) {
-        const Stage &s = stage[buf];
-        v16f st[2];
+    auto step = [&](int t0, const Stage &s) {  // one group of 64 tokens
+      v16f st[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[t][r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+          st[t] = mfma32_f16(__builtin_bit_cast(v8h, s.k[(2 * c + h) * kp + 32 * t + col]), q[c],
+                             st[t]);
+      }
+      float f[2], v[2], high = -INFINITY, big = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f[t] = s.ks[2 * t + h] * q_scale;
+        f[t] = f[t] < 0x1p-126f ? 0x1p-126f : f[t];  // so that -inf stays -inf
+        v[t] = s.vs[2 * t + h];
+      }
+      if (t0 < wbot.lo || t0 + kGroup > wtop.hi) {  // some row does not see all 64
+        asm volatile("");  // stays a branch: few groups need it
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+          const int t1 = t0 + 32 * t + 16 * h;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) st[t][r] = 0.0f;
-#pragma unroll
-          for (int c = 0; c < KC; ++c)
-            st[t] = mfma32_f16(
-                __builtin_bit_cast(v8h, s.k[(2 * c + h) * kp + 32 * t + col]), q[c], st[t]);
+          for (int r = 0; r < 16; ++r)
+            st[t][r] = t1 + r >= me.lo && t1 + r < me.hi ? st[t][r] : -INFINITY;
+          if (t1 + 16 <= me.lo || t1 >= me.hi) f[t] = v[t] = 1.0f;  // a hidden page's may be NaN
         }
-        const bool whole = t0 >= wbot.lo && t0 + kGroup <= wtop.hi;
-        float f[2], high = -INFINITY;
+      }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          f[t] = s.ks[2 * t + h] * q_scale;
-          if (!whole) {
+      for (int t = 0; t < 2; ++t) {
+        float x = st[t][0];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int64_t tok = t0 + 32 * t + 16 * h + r;
-              st[t][r] = tok >= me.lo && tok < me.hi ? sign * st[t][r] : -INFINITY;
-            }
-          } else if (sign < 0.0f) {
+        for (int r = 1; r < 16; ++r) x = fmaxf(x, st[t][r]);
+        high = fmaxf(high, x * f[t]);
+      }
+      high = fmaxf(high, __shfl_xor(high, 32, kWave));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) st[t][r] = -st[t][r];
-          }
-          float x = st[t][0];
-#pragma unroll
-          for (int r = 1; r < 16; ++r) x = fmaxf(x, st[t][r]);
-          if (x != -INFINITY) high = fmaxf(high, x * f[t]);
-        }
-        high = fmaxf(high, __shfl_xor(high, 32, kWave));
-        float big = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) big = fmaxf(big, s.vs[t]);
-        const bool turn = big > 0.0f && (big > ref || big * 8.0f < ref);
-        if (__any(high > m + 8.0f) || turn) {
-          const float was = m;
-          m = fmaxf(m, high);
-          float fix = exp2f(was - (m == -INFINITY ? 0.0f : m));
-          l *= fix;
-          if (turn) {
-            fix *= ref / big;
-            ref = big;
-          }
-#pragma unroll
-          for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[u][r] *= fix;
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-        v8h p[4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const float v = s.vs[2 * t + h];
-          const float ratio = v == v ? fmaxf(v / ref, 0x1p-40f) : v;  // below: rounds to 0 anyway
-          const float c = __log2f(ratio) - base;
-          float sum = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float x = __builtin_fmaf(st[t][r], f[t], c);
-            if (!whole) x = st[t][r] == -INFINITY ? -INFINITY : x;
-            const float e = __builtin_amdgcn_exp2f(x);
-            sum += e;
-            p[2 * t + r / 8][r % 8] = static_cast<_Float16>(e);
-          }
-          l += sum == 0.0f ? 0.0f : sum / ratio;  // a NaN page counts where a token of it is seen
+      for (int t = 0; t < 4; ++t) big = fmaxf(big, s.vs[t]);
+      const bool turn = big > 0.0f && (big > ref || big * 8.0f < ref);
+      if (__any(high > m + 8.0f) || turn) {
+        const float was = m;
+        m = fmaxf(m, high);
+        float fix = exp2f(was - (m == -INFINITY ? 0.0f : m));
+        l *= fix;
+        if (turn) {
+          fix *= ref / big;
+          ref = big;
+          inv_ref = 1.0f / big;
         }
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            // weights c: tokens 32 (c / 2) + 16 h + 8 (c % 2) + 0..7
-            const int chunk = 4 * (c / 2) + 2 * h + c % 2;
-            acc[u] = mfma32_f16(__builtin_bit_cast(v8h, s.v[chunk * vp + 32 * u + col]), p[c], acc[u]);
-          }
+          for (int r = 0; r < 16; ++r) acc[u][r] *= fix;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      v8h p[4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float ratio = v[t] * inv_ref;
+        ratio = ratio < 0x1p-40f ? 0x1p-40f : ratio;  // below that: rounds to 0 anyway
+        const float c = __builtin_amdgcn_logf(ratio) - base;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = __builtin_fmaf(st[t][r], f[t], c);
+          const float e = __builtin_amdgcn_exp2f(x);
+          sum += e;
+          p[2 * t + r / 8][r % 8] = static_cast<_Float16>(e);
+        }
+        l += sum * __builtin_amdgcn_rcpf(ratio);
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          // weights c: tokens 32 (c / 2) + 16 h + 8 (c % 2) + 0..7
+          const int chunk = 4 * (c / 2) + 2 * h + c % 2;
+          acc[u] = mfma32_f16(__builtin_bit_cast(v8h, s.v[chunk * vp + 32 * u + col]), p[c], acc[u]);
+        }
+    };
+
+    if (begin < end) {
+      look_up(begin);
+      fetch(begin);
+      look_up(begin + kGroup);
+      put(stage[0]);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int t0 = begin; t0 < end; t0 += kGroup, buf ^= 1) {
+      const bool more = t0 + kGroup < end;
+      if (more) {
+        fetch(t0 + kGroup);
+        look_up(t0 + 2 * kGroup);
+      }
+      if (t0 < wbot.hi && t0 + kGroup > wtop.lo && w0 < rows) {
+        step(t0, stage[buf]);
       }
       if (more) put(stage[buf ^ 1]);
       __syncthreads();
@@ -514,8 +559,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
 
     l += __shfl_xor(l, 32, kWave);
     if (valid) {
-      const int64_t place = (q0 + row / G) * a.q_heads + head * static_cast<int64_t>(G) + row % G;
-      const int64_t at = split * a.queries * a.q_heads + place;
+      const int64_t place = static_cast<int64_t>(seq.q0 + row / G) * a.q_heads + head * G + row % G;
+      const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;
       const float f = a.splits > 1 ? ref : l == 0.0f ? 0.0f : ref / l;
       if (a.splits > 1 && h == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
       if (a.splits == 1 || begin < end) {
@@ -548,8 +593,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
 template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
   constexpr int E = D / 64;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t rows = a.queries * a.q_heads;
+  const int lane = threadIdx.x % kWave, wave = wave_id();
+  const int64_t rows = static_cast<int64_t>(a.queries) * a.q_heads;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (kWaves / W) + (W == 1 ? wave : 0);
   if (row >= rows) return;  // whole workgroups where they meet at a barrier
   float best = -INFINITY, total = 0.0f;
@@ -599,8 +644,10 @@ struct Plan {
 
 // Chunks of the token axis: enough workgroups to fill the GPU (four for each of 256 CUs), each
 // with at least 512 tokens, eight groups, so that its start and its sums' join stay small beside them.
-Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t max_query, int64_t max_length,
-              int64_t window) {
+Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t queries, int64_t max_query,
+              int64_t max_length, int64_t window) {
+  if (max_query > queries) max_query = queries;
+  if (max_length > kMost) max_length = kMost;
   Plan p;
   const int64_t rows = (max_query < 1 ? 1 : max_query) * group;
   p.tile = rows >= 64;
@@ -629,7 +676,8 @@ extern "C" int64_t rxmet_kv_attention_workspace_bytes(const rxmet_kv_cache *cach
                                                       int64_t max_query, int64_t max_length,
                                                       int64_t window) {
   if (!cache || cache->heads < 1 || q_heads < cache->heads || queries <= 0 || seqs <= 0) return 0;
-  const Plan p = plan_for(cache->heads, seqs, q_heads / cache->heads, max_query, max_length, window);
+  const Plan p = plan_for(cache->heads, seqs, q_heads / cache->heads, queries, max_query,
+                          max_length, window);
   return p.splits == 1 ? 0 : p.splits * queries * q_heads * (cache->dim + 2) * 4;
 }
 
@@ -648,20 +696,25 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
                   "queries, max_query, max_length and window must be >= 0");
   RXMET_CHECK_ARG(max_query <= INT32_MAX && max_length <= INT32_MAX && queries <= INT32_MAX,
                   "lengths must be below 2^31");
-  RXMET_CHECK_ARG(queries * q_heads <= INT32_MAX, "too many query rows for one call");
+  RXMET_CHECK_ARG(queries * q_heads <= kMost, "too many query rows for one call");
   RXMET_CHECK_ARG(cu_query || queries == table->seqs,
                   "without cu_query there is one query a sequence");
   if (queries == 0 || table->seqs == 0) return 0;
   RXMET_CHECK_ARG(lengths && query && out, "lengths, query and out are needed");
   const int group = q_heads / cache->heads;
-  const Plan p = plan_for(cache->heads, table->seqs, group, max_query, max_length, window);
+  int64_t cap = static_cast<int64_t>(table->cols) * cache->page_size;
+  if (cap > kMost) cap = kMost;
+  const Plan p = plan_for(cache->heads, table->seqs, group, queries, max_query, max_length, window);
+  if (window > INT32_MAX) window = 0;  // hides nothing
   RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
   RXMET_CHECK_ARG(p.row_tiles * p.splits <= INT32_MAX, "too many query rows for one call");
   const int64_t rows = queries * q_heads;
   float *part = static_cast<float *>(workspace);
-  const AttnArgs a{{*cache, *table}, lengths, cu_query, queries, query, query_stride_t,
-                   query_stride_h, q_heads, group, scale * 1.44269504088896340736f, causal, window,
-                   p.chunk, p.splits, static_cast<int>(p.row_tiles), out, part,
+  const AttnArgs a{{*cache, *table}, lengths, cu_query, static_cast<int>(queries), query,
+                   query_stride_t, query_stride_h, q_heads, group,
+                   scale * 1.44269504088896340736f, causal, static_cast<int>(window),
+                   static_cast<int>(p.chunk), p.splits, static_cast<int>(p.row_tiles),
+                   static_cast<int>(cap), out, part,
                    part ? part + p.splits * rows * cache->dim : nullptr};
   auto st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(p.row_tiles * p.splits), cache->heads, table->seqs);
