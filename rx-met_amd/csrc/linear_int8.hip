@@ -25,6 +25,8 @@ struct LinArgs {
   void *y;
   int64_t M, N;
   int K, act;
+  int *part;        // [splits, M, N] sums of a part of K each, where splits > 1
+  int splits, run;  // run: steps of K of a part
 };
 
 __device__ __forceinline__ float activate(float v, int act) {
@@ -113,8 +115,22 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few(const LinArgs a) {
   v4i acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = v4i{0, 0, 0, 0};
+  int k0 = wave * 128;
 #pragma unroll 4
-  for (int k0 = wave * 128; k0 < a.K; k0 += kFewWaves * 128) {
+  for (; k0 + 128 <= a.K; k0 += kFewWaves * 128) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int k = k0 + 64 * c + 16 * g;
+      v4i wf, xf;
+      __builtin_memcpy(&wf, w + k, 16);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        __builtin_memcpy(&xf, x[t] + k, 16);
+        acc[t] = mfma_i8(wf, xf, acc[t]);
+      }
+    }
+  }
+  if (k0 < a.K) {  // K ends in this run
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int k = k0 + 64 * c + 16 * g;
@@ -139,88 +155,235 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few(const LinArgs a) {
   }
 }
 
-// Tiles of 128 weight rows x 128 token rows, 128 of K at a time through LDS; four waves take
-// 64 x 64 each.  A row's eight 16-byte pieces lie at the places (piece ^ f(row)), so that the 16 lanes that
-// read one piece of 16 rows find it in 16 different bank groups.
-constexpr int kTile = 128, kStep = 128;
+// ---------------------------------------------------------------------------------------------
+// Tiles of TN weight rows x TM token rows on mfma 32x32x32; WN x WM waves take equal parts.
+//
+// K goes through LDS in steps of 64 bytes.  A row's four 16-byte pieces lie at the places
+// piece ^ f(row), so that 16 lanes that read one piece of 16 rows meet 16 different bank groups.
+// Row i of a wave's 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4: a lane
+// holds 16 consecutive n of one m.  ASYNC (rows of whole aligned pieces): memory -> LDS without
+// registers, three steps ahead in a ring of four; else through registers, one step ahead.
+constexpr int kStep = 64;
 
-__device__ __forceinline__ int place_w(int row, int piece) {
-  return (row * 8 + (piece ^ ((row >> 1 & 1) | (row >> 4 & 3) << 1))) * 16;
-}
-__device__ __forceinline__ int place_x(int row, int piece) {
-  return (row * 8 + (piece ^ (row >> 1 & 7))) * 16;
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+// f of a weight row and of a token row
+__device__ __forceinline__ int turn_w(int row) { return (row >> 2 & 1) | (row >> 3 & 2); }
+__device__ __forceinline__ int turn_x(int row) { return row >> 2 & 3; }
+
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>(p));  // the aperture is the high half
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void linear_tile(const LinArgs a) {
-  __shared__ __attribute__((aligned(16))) int8_t s[2][2][kTile * kStep];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int col = lane % 16, g = lane / 16;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kTile, m0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  // staging: thread takes piece tid % 8 of rows tid / 8 + 32 j
-  const int8_t *wp[4], *xp[4];
+// 16 bytes of each lane's address to LDS at `lds` + 16 * lane, in flight until vmcnt says so.
+__device__ __forceinline__ void load_to_lds(const int8_t *p, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(p)
+               : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+template <typename T, int TN, int TM, int WN, int WM, bool ASYNC>
+__global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
+  constexpr int threads = 64 * WN * WM;
+  constexpr int FN = TN / WN / 32, FM = TM / WM / 32;
+  constexpr int bytes = (TN + TM) * kStep;
+  constexpr int ring = ASYNC ? 4 : 2;
+  constexpr int loads = bytes / 16 / threads;  // pieces of a thread in a step
+  __shared__ __attribute__((aligned(16))) int8_t s[ring][bytes];
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int col = lane % 32, h = lane / 32;
+  const int tiles_n = static_cast<int>((a.N + TN - 1) / TN);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x % tiles_n) * TN;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.x / tiles_n) * TM;
+  // the steps of this part of K; the last part also takes the one that K ends in
+  const int split = blockIdx.y, from = split * a.run;
+  const bool last = split == a.splits - 1;
+  const int all = a.K / kStep, whole = last ? all - from : a.run;
+
+  // piece j of a thread lies at place tid + threads * j of the step, which holds this piece of a row
+  const int8_t *src[loads];
+  auto piece_at = [&](int j) {
+    const int at = tid + threads * j, row = at / 4;
+    return (at % 4) ^ (row < TN ? turn_w(row) : turn_x(row - TN));
+  };
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = tid / 8 + 32 * j;
-    wp[j] = a.w + (n0 + r < a.N ? n0 + r : a.N - 1) * a.w_stride;
-    xp[j] = a.x + (m0 + r < a.M ? m0 + r : a.M - 1) * a.x_stride;
+  for (int j = 0; j < loads; ++j) {
+    const int row = (tid + threads * j) / 4;
+    if (row < TN) {
+      const int64_t n = n0 + row < a.N ? n0 + row : a.N - 1;
+      src[j] = a.w + n * a.w_stride;
+    } else {
+      const int64_t m = m0 + row - TN < a.M ? m0 + row - TN : a.M - 1;
+      src[j] = a.x + m * a.x_stride;
+    }
+    src[j] += piece_at(j) * 16 + from * kStep;
   }
-  uint4 wr[4], xr[4];
-  auto fetch = [&](int k0) {
-    const int k = k0 + 16 * (tid % 8);
+  v16i acc[FN][FM];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      wr[j] = load_piece(wp[j], k, a.K);
-      xr[j] = load_piece(xp[j], k, a.K);
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+  const int wn = wave % WN * (TN / WN), wm = wave / WN * (TM / WM);
+  int wat[FN][2], xat[FM][2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int row = wn + 32 * i + 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
+      wat[i][c] = row * kStep + ((2 * c + h) ^ turn_w(row)) * 16;
     }
-  };
-  auto put = [&](int buf) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = tid / 8 + 32 * j;
-      *reinterpret_cast<uint4 *>(&s[buf][0][place_w(r, tid % 8)]) = wr[j];
-      *reinterpret_cast<uint4 *>(&s[buf][1][place_x(r, tid % 8)]) = xr[j];
+    for (int j = 0; j < FM; ++j) {
+      const int row = wm + 32 * j + col;
+      xat[j][c] = (TN + row) * kStep + ((2 * c + h) ^ turn_x(row)) * 16;
     }
-  };
-  v4i acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
-  const int wn = wave % 2 * 64, wm = wave / 2 * 64;
-  fetch(0);
-  put(0);
-  __syncthreads();
-  int buf = 0;
-  for (int k0 = 0; k0 < a.K; k0 += kStep, buf ^= 1) {
-    const bool more = k0 + kStep < a.K;
-    if (more) fetch(k0 + kStep);
+  }
+  auto compute = [&](const int8_t *buf) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      v4i wf[4], xf[4];
+      v4i wf[FN], xf[FM];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int r = wn + 16 * (col >> 2) + 4 * t + (col & 3);
-        wf[t] = as_v4i(*reinterpret_cast<const uint4 *>(&s[buf][0][place_w(r, 4 * c + g)]));
-        xf[t] = as_v4i(*reinterpret_cast<const uint4 *>(&s[buf][1][place_x(wm + 16 * t + col, 4 * c + g)]));
-      }
+      for (int i = 0; i < FN; ++i) wf[i] = *reinterpret_cast<const v4i *>(buf + wat[i][c]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < FM; ++j) xf[j] = *reinterpret_cast<const v4i *>(buf + xat[j][c]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma_i8(wf[i], xf[j], acc[i][j]);
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
     }
-    if (more) put(buf ^ 1);
+  };
+  // a step through registers
+  uint4 reg[loads];
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int j = 0; j < loads; ++j) __builtin_memcpy(&reg[j], src[j] + step * kStep, 16);
+  };
+  auto fetch_end = [&](int step) {
+#pragma unroll
+    for (int j = 0; j < loads; ++j) {
+      const int k = step * kStep + 16 * piece_at(j);
+      reg[j] = load_piece(src[j] + step * kStep - k, k, a.K - from * kStep);
+    }
+  };
+  auto put = [&](int8_t *buf) {
+#pragma unroll
+    for (int j = 0; j < loads; ++j)
+      *reinterpret_cast<uint4 *>(buf + 16 * (tid + threads * j)) = reg[j];
+  };
+  if constexpr (ASYNC) {
+    const unsigned base = lds_address(&s[0][0]) + wave * 1024;
+    auto issue = [&](int step, int slot) {
+#pragma unroll
+      for (int j = 0; j < loads; ++j)
+        load_to_lds(src[j] + step * kStep, base + slot * bytes + j * threads * 16);
+    };
+    if (whole > 0) {
+      // past the end a step is read once more, so that the count of loads in flight holds
+#pragma unroll
+      for (int k = 0; k < ring - 1; ++k) issue(k < whole ? k : 0, k);
+      for (int k = 0; k < whole; ++k) {
+        wait_loads<(ring - 2) * loads>();
+        __syncthreads();  // step k is there for all, and step k - 1 has been read by all
+        issue(k + ring - 1 < whole ? k + ring - 1 : k, (k + ring - 1) % ring);
+        compute(s[k % ring]);
+      }
+      wait_loads<0>();
+    }
+  } else {
+    if (whole > 0) {
+      fetch(0);
+      put(s[0]);
+    }
+    for (int k = 0; k < whole; ++k) {
+      __syncthreads();
+      if (k + 1 < whole) fetch(k + 1);
+      compute(s[k & 1]);
+      if (k + 1 < whole) put(s[(k + 1) & 1]);
+    }
+  }
+  if (last && all * kStep < a.K) {
+    fetch_end(whole);
     __syncthreads();
+    put(s[0]);
+    __syncthreads();
+    compute(s[0]);
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    int v[16];
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < FM; ++j) {
+      int v[16];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[4 * i + r] = acc[i][j][r];
-    finish<T, 16>(a, m0 + wm + 16 * j + col, n0 + wn + 16 * g, v);
+      for (int r = 0; r < 16; ++r) v[r] = acc[i][j][r];
+      const int64_t m = m0 + wm + 32 * j + col, n = n0 + wn + 32 * i + 16 * h;
+      if (a.splits == 1) {
+        finish<T, 16>(a, m, n, v);
+      } else if (m < a.M) {
+        int *p = a.part + (split * a.M + m) * a.N + n;
+        if (n + 16 <= a.N) {
+          __builtin_memcpy(p, v, sizeof(v));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (n + r < a.N) p[r] = v[r];
+        }
+      }
+    }
+}
+
+// Adds the parts of K up and finishes four n of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join(const LinArgs a) {
+  const int64_t quads = (a.N + 3) / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= a.M * quads) return;
+  const int64_t m = i / quads, n = i % quads * 4;
+  const int left = a.N - n < 4 ? static_cast<int>(a.N - n) : 4;
+  int v[4] = {0, 0, 0, 0};
+  for (int s = 0; s < a.splits; ++s) {
+    const int *p = a.part + (s * a.M + m) * a.N + n;
+    int u[4] = {0, 0, 0, 0};
+    if (left == 4) {
+      __builtin_memcpy(u, p, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) u[e] = p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += u[e];
   }
+  finish<T, 4>(a, m, n, v);
+}
+
+struct Plan {
+  bool few, big;
+  int splits, run;
+};
+
+Plan plan_for(int64_t M, int64_t N, int64_t K) {
+  Plan p{M <= 64, false, 1, 0};
+  const int64_t steps = K / kStep;
+  p.big = cdiv(M, 256) * cdiv(N, 256) >= 192;
+  const int64_t tiles = cdiv(M, 128) * cdiv(N, 128);
+  if (!p.few && !p.big && tiles < 256) {
+    int64_t splits = cdiv(512, tiles);
+    if (splits > steps / 8) splits = steps / 8;
+    if (splits > 1) {
+      p.run = static_cast<int>(cdiv(steps, splits));
+      p.splits = static_cast<int>(cdiv(steps, p.run));
+    }
+  }
+  return p;
 }
 
 }  // namespace
@@ -230,7 +393,11 @@ __global__ __launch_bounds__(256) void linear_tile(const LinArgs a) {
 using namespace rxmet;
 using namespace rxmet::dec;
 
-extern "C" int64_t rxmet_linear_int8_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t rxmet_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const Plan p = plan_for(M, N, K);
+  return p.splits > 1 ? p.splits * M * N * 4 : 0;
+}
 
 extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, const float *scales,
                                  const int8_t *weight, int64_t weight_stride,
@@ -238,7 +405,6 @@ extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, cons
                                  const void *residual, int64_t residual_stride, void *y, int64_t M,
                                  int64_t N, int64_t K, int32_t activation, int32_t dtype,
                                  void *workspace, void *stream) {
-  (void)workspace;
   RXMET_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && K <= RXMET_LINEAR_INT8_K_MAX,
                   "M must be >= 0, N >= 1 and K between 1 and 131071");
   RXMET_CHECK_ARG(M <= INT32_MAX && N <= INT32_MAX, "M and N must be below 2^31");
@@ -249,20 +415,34 @@ extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, cons
   if (M == 0) return 0;
   RXMET_CHECK_ARG(codes && scales && weight && weight_scales && y,
                   "codes, weight, their scales and y are needed");
+  RXMET_CHECK_ARG(cdiv(M, 128) * cdiv(N, 128) <= INT32_MAX / 64, "too many outputs for one call");
+  const Plan p = plan_for(M, N, K);
+  RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
   const LinArgs a{codes, weight, codes_stride, weight_stride, scales, weight_scales, bias,
-                  residual, residual_stride, y, M, N, static_cast<int>(K), activation};
+                  residual, residual_stride, y, M, N, static_cast<int>(K), activation,
+                  static_cast<int *>(workspace), p.splits, p.run};
+  const bool whole = (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(weight) |
+                      static_cast<uintptr_t>(codes_stride) |
+                      static_cast<uintptr_t>(weight_stride)) % 16 == 0;
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("linear_int8", st);
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (M <= 64) {
+    if (p.few) {
       const unsigned grid = static_cast<unsigned>(cdiv(N, 16));
       if (M <= 16) linear_few<T, 1><<<grid, 64 * kFewWaves, 0, st>>>(a);
       else if (M <= 32) linear_few<T, 2><<<grid, 64 * kFewWaves, 0, st>>>(a);
       else linear_few<T, 4><<<grid, 64 * kFewWaves, 0, st>>>(a);
+    } else if (p.big) {
+      const unsigned grid = static_cast<unsigned>(cdiv(N, 256) * cdiv(M, 256));
+      if (whole) linear_tile<T, 256, 256, 2, 4, true><<<grid, 512, 0, st>>>(a);
+      else linear_tile<T, 256, 256, 2, 4, false><<<grid, 512, 0, st>>>(a);
     } else {
-      const dim3 grid(static_cast<unsigned>(cdiv(N, kTile)), static_cast<unsigned>(cdiv(M, kTile)));
-      linear_tile<T><<<grid, 256, 0, st>>>(a);
+      const dim3 grid(static_cast<unsigned>(cdiv(N, 128) * cdiv(M, 128)), p.splits);
+      if (whole) linear_tile<T, 128, 128, 2, 2, true><<<grid, 256, 0, st>>>(a);
+      else linear_tile<T, 128, 128, 2, 2, false><<<grid, 256, 0, st>>>(a);
+      if (p.splits > 1)
+        linear_join<T><<<static_cast<unsigned>(cdiv(M * cdiv(N, 4), 256)), 256, 0, st>>>(a);
     }
   });
   RXMET_CHECK_LAUNCH();
