@@ -58,7 +58,7 @@ def activation(v, act):
 
 def linear(codes, scales, weight, weight_scales, bias, act, residual):
     """(y, magnitude of what was added up for it)."""
-    acc = codes.astype(np.int64) @ weight.astype(np.int64).T
+    acc = codes.astype(np.float64) @ weight.astype(np.float64).T  # whole numbers below 2^53: exact
     v = acc * np.asarray(scales, np.float64)[:, None] * np.asarray(weight_scales, np.float64)
     size = np.abs(v)
     if bias is not None:

@@ -94,64 +94,60 @@ __device__ __forceinline__ void finish(const LinArgs &a, int64_t m, int64_t n0, 
   }
 }
 
-// Few rows of x: a workgroup takes 16 weight rows and all of K, its eight waves take runs of 128
-// of K in turn; the weights go from memory into the matrix instruction with no stop in LDS.
-constexpr int kFewWaves = 8;
+// ---------------------------------------------------------------------------------------------
+// At most 16 rows of x: a workgroup takes 16 weight rows and all of K, its eight waves take runs
+// of 128 of K in turn; the weights go from memory into the matrix instruction with no stop in
+// LDS.  The eight sums meet in LDS, so there is one launch.
+//
+// Bound: the weights' bytes, and below some 20 MB the launch and one trip to memory.  [16, 4096] x
+// [4096, 4096]: 7.0 us (17 MB: 3.4 us at the copy rate); 32 or 64 weight rows a workgroup, which read x
+// less often, 8.8 and 11.5 us; tiles of 64 x 32 with K in four parts 8.9 us.
+constexpr int kFewRows = 16, kFewWaves = 8;
 
-template <typename T, int MT>
+template <typename T>
 __global__ __launch_bounds__(64 * kFewWaves) void linear_few(const LinArgs a) {
-  __shared__ int s[kFewWaves][MT * 16][20];
+  __shared__ int s[kFewWaves][kFewRows][20];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int col = lane % 16, g = lane / 16;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int64_t nrow = n0 + col < a.N ? n0 + col : a.N - 1;
-  const int8_t *w = a.w + nrow * a.w_stride;
-  const int8_t *x[MT];
+  const int8_t *w = a.w + (n0 + col < a.N ? n0 + col : a.N - 1) * a.w_stride;
+  const int8_t *x = a.x + (col < a.M ? col : a.M - 1) * a.x_stride;
+  v4i acc = {0, 0, 0, 0};
+  constexpr int turn = kFewWaves * 128;  // from a wave's run of K to its next
+  auto runs = [&](auto N, int k0) {      // N of them, all their loads before the first product
+    v4i wf[N.value][2], xf[N.value][2];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int64_t m = t * 16 + col < a.M ? t * 16 + col : a.M - 1;
-    x[t] = a.x + m * a.x_stride;
-  }
-  v4i acc[MT];
+    for (int i = 0; i < N.value; ++i)
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = v4i{0, 0, 0, 0};
-  int k0 = wave * 128;
-#pragma unroll 4
-  for (; k0 + 128 <= a.K; k0 += kFewWaves * 128) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int k = k0 + 64 * c + 16 * g;
-      v4i wf, xf;
-      __builtin_memcpy(&wf, w + k, 16);
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        __builtin_memcpy(&xf, x[t] + k, 16);
-        acc[t] = mfma_i8(wf, xf, acc[t]);
+      for (int c = 0; c < 2; ++c) {
+        const int k = k0 + turn * i + 64 * c + 16 * g;
+        __builtin_memcpy(&wf[i][c], w + k, 16);
+        __builtin_memcpy(&xf[i][c], x + k, 16);
       }
-    }
-  }
+#pragma unroll
+    for (int i = 0; i < N.value; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) acc = mfma_i8(wf[i][c], xf[i][c], acc);
+  };
+  int k0 = wave * 128;
+  for (; k0 + 3 * turn + 128 <= a.K; k0 += 4 * turn) runs(std::integral_constant<int, 4>{}, k0);
+  for (; k0 + 128 <= a.K; k0 += turn) runs(std::integral_constant<int, 1>{}, k0);
   if (k0 < a.K) {  // K ends in this run
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int k = k0 + 64 * c + 16 * g;
-      const v4i wf = as_v4i(load_piece(w, k, a.K));
-#pragma unroll
-      for (int t = 0; t < MT; ++t) acc[t] = mfma_i8(wf, as_v4i(load_piece(x[t], k, a.K)), acc[t]);
+      acc = mfma_i8(as_v4i(load_piece(w, k, a.K)), as_v4i(load_piece(x, k, a.K)), acc);
     }
   }
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s[wave][t * 16 + col][4 * g + r] = acc[t][r];
+  *reinterpret_cast<v4i *>(&s[wave][col][4 * g]) = acc;
   __syncthreads();
-  for (int i = threadIdx.x; i < MT * 16 * 4; i += 64 * kFewWaves) {
-    const int m = i / 4, n = i % 4 * 4;
-    int sum[4] = {0, 0, 0, 0};
+  if (threadIdx.x < kFewRows * 4) {
+    const int m = threadIdx.x / 4, n = threadIdx.x % 4 * 4;
+    v4i sum = *reinterpret_cast<const v4i *>(&s[0][m][n]);
 #pragma unroll
-    for (int v = 0; v < kFewWaves; ++v)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += s[v][m][n + e];
-    finish<T, 4>(a, m, n0 + n, sum);
+    for (int v = 1; v < kFewWaves; ++v) sum += *reinterpret_cast<const v4i *>(&s[v][m][n]);
+    const int r[4] = {sum[0], sum[1], sum[2], sum[3]};
+    finish<T, 4>(a, m, n0 + n, r);
   }
 }
 
@@ -171,20 +167,20 @@ typedef int v16i __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ int turn_w(int row) { return (row >> 2 & 1) | (row >> 3 & 2); }
 __device__ __forceinline__ int turn_x(int row) { return row >> 2 & 3; }
 
-__device__ __forceinline__ unsigned lds_address(const void *p) {
-  return static_cast<unsigned>(reinterpret_cast<uintptr_t>(p));  // the aperture is the high half
-}
-
 // 16 bytes of each lane's address to LDS at `lds` + 16 * lane, in flight until vmcnt says so.
-__device__ __forceinline__ void load_to_lds(const int8_t *p, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(lds), "v"(p)
-               : "memory", "m0");
+__device__ __forceinline__ void load_to_lds(const int8_t *p, int8_t *lds) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) void *)p,
+      (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+// A barrier that lets loads to LDS stay in flight (__syncthreads waits for them).  What this wave
+// wrote to or read from LDS before it is done.
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
 template <typename T, int TN, int TM, int WN, int WM, bool ASYNC>
@@ -199,8 +195,21 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 32, h = lane / 32;
   const int tiles_n = static_cast<int>((a.N + TN - 1) / TN);
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x % tiles_n) * TN;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x / tiles_n) * TM;
+  const int tiles_m = static_cast<int>((a.M + TM - 1) / TM);
+  int tn = blockIdx.x % tiles_n, tm = blockIdx.x / tiles_n;
+  if constexpr (TN * TM >= 256 * 128) {
+    // Workgroups go to the eight XCDs in turn: each XCD gets a run of the tiles' order, in which
+    // bands of four tiles of x go through the weights together, so that its L2 holds what they share
+    // (8192^3: 598 us; row by row, over all XCDs: 624 us).
+    const int total = tiles_n * tiles_m, per = total / 8, rest = total % 8;
+    const int xcd = blockIdx.x % 8;
+    const int id = xcd * per + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    const int first = id / (4 * tiles_n) * 4, in = id - first * tiles_n;
+    const int high = tiles_m - first < 4 ? tiles_m - first : 4;
+    tm = first + in % high;
+    tn = in / high;
+  }
+  const int64_t n0 = static_cast<int64_t>(tn) * TN, m0 = static_cast<int64_t>(tm) * TM;
   // the steps of this part of K; the last part also takes the one that K ends in
   const int split = blockIdx.y, from = split * a.run;
   const bool last = split == a.splits - 1;
@@ -280,11 +289,10 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
       *reinterpret_cast<uint4 *>(buf + 16 * (tid + threads * j)) = reg[j];
   };
   if constexpr (ASYNC) {
-    const unsigned base = lds_address(&s[0][0]) + wave * 1024;
     auto issue = [&](int step, int slot) {
 #pragma unroll
       for (int j = 0; j < loads; ++j)
-        load_to_lds(src[j] + step * kStep, base + slot * bytes + j * threads * 16);
+        load_to_lds(src[j] + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
     };
     if (whole > 0) {
       // past the end a step is read once more, so that the count of loads in flight holds
@@ -292,7 +300,7 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
       for (int k = 0; k < ring - 1; ++k) issue(k < whole ? k : 0, k);
       for (int k = 0; k < whole; ++k) {
         wait_loads<(ring - 2) * loads>();
-        __syncthreads();  // step k is there for all, and step k - 1 has been read by all
+        meet();  // step k is there for all, and step k - 1 has been read by all
         issue(k + ring - 1 < whole ? k + ring - 1 : k, (k + ring - 1) % ring);
         compute(s[k % ring]);
       }
@@ -365,25 +373,46 @@ __global__ __launch_bounds__(256) void linear_join(const LinArgs a) {
   finish<T, 4>(a, m, n, v);
 }
 
+// How a call is run: linear_few up to 16 rows; else the largest tile of which there is one for
+// each of 256 CUs, because a step costs much the same for every tile ([1024, 4096] x [4096, 4096]: 128 x 128
+// 32 us, 64 x 128 36, 256 x 256 79; [512, ..]: 64 x 128 20 us, 128 x 128 29; [256, ..]: 64 x 64 13 us,
+// 64 x 128 18; [2048, ..]: 256 x 128 48 us, 128 x 128 54); where even the smallest tiles are fewer, K is cut
+// into parts of at least 16 steps ([64, 4096] x [4096, 12288]: four parts 19 us, one 42).
+enum Shape { kFew, k64x32, k64x64, k64x128, k128x128, k256x128, k256x256 };
+
 struct Plan {
-  bool few, big;
+  Shape shape;
   int splits, run;
 };
 
-Plan plan_for(int64_t M, int64_t N, int64_t K) {
-  Plan p{M <= 64, false, 1, 0};
+// `whole`: rows of aligned 16-byte pieces; the others have fewer shapes.
+Plan plan_for(int64_t M, int64_t N, int64_t K, bool whole) {
+  if (M <= kFewRows) return {kFew, 1, 0};
+  auto tiles = [&](int64_t tn, int64_t tm) { return cdiv(N, tn) * cdiv(M, tm); };
+  if (M > 64) {
+    if (whole && tiles(256, 256) >= 256) return {k256x256, 1, 0};
+    if (whole && tiles(256, 128) >= 256) return {k256x128, 1, 0};
+    if (tiles(128, 128) >= 256) return {k128x128, 1, 0};
+    if (whole && tiles(64, 128) >= 256) return {k64x128, 1, 0};
+  }
+  Plan p{whole && M <= 32 ? k64x32 : k64x64, 1, 0};
   const int64_t steps = K / kStep;
-  p.big = cdiv(M, 256) * cdiv(N, 256) >= 192;
-  const int64_t tiles = cdiv(M, 128) * cdiv(N, 128);
-  if (!p.few && !p.big && tiles < 256) {
-    int64_t splits = cdiv(512, tiles);
-    if (splits > steps / 8) splits = steps / 8;
-    if (splits > 1) {
-      p.run = static_cast<int>(cdiv(steps, splits));
-      p.splits = static_cast<int>(cdiv(steps, p.run));
-    }
+  int64_t splits = 256 / tiles(64, p.shape == k64x32 ? 32 : 64);
+  if (splits > steps / 16) splits = steps / 16;
+  if (splits > 1) {
+    p.run = static_cast<int>(cdiv(steps, splits));
+    p.splits = static_cast<int>(cdiv(steps, p.run));
   }
   return p;
+}
+
+template <typename T, int TN, int TM, int WN, int WM>
+void launch_tile(const LinArgs &a, bool whole, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(cdiv(a.N, TN) * cdiv(a.M, TM)), a.splits);
+  if (whole)
+    linear_tile<T, TN, TM, WN, WM, true><<<grid, 64 * WN * WM, 0, st>>>(a);
+  else if constexpr (TN == TM && TN < 256)
+    linear_tile<T, TN, TM, WN, WM, false><<<grid, 64 * WN * WM, 0, st>>>(a);
 }
 
 }  // namespace
@@ -395,8 +424,10 @@ using namespace rxmet::dec;
 
 extern "C" int64_t rxmet_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan p = plan_for(M, N, K);
-  return p.splits > 1 ? p.splits * M * N * 4 : 0;
+  // the alignment is not known here: the larger of both ways
+  const Plan p = plan_for(M, N, K, true), q = plan_for(M, N, K, false);
+  const int splits = p.splits > q.splits ? p.splits : q.splits;
+  return splits > 1 ? splits * M * N * 4 : 0;
 }
 
 extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, const float *scales,
@@ -415,35 +446,32 @@ extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, cons
   if (M == 0) return 0;
   RXMET_CHECK_ARG(codes && scales && weight && weight_scales && y,
                   "codes, weight, their scales and y are needed");
-  RXMET_CHECK_ARG(cdiv(M, 128) * cdiv(N, 128) <= INT32_MAX / 64, "too many outputs for one call");
-  const Plan p = plan_for(M, N, K);
+  RXMET_CHECK_ARG(cdiv(M, 16) * cdiv(N, 64) <= INT32_MAX / 64, "too many outputs for one call");
+  const bool whole = (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(weight) |
+                      static_cast<uintptr_t>(codes_stride) |
+                      static_cast<uintptr_t>(weight_stride)) % 16 == 0;
+  const Plan p = plan_for(M, N, K, whole);
   RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
   const LinArgs a{codes, weight, codes_stride, weight_stride, scales, weight_scales, bias,
                   residual, residual_stride, y, M, N, static_cast<int>(K), activation,
                   static_cast<int *>(workspace), p.splits, p.run};
-  const bool whole = (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(weight) |
-                      static_cast<uintptr_t>(codes_stride) |
-                      static_cast<uintptr_t>(weight_stride)) % 16 == 0;
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("linear_int8", st);
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (p.few) {
-      const unsigned grid = static_cast<unsigned>(cdiv(N, 16));
-      if (M <= 16) linear_few<T, 1><<<grid, 64 * kFewWaves, 0, st>>>(a);
-      else if (M <= 32) linear_few<T, 2><<<grid, 64 * kFewWaves, 0, st>>>(a);
-      else linear_few<T, 4><<<grid, 64 * kFewWaves, 0, st>>>(a);
-    } else if (p.big) {
-      const unsigned grid = static_cast<unsigned>(cdiv(N, 256) * cdiv(M, 256));
-      if (whole) linear_tile<T, 256, 256, 2, 4, true><<<grid, 512, 0, st>>>(a);
-      else linear_tile<T, 256, 256, 2, 4, false><<<grid, 512, 0, st>>>(a);
-    } else {
-      const dim3 grid(static_cast<unsigned>(cdiv(N, 128) * cdiv(M, 128)), p.splits);
-      if (whole) linear_tile<T, 128, 128, 2, 2, true><<<grid, 256, 0, st>>>(a);
-      else linear_tile<T, 128, 128, 2, 2, false><<<grid, 256, 0, st>>>(a);
-      if (p.splits > 1)
-        linear_join<T><<<static_cast<unsigned>(cdiv(M * cdiv(N, 4), 256)), 256, 0, st>>>(a);
+    switch (p.shape) {
+      case kFew:
+        linear_few<T><<<static_cast<unsigned>(cdiv(N, 16)), 64 * kFewWaves, 0, st>>>(a);
+        break;
+      case k64x32: launch_tile<T, 64, 32, 2, 1>(a, whole, st); break;
+      case k64x64: launch_tile<T, 64, 64, 2, 2>(a, whole, st); break;
+      case k64x128: launch_tile<T, 64, 128, 2, 2>(a, whole, st); break;
+      case k128x128: launch_tile<T, 128, 128, 2, 2>(a, whole, st); break;
+      case k256x128: launch_tile<T, 256, 128, 4, 2>(a, whole, st); break;
+      case k256x256: launch_tile<T, 256, 256, 2, 4>(a, whole, st); break;
     }
+    if (p.splits > 1)
+      linear_join<T><<<static_cast<unsigned>(cdiv(M * cdiv(N, 4), 256)), 256, 0, st>>>(a);
   });
   RXMET_CHECK_LAUNCH();
   return 0;

@@ -57,7 +57,12 @@ def test_epilogue(cuda, M, N, K, act, dtype):
             check(y, x, sx, w, sw, b, act, r)
 
 
-@pytest.mark.parametrize("M,N,K", [(512, 512, 1024), (700, 1000, 640), (256, 768, 4112), (2049, 513, 192)])
+# every shape of tile: whole ones, ragged edges, K that ends inside a step, fewer steps than are
+# loaded ahead, K in parts
+@pytest.mark.parametrize("M,N,K", [(512, 512, 1024), (700, 1000, 640), (256, 768, 4112), (2049, 513, 192),
+                                   (3900, 4100, 208), (4096, 4096, 64), (4096, 4096, 16), (4000, 4099, 130),
+                                   (2000, 4100, 336), (1000, 4100, 1040), (1001, 4100, 70), (500, 4096, 272),
+                                   (24, 2000, 4112), (60, 1000, 8208), (100, 700, 5000), (90, 500, 4107)])
 def test_larger_tiles(cuda, M, N, K):
     x, sx, w, sw = make(M, N, K, 9, cuda)
     bias = torch.randn(N, generator=torch.Generator().manual_seed(1)).to(cuda)
