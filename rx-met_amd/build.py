@@ -99,10 +99,11 @@ def build_ort_ops(verbose: bool = True) -> Path | None:
     return ORT_LIB
 
 
-# The autograd node of the learnable min / max path (torch_ext/rxmet_torch.cpp): host code over
-# PyTorch's C++ headers, without a link to librxmet.so (it is handed the entry points of the
-# loaded one).  Users of the C ABI alone need no PyTorch: without it this module is not built.
-TORCH_SRC = PKG / "torch_ext" / "rxmet_torch.cpp"
+# The autograd node of the learnable min / max path (torch_ext/rxmet_torch.cpp) and the decoder
+# operators' calls (decoder_torch.cpp): host code over PyTorch's C++ headers, without a link to
+# librxmet.so (it is handed the entry points of the loaded one).  Users of the C ABI alone need no
+# PyTorch: without it this module is not built.
+TORCH_SRC = (PKG / "torch_ext" / "rxmet_torch.cpp", PKG / "torch_ext" / "decoder_torch.cpp")
 TORCH_LIB = PKG / ("rxmet_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
@@ -117,17 +118,26 @@ def build_torch_ext(verbose: bool = True) -> Path | None:
     BUILD.mkdir(exist_ok=True)
     tmp = TORCH_LIB.with_suffix(".so.tmp")
     torch_lib = Path(torch.__file__).parent / "lib"
-    cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-Wall",
-           "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f"-I{ROOT / 'include'}", f"-I{sysconfig.get_paths()['include']}",
-           *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")), "-o", str(tmp),
-           str(TORCH_SRC), f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
-           "-ltorch"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"PyTorch module build failed: {' '.join(cmd)}\n{proc.stdout}\n"
-                           f"{proc.stderr}")
+    cxx = shutil.which("g++") or "g++"
+    flags = ["-std=c++17", "-O2", "-fPIC", "-Wall",
+             "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-DTORCH_EXTENSION_NAME={TORCH_LIB.name.split('.')[0]}",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             f"-I{ROOT / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+             *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda"))]
+
+    def run(cmd):
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"PyTorch module build failed: {' '.join(cmd)}\n{proc.stdout}\n"
+                               f"{proc.stderr}")
+
+    objs = [BUILD / (s.name + ".o") for s in TORCH_SRC]
+    with cf.ThreadPoolExecutor(len(objs)) as ex:
+        list(ex.map(lambda so: run([cxx, *flags, "-c", str(so[0]), "-o", str(so[1])]),
+                    zip(TORCH_SRC, objs)))
+    run([cxx, "-shared", "-o", str(tmp), *map(str, objs), f"-L{torch_lib}", "-lc10", "-lc10_hip",
+         "-ltorch_cpu", "-ltorch_python", "-ltorch"])
     os.replace(tmp, TORCH_LIB)
     if verbose:
         print(f"built {TORCH_LIB}")

@@ -34,6 +34,28 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+_NATIVE = ("rxmet_rms_quantize_forward", "rxmet_rms_quantize_backward",
+           "rxmet_rms_quantize_backward_workspace_bytes", "rxmet_linear_int8",
+           "rxmet_linear_int8_workspace_bytes", "rxmet_kv_append", "rxmet_kv_read",
+           "rxmet_kv_attention", "rxmet_kv_attention_workspace_bytes", "rxmet_last_error")
+_ext = None
+
+
+def _native():
+    """The same calls in C++ (module ``rxmet_torch``, torch_ext/decoder_torch.cpp), which take
+    the host 4 - 6 us each instead of 14 - 18; False where the module cannot be imported.  They
+    return None (append: False) for what needs a copy or has to be refused: that is done here."""
+    global _ext
+    if _ext is None:
+        ext = _rx.torch_ext()
+        if ext is not None:
+            lib = _rx.load()
+            ext.bind_decoder([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
+                              for n in _NATIVE])
+        _ext = ext or False
+    return _ext
+
+
 def _float_type(t, name):
     if t.dtype not in _DTYPE:
         raise RuntimeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
@@ -115,6 +137,11 @@ def rms_norm_quantize(x, weight, residual=None, eps: float = 1e-6
     """
     if weight is None:
         raise RuntimeError("rms_norm_quantize needs a weight (quantize_rows has none)")
+    ext = _ext or _native()
+    if ext:
+        out = ext.rms_norm_quantize(x, weight, residual, eps)
+        if out is not None:
+            return out
     codes, _, scales, _, h = _row_forward(x, weight, residual, eps, True, False, False)
     return codes, scales, h
 
@@ -122,6 +149,11 @@ def rms_norm_quantize(x, weight, residual=None, eps: float = 1e-6
 def quantize_rows(x) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)``: the int8 grid of each row of x [..., C] as it is (scale = largest
     magnitude / 127)."""
+    ext = _ext or _native()
+    if ext:
+        out = ext.quantize_rows(x)
+        if out is not None:
+            return out
     codes, _, scales, _, _ = _row_forward(x, None, None, 0.0, True, False, False)
     return codes, scales
 
@@ -178,6 +210,11 @@ def rms_norm_quantize_dequantize(x, weight, residual=None, eps: float = 1e-6
     """
     if weight is None:
         raise RuntimeError("rms_norm_quantize_dequantize needs a weight")
+    ext = _ext or _native()
+    if ext:
+        out = ext.rms_norm_quantize_dequantize(x, weight, residual, eps)
+        if out is not None:
+            return out
     return _RmsQuantDequant.apply(x, weight, residual, eps)
 
 
@@ -194,6 +231,12 @@ def linear_int8(codes, scales, weight, weight_scales, bias=None, activation: Opt
     [..., N] in ``dtype``.  activation: None, "relu", "silu" or "gelu" (with the error function).
     The sum over K is exact, the rest float32.  K is at most 131071.
     """
+    ext = _ext or _native()
+    if ext and activation in ACTIVATIONS:
+        out = ext.linear_int8(codes, scales, weight, weight_scales, bias, ACTIVATIONS[activation],
+                              residual, dtype)
+        if out is not None:
+            return out
     _on_gpu(codes, "codes")
     dev = codes.device
     if dtype not in _DTYPE:
@@ -316,6 +359,9 @@ def kv_cache_append(cache: KVCache, key, value, block_table, lengths, cu_new=Non
     grid.  The sequences' open pages must be their own.  Tokens whose page is missing (an id outside the cache,
     a place past the table) are left out.
     """
+    ext = _ext or _native()
+    if ext and ext.kv_append(*cache, key, value, block_table, lengths, cu_new, max_new):
+        return
     seqs = block_table.shape[0] if block_table.dim() else 0
     c, t, dev = _cache_args(cache, block_table, ("lengths", lengths, seqs),
                             ("cu_new", cu_new, seqs + 1))
@@ -346,6 +392,11 @@ def kv_cache_read(cache: KVCache, block_table, first, cu_tokens, tokens: int,
     ``tokens`` is ``cu_tokens[-1]``, which the caller knows; rows that no sequence covers are
     undefined.  A token whose page is missing reads as NaN.
     """
+    ext = _ext or _native()
+    if ext:
+        out = ext.kv_read(*cache, block_table, first, cu_tokens, tokens, max_tokens, dtype)
+        if out is not None:
+            return out
     seqs = block_table.shape[0] if block_table.dim() else 0
     c, t, dev = _cache_args(cache, block_table, ("first", first, seqs),
                             ("cu_tokens", cu_tokens, seqs + 1))
@@ -377,6 +428,12 @@ def kv_cache_attention(query, cache: KVCache, block_table, lengths, cu_query=Non
     default to all rows and to the table's width.  Larger values in the device vectors are computed
     as well, more slowly.
     """
+    ext = _ext or _native()
+    if ext:
+        out = ext.kv_attention(query, *cache, block_table, lengths, cu_query, max_query, max_length,
+                               scale, causal, window)
+        if out is not None:
+            return out
     seqs = block_table.shape[0] if block_table.dim() else 0
     c, t, dev = _cache_args(cache, block_table, ("lengths", lengths, seqs),
                             ("cu_query", cu_query, seqs + 1))

@@ -7,15 +7,10 @@
 // without the interpreter: 67 us (bf16 [3001, 4099], per tensor: 156 -> 67 us for 62 us of
 // kernels).  mi355x_qdq.py keeps the Python Function for what this one does not take: tensors that
 // have to be copied first, tracing and tensor subclasses (_native_node there).
-#include <torch/extension.h>
-
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
+#include "rxmet_torch.h"
 
 #include <algorithm>
 #include <memory>
-#include <stdexcept>
-#include <string>
 
 #include "rxmet_qdq.h"
 
@@ -41,9 +36,8 @@ struct MinMaxPlan : torch::CustomClassHolder {
   float sym_offset, min_scale;
 };
 
-struct LibraryError : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
+using rxmet_torch::LibraryError;
+using rxmet_torch::stream_of;
 
 void check(int rc, const char *what) {
   if (rc != 0)
@@ -65,10 +59,6 @@ void check_tensors(const at::Tensor &x, const at::Tensor &mn, const at::Tensor &
                   mx.scalar_type() == at::kFloat && x.is_contiguous() && mn.is_contiguous() &&
                   mx.is_contiguous() && x.numel() == n && mn.numel() == c && mx.numel() == c,
               "qdq_minmax: the tensors do not match the plan");
-}
-
-void *stream_of(const at::Tensor &t) {
-  return c10::hip::getCurrentHIPStream(t.get_device()).stream();
 }
 
 struct QdqMinMax : public torch::autograd::Function<QdqMinMax> {
@@ -162,4 +152,5 @@ PYBIND11_MODULE(rxmet_torch, m) {
   m.def("bind", &bind);
   m.def("make_plan", &make_plan);
   m.def("qdq_minmax", &qdq_minmax);
+  rxmet_torch::add_decoder(m);
 }
