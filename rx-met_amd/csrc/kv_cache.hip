@@ -6,12 +6,13 @@
 // dimension by dimension (each dimension's tokens side by side): both are what a lane of the
 // attention's matrix instructions reads as 16 consecutive bytes.
 //
-// A workgroup owns a page's keys or values of one head, in pieces of 16 bytes: 16 dimensions of a
-// token, or 16 tokens of a dimension.  No two workgroups write the same bytes, and the older codes are
-// read only where they move or share a piece with a new token.
+// A workgroup owns a page's keys or values of one head.  No two workgroups write the same bytes, and the
+// older codes are read only where they move or share 16 bytes with a new token.
 //
 // Bound: HBM traffic for prompts (each new token read, its codes written); for single tokens the
 // launch and two dependent reads.
+#include <type_traits>
+
 #include "kv_cache.h"
 
 namespace rxmet {
@@ -35,10 +36,22 @@ __device__ __forceinline__ float block_max(float v) {
   return nan_max(nan_max(s[0], s[1]), nan_max(s[2], s[3]));
 }
 
-template <typename T>
+// Four codes of an old page on its new grid.
+__device__ __forceinline__ unsigned move_codes(unsigned w, float ratio) {
+  return code_bytes4(code_value(w, 0) * ratio, code_value(w, 1) * ratio, code_value(w, 2) * ratio,
+                     code_value(w, 3) * ratio);
+}
+
+// A thread holds units of four tokens x eight dimensions in registers between the maximum and the
+// codes, so that the tokens are read once; values are turned in LDS, where a unit gives one word (four
+// tokens) for each dimension.
+template <typename T, int D, int P>
 __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
-  const int P = a.g.c.page_size, D = a.g.c.dim, b = blockIdx.y;
-  const int which = blockIdx.z & 1, head = blockIdx.z >> 1;
+  constexpr int C = D / 8;                              // chunks of eight dimensions
+  constexpr int units = P / 4 * C, NU = (units + 255) / 256;
+  constexpr int pitch = P / 4 + 1;                      // words of a dimension in LDS
+  __shared__ unsigned s_v[D * pitch];
+  const int b = blockIdx.y, which = blockIdx.z & 1, head = blockIdx.z >> 1, tid = threadIdx.x;
   const int64_t start = a.lengths[b];
   const int64_t row0 = a.cu ? a.cu[b] : b;
   int64_t count = a.cu ? a.cu[b + 1] - row0 : 1;
@@ -48,6 +61,7 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
   const int64_t first = start / P, last = (start + count - 1) / P;
   int8_t *pool = which ? a.g.c.v : a.g.c.k;
   float *scales = which ? a.g.c.v_scale : a.g.c.k_scale;
+  const int64_t stride = a.stride_t[which];
   const T *x = static_cast<const T *>(a.x[which]) + head * a.stride_h[which];
   for (int64_t p = first + blockIdx.x; p <= last; p += gridDim.x) {
     const int64_t page = page_of(a.g, b, p);
@@ -55,18 +69,28 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
     // new tokens stand in slots s0..s1-1, older ones below s0
     const int s0 = static_cast<int>(p == first ? start - p * P : 0);
     const int s1 = static_cast<int>(p == last ? start + count - p * P : P);
-    const T *xp = x + (row0 + p * P - start) * a.stride_t[which];  // slot 0's token (may lie before x)
+    const int64_t row = row0 + p * P - start;  // of slot 0 (may lie before the rows)
     const int64_t at = page * a.g.c.heads + head;
     int8_t *codes = pool + at * P * D;
-    const int vecs = (s1 - s0) * (D / 8);
-    float top = 0.0f;
-    for (int i = threadIdx.x; i < vecs; i += 256) {
-      float f[8];
-      load8(xp + (s0 + i / (D / 8)) * a.stride_t[which] + i % (D / 8) * 8, f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = nan_max(top, fabsf(f[e]));
-    }
     const float was = s0 > 0 ? scales[at] : 0.0f;
+    Vec8<T> u[NU][4];
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+      const int i = tid + 256 * j, c = i % C, q = i / C * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u[j][e] = {};
+        if (q + e >= s0 && q + e < s1)  // false past the last unit, where q >= P
+          __builtin_memcpy(&u[j][e], x + (row + q + e) * stride + 8 * c, sizeof(Vec8<T>));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NU; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) top = nan_max(top, fabsf(static_cast<float>(u[j][e].v[d])));
     top = block_max(top);
     // block_max's barriers stand between every thread's read of the old scale and this write
     const bool good = top <= 3.402823466e38f && was == was;
@@ -75,53 +99,66 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
     const float inv = good ? 1.0f / scale : 0.0f;
     const float ratio = good ? was * inv : 0.0f;
     const bool moves = s0 > 0 && !(scale == was);
-    if (threadIdx.x == 0) scales[at] = scale;
-    // pieces: keys (slot, 16 dimensions), values (16 slots, dimension)
-    const int pieces = P * D / 16;
-    for (int i = threadIdx.x; i < pieces; i += 256) {
-      int lo, hi, off;  // slots of the piece, its bytes' place
-      if (which == 0) {
-        lo = i / (D / 16), hi = lo + 1, off = i * 16;
-      } else {
-        const int d = i % D, g = i / D;
-        lo = g * 16, hi = lo + 16, off = d * P + lo;
-      }
-      const bool has_new = lo < s1 && hi > s0, has_old = lo < s0;
-      if (!(has_new || (has_old && moves))) continue;
-      unsigned w[4] = {};
-      if (has_old) {
-        __builtin_memcpy(w, codes + off, 16);
-        if (moves) {
+    if (tid == 0) scales[at] = scale;
+    if (which == 0) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = code_bytes4(code_value(w[k], 0) * ratio, code_value(w[k], 1) * ratio,
-                               code_value(w[k], 2) * ratio, code_value(w[k], 3) * ratio);
+      for (int j = 0; j < NU; ++j) {
+        const int i = tid + 256 * j, c = i % C, q = i / C * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (q + e < s0 || q + e >= s1) continue;
+          unsigned w[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            w[k] = code_bytes4(static_cast<float>(u[j][e].v[4 * k]) * inv,
+                               static_cast<float>(u[j][e].v[4 * k + 1]) * inv,
+                               static_cast<float>(u[j][e].v[4 * k + 2]) * inv,
+                               static_cast<float>(u[j][e].v[4 * k + 3]) * inv);
+          *reinterpret_cast<uint2 *>(codes + (q + e) * D + 8 * c) = make_uint2(w[0], w[1]);
         }
       }
-      if (has_new) {
-        if (which == 0) {
-          const T *q = xp + lo * a.stride_t[0] + i % (D / 16) * 16;
-          float f[8];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            load8(q + 8 * k, f);
-            w[2 * k] = code_bytes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-            w[2 * k + 1] = code_bytes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-          }
-        } else {
-          const T *q = xp + i % D;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int s = lo + e;
-            if (s >= s0 && s < s1) {
-              const float f = static_cast<float>(q[s * a.stride_t[1]]);
-              const int sh = 8 * (e % 4);
-              w[e / 4] = (w[e / 4] & ~(0xffu << sh)) | code_byte(f * inv) << sh;
-            }
-          }
+      if (moves) {
+        for (int i = tid; i < s0 * (D / 16); i += 256) {
+          uint4 w = *reinterpret_cast<const uint4 *>(codes + i * 16);
+          w = make_uint4(move_codes(w.x, ratio), move_codes(w.y, ratio), move_codes(w.z, ratio),
+                         move_codes(w.w, ratio));
+          *reinterpret_cast<uint4 *>(codes + i * 16) = w;
         }
       }
-      __builtin_memcpy(codes + off, w, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NU; ++j) {
+        const int i = tid + 256 * j, c = i % C, q = i / C;
+        if (i < units) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            s_v[(8 * c + d) * pitch + q] = code_bytes4(
+                static_cast<float>(u[j][0].v[d]) * inv, static_cast<float>(u[j][1].v[d]) * inv,
+                static_cast<float>(u[j][2].v[d]) * inv, static_cast<float>(u[j][3].v[d]) * inv);
+        }
+      }
+      __syncthreads();
+      // pieces of 16 slots of a dimension: those with a new token, and those whose codes move
+      const int from = moves ? 0 : s0 / 16, to = (s1 + 15) / 16;
+      for (int i = tid; i < (to - from) * D; i += 256) {
+        const int g = from + i % (to - from), d = i / (to - from), old = s0 - 16 * g;
+        uint4 *place = reinterpret_cast<uint4 *>(codes + d * P + 16 * g);
+        const unsigned *n = s_v + d * pitch + 4 * g;
+        unsigned w[4] = {n[0], n[1], n[2], n[3]};
+        if (old > 0) {  // the older codes of the piece
+          unsigned o[4];
+          __builtin_memcpy(o, place, 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (moves) o[k] = move_codes(o[k], ratio);
+            const int keep = old - 4 * k;  // of this word's bytes
+            const unsigned mask = keep <= 0 ? 0u : keep >= 4 ? ~0u : (1u << (8 * keep)) - 1;
+            w[k] = (o[k] & mask) | (w[k] & ~mask);
+          }
+        }
+        *place = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncthreads();  // the next page's codes take the LDS
     }
   }
 }
@@ -133,49 +170,80 @@ struct ReadArgs {
   void *out[2];
 };
 
-template <typename T>
+template <typename T, int D, int P>
 __global__ __launch_bounds__(256) void kv_read(const ReadArgs a) {
-  const int P = a.g.c.page_size, D = a.g.c.dim, b = blockIdx.y;
-  const int which = blockIdx.z & 1, head = blockIdx.z >> 1;
+  const int b = blockIdx.y, which = blockIdx.z & 1, head = blockIdx.z >> 1, tid = threadIdx.x;
   const int64_t start = a.first[b], row0 = a.cu[b];
   int64_t count = a.cu[b + 1] - row0;
   if (row0 < 0) return;
   if (count > a.tokens - row0) count = a.tokens - row0;
   if (count <= 0) return;
+  // pages of tokens before 0 have no place in the table: their values are NaN
   const int64_t first = start >= 0 ? start / P : -((-start + P - 1) / P);
-  const int64_t last = (start + count - 1) / P;
-  const int64_t row = static_cast<int64_t>(a.g.c.heads) * D;
+  const int64_t end = start + count, last = end > 0 ? (end - 1) / P : -((-end + P) / P);
+  const int64_t pitch = static_cast<int64_t>(a.g.c.heads) * D;
+  T *out = static_cast<T *>(a.out[which]) + head * D;
   for (int64_t p = first + blockIdx.x; p <= last; p += gridDim.x) {
     const int64_t page = page_of(a.g, b, p);
     const int s0 = static_cast<int>(p == first ? start - p * P : 0);
-    const int s1 = static_cast<int>(p == last ? start + count - p * P : P);
+    const int s1 = static_cast<int>(p == last ? end - p * P : P);
     const int64_t at = (page < 0 ? 0 : page) * a.g.c.heads + head;
     const int8_t *codes = (which ? a.g.c.v : a.g.c.k) + at * P * D;
     const float scale = page < 0 ? nanf32() : (which ? a.g.c.v_scale : a.g.c.k_scale)[at];
-    T *out = static_cast<T *>(a.out[which]) + head * D;
-    for (int i = threadIdx.x; i < P * D / 16; i += 256) {
-      const int lo = which == 0 ? i / (D / 16) : i / D * 16;
-      if (lo >= s1 || lo + (which == 0 ? 1 : 16) <= s0) continue;
-      unsigned w[4] = {};
-      if (page >= 0)
-        __builtin_memcpy(w, codes + (which == 0 ? i * 16 : i % D * P + lo), 16);
-      if (which == 0) {
-        T *q = out + (row0 + p * P + lo - start) * row + i % (D / 16) * 16;
+    T *q = out + (row0 + p * P - start) * pitch;  // slot 0's row (may lie before the rows)
+    if (which == 0) {
+      constexpr int C = D / 16;
+#pragma unroll 4
+      for (int i = s0 * C + tid; i < s1 * C; i += 256) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(codes + i * 16);
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+        T *o = q + i / C * pitch + i % C * 16;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = code_value(w[2 * k + e / 4], e % 4) * scale;
-          store8(q + 8 * k, f);
+          store8(o + 8 * k, f);
         }
-      } else {
-        T *q = out + (row0 + p * P - start) * row + i % D;
+      }
+    } else {
+      // a thread takes 16 slots of two dimensions, so that a wave writes 128 or 256 bytes of a row
+      const int from = s0 / 16, groups = (s1 + 15) / 16 - from;
+      for (int i = tid; i < groups * (D / 2); i += 256) {
+        const int d = i % (D / 2) * 2, lo = (from + i / (D / 2)) * 16;
+        const uint4 u0 = *reinterpret_cast<const uint4 *>(codes + d * P + lo);
+        const uint4 u1 = *reinterpret_cast<const uint4 *>(codes + (d + 1) * P + lo);
+        const unsigned w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (lo + e >= s0 && lo + e < s1)
-            q[(lo + e) * row] = static_cast<T>(code_value(w[e / 4], e % 4) * scale);
+        for (int e = 0; e < 16; ++e) {
+          if (lo + e < s0 || lo + e >= s1) continue;
+          struct {
+            T v[2];
+          } o = {{static_cast<T>(code_value(w0[e / 4], e % 4) * scale),
+                  static_cast<T>(code_value(w1[e / 4], e % 4) * scale)}};
+          __builtin_memcpy(q + (lo + e) * pitch + d, &o, sizeof(o));
+        }
       }
     }
+  }
+}
+
+// Runs f(dim, page size) for a cache that check_cache has passed.
+template <typename F>
+void with_page_shape(const rxmet_kv_cache &c, F &&f) {
+  auto sized = [&](auto d) {
+    switch (c.page_size) {
+      case 16: f(d, std::integral_constant<int, 16>{}); break;
+      case 32: f(d, std::integral_constant<int, 32>{}); break;
+      case 64: f(d, std::integral_constant<int, 64>{}); break;
+      default: f(d, std::integral_constant<int, 128>{}); break;
+    }
+  };
+  switch (c.dim) {
+    case 64: sized(std::integral_constant<int, 64>{}); break;
+    case 128: sized(std::integral_constant<int, 128>{}); break;
+    case 192: sized(std::integral_constant<int, 192>{}); break;
+    default: sized(std::integral_constant<int, 256>{}); break;
   }
 }
 
@@ -224,7 +292,11 @@ extern "C" int rxmet_kv_append(const rxmet_kv_cache *cache, const rxmet_kv_table
                   2 * cache->heads);
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("kv_append", st);
-  with_type(dtype, [&](auto t) { kv_append<decltype(t)><<<grid, 256, 0, st>>>(a); });
+  with_type(dtype, [&](auto t) {
+    with_page_shape(*cache, [&](auto d, auto p) {
+      kv_append<decltype(t), d.value, p.value><<<grid, 256, 0, st>>>(a);
+    });
+  });
   RXMET_CHECK_LAUNCH();
   return 0;
 }
@@ -245,7 +317,11 @@ extern "C" int rxmet_kv_read(const rxmet_kv_cache *cache, const rxmet_kv_table *
                   2 * cache->heads);
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("kv_read", st);
-  with_type(dtype, [&](auto t) { kv_read<decltype(t)><<<grid, 256, 0, st>>>(a); });
+  with_type(dtype, [&](auto t) {
+    with_page_shape(*cache, [&](auto d, auto p) {
+      kv_read<decltype(t), d.value, p.value><<<grid, 256, 0, st>>>(a);
+    });
+  });
   RXMET_CHECK_LAUNCH();
   return 0;
 }
