@@ -70,9 +70,13 @@ enum {
  *           + residual[m, n]
  * The sum is exact (int32); the rest is fp32, rounded once to dtype.  codes [M, K] and weight
  * [N, K] int8 with row strides in bytes; bias [N] and residual [M, N] in dtype, may be NULL;
- * y [M, N] dense.  The workspace may be NULL where its size is 0.
+ * y [M, N] dense.  The workspace (aligned to 16 bytes) may be NULL where its size is 0.  Rows that do not all
+ * start on 16 bytes are copied into it for more than 16 rows of x; a weight laid out with such
+ * a row stride once saves that.
  */
-int64_t rxmet_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int64_t rxmet_linear_int8_workspace_bytes(const int8_t *codes, int64_t codes_stride,
+                                          const int8_t *weight, int64_t weight_stride, int64_t M,
+                                          int64_t N, int64_t K);
 int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, const float *scales,
                       const int8_t *weight, int64_t weight_stride, const float *weight_scales,
                       const void *bias, const void *residual, int64_t residual_stride, void *y,

@@ -55,42 +55,38 @@ __device__ __forceinline__ uint4 load_piece(const int8_t *row, int k, int K) {
 
 __device__ __forceinline__ v4i as_v4i(uint4 u) { return __builtin_bit_cast(v4i, u); }
 
-// Writes C consecutive n of row m.
+// Finishes and writes C consecutive n of row m: as vectors, and one by one at N's end.
 template <typename T, int C>
 __device__ __forceinline__ void finish(const LinArgs &a, int64_t m, int64_t n0, const int (&acc)[C]) {
   if (m >= a.M || n0 >= a.N) return;
   const float sx = a.sx[m];
-  const T *bias = static_cast<const T *>(a.bias);
+  const T *bias = a.bias ? static_cast<const T *>(a.bias) + n0 : nullptr;
   const T *res = a.res ? static_cast<const T *>(a.res) + m * a.res_stride + n0 : nullptr;
   T *y = static_cast<T *>(a.y) + m * a.N + n0;
-  struct Run {
-    T v[C];
-  } out, r;
-  const int left = a.N - n0 < C ? static_cast<int>(a.N - n0) : C;
-  if (res) {
-    if (left == C) {
-      __builtin_memcpy(&r, res, sizeof(r));
-    } else {
-#pragma unroll
-      for (int e = 0; e < C; ++e)
-        if (e < left) r.v[e] = res[e];
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < C; ++e) {
-    if (e >= left) continue;
-    float v = static_cast<float>(acc[e]) * sx * a.sw[n0 + e];
-    if (bias) v += static_cast<float>(bias[n0 + e]);
+  auto value = [&](int acc, float sw, T b, T r) {
+    float v = static_cast<float>(acc) * sx * sw;
+    if (bias) v += static_cast<float>(b);
     v = activate(v, a.act);
-    if (res) v += static_cast<float>(r.v[e]);
-    out.v[e] = static_cast<T>(v);
-  }
-  if (left == C) {
+    if (res) v += static_cast<float>(r);
+    return static_cast<T>(v);
+  };
+  if (n0 + C <= a.N) {
+    struct {
+      T v[C];
+    } out, b = {}, r = {};
+    float sw[C];
+    __builtin_memcpy(sw, a.sw + n0, sizeof(sw));
+    if (bias) __builtin_memcpy(&b, bias, sizeof(b));
+    if (res) __builtin_memcpy(&r, res, sizeof(r));
+#pragma unroll
+    for (int e = 0; e < C; ++e) out.v[e] = value(acc[e], sw[e], b.v[e], r.v[e]);
     __builtin_memcpy(y, &out, sizeof(out));
   } else {
 #pragma unroll
     for (int e = 0; e < C; ++e)
-      if (e < left) y[e] = out.v[e];
+      if (n0 + e < a.N)
+        y[e] = value(acc[e], a.sw[n0 + e], bias ? bias[e] : static_cast<T>(0.0f),
+                     res ? res[e] : static_cast<T>(0.0f));
   }
 }
 
@@ -154,11 +150,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few(const LinArgs a) {
 // ---------------------------------------------------------------------------------------------
 // Tiles of TN weight rows x TM token rows on mfma 32x32x32; WN x WM waves take equal parts.
 //
-// K goes through LDS in steps of 64 bytes.  A row's four 16-byte pieces lie at the places
-// piece ^ f(row), so that 16 lanes that read one piece of 16 rows meet 16 different bank groups.
-// Row i of a wave's 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4: a lane
-// holds 16 consecutive n of one m.  ASYNC (rows of whole aligned pieces): memory -> LDS without
-// registers, three steps ahead in a ring of four; else through registers, one step ahead.
+// K goes through LDS in steps of 64 bytes, memory -> LDS without registers, three steps ahead in
+// a ring of four.  A row's four 16-byte pieces lie at the places piece ^ f(row), so that 16 lanes
+// that read one piece of 16 rows meet 16 different bank groups.  Row i of a wave's 32 weight rows stands
+// for n = 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4: a lane holds 16 consecutive n of one m.  Rows have to
+// start on 16 bytes; others are copied first (linear_align).
 constexpr int kStep = 64;
 
 typedef int v16i __attribute__((ext_vector_type(16)));
@@ -183,13 +179,16 @@ __device__ __forceinline__ void meet() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
 }
 
-template <typename T, int TN, int TM, int WN, int WM, bool ASYNC>
+template <typename T, int TN, int TM, int WN, int WM>
 __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
   constexpr int threads = 64 * WN * WM;
   constexpr int FN = TN / WN / 32, FM = TM / WM / 32;
   constexpr int bytes = (TN + TM) * kStep;
-  constexpr int ring = ASYNC ? 4 : 2;
+  constexpr int ring = 4;
   constexpr int loads = bytes / 16 / threads;  // pieces of a thread in a step
+  constexpr int CH = 8 * FN;                   // chunks of four n in a wave's row (epilogue)
+  static_assert(loads * 16 * threads == bytes, "a step is whole pieces of all threads");
+  static_assert(WN * WM * 32 * CH * 16 <= ring * bytes, "the epilogue fits the ring");
   __shared__ __attribute__((aligned(16))) int8_t s[ring][bytes];
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -270,82 +269,93 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
           acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
     }
   };
-  // a step through registers
-  uint4 reg[loads];
-  auto fetch = [&](int step) {
-#pragma unroll
-    for (int j = 0; j < loads; ++j) __builtin_memcpy(&reg[j], src[j] + step * kStep, 16);
-  };
-  auto fetch_end = [&](int step) {
-#pragma unroll
-    for (int j = 0; j < loads; ++j) {
-      const int k = step * kStep + 16 * piece_at(j);
-      reg[j] = load_piece(src[j] + step * kStep - k, k, a.K - from * kStep);
-    }
-  };
-  auto put = [&](int8_t *buf) {
+  auto issue = [&](int step, int slot) {
 #pragma unroll
     for (int j = 0; j < loads; ++j)
-      *reinterpret_cast<uint4 *>(buf + 16 * (tid + threads * j)) = reg[j];
+      load_to_lds(src[j] + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
   };
-  if constexpr (ASYNC) {
-    auto issue = [&](int step, int slot) {
+  if (whole > 0) {
+    // past the end a step is read once more, so that the count of loads in flight holds
 #pragma unroll
-      for (int j = 0; j < loads; ++j)
-        load_to_lds(src[j] + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
-    };
-    if (whole > 0) {
-      // past the end a step is read once more, so that the count of loads in flight holds
-#pragma unroll
-      for (int k = 0; k < ring - 1; ++k) issue(k < whole ? k : 0, k);
-      for (int k = 0; k < whole; ++k) {
-        wait_loads<(ring - 2) * loads>();
-        meet();  // step k is there for all, and step k - 1 has been read by all
-        issue(k + ring - 1 < whole ? k + ring - 1 : k, (k + ring - 1) % ring);
-        compute(s[k % ring]);
-      }
-      wait_loads<0>();
-    }
-  } else {
-    if (whole > 0) {
-      fetch(0);
-      put(s[0]);
-    }
+    for (int k = 0; k < ring - 1; ++k) issue(k < whole ? k : 0, k);
     for (int k = 0; k < whole; ++k) {
-      __syncthreads();
-      if (k + 1 < whole) fetch(k + 1);
-      compute(s[k & 1]);
-      if (k + 1 < whole) put(s[(k + 1) & 1]);
+      wait_loads<(ring - 2) * loads>();
+      meet();  // step k is there for all, and step k - 1 has been read by all
+      issue(k + ring - 1 < whole ? k + ring - 1 : k, (k + ring - 1) % ring);
+      compute(s[k % ring]);
     }
+    wait_loads<0>();
   }
+  __syncthreads();
   if (last && all * kStep < a.K) {
-    fetch_end(whole);
-    __syncthreads();
-    put(s[0]);
+#pragma unroll
+    for (int j = 0; j < loads; ++j) {
+      const int k = whole * kStep + 16 * piece_at(j);  // from this part's first byte
+      *reinterpret_cast<uint4 *>(&s[0][16 * (tid + threads * j)]) =
+          load_piece(src[j] + whole * kStep - k, k, a.K - from * kStep);
+    }
     __syncthreads();
     compute(s[0]);
+    __syncthreads();
   }
+
+  // 32 rows of x at a time the wave's sums go through its own part of the LDS, from where eight
+  // consecutive n of a row are finished by a lane and neighbouring lanes write what lies side by
+  // side.  Chunk c of row m lies at c ^ turn, for the banks.
+  auto turn = [](int m) { return CH >= 16 ? m & 15 : m >> 1 & 7; };
+  v4i *part = reinterpret_cast<v4i *>(&s[0][0]) + wave * 32 * CH;
 #pragma unroll
-  for (int i = 0; i < FN; ++i)
+  for (int j = 0; j < FM; ++j) {
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      int v[16];
+    for (int i = 0; i < FN; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = acc[i][j][r];
-      const int64_t m = m0 + wm + 32 * j + col, n = n0 + wn + 32 * i + 16 * h;
+      for (int k = 0; k < 4; ++k)
+        part[col * CH + ((8 * i + 4 * h + k) ^ turn(col))] =
+            v4i{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+#pragma unroll 1
+    for (int at = lane; at < 32 * CH / 2; at += kWave) {
+      const int r = at / (CH / 2), c = at % (CH / 2) * 2;
+      const v4i lo = part[r * CH + (c ^ turn(r))], hi = part[r * CH + ((c + 1) ^ turn(r))];
+      const int v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      const int64_t m = m0 + wm + 32 * j + r, n = n0 + wn + 4 * c;
       if (a.splits == 1) {
-        finish<T, 16>(a, m, n, v);
+        finish<T, 8>(a, m, n, v);
       } else if (m < a.M) {
         int *p = a.part + (split * a.M + m) * a.N + n;
-        if (n + 16 <= a.N) {
+        if (n + 8 <= a.N) {
           __builtin_memcpy(p, v, sizeof(v));
         } else {
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (n + r < a.N) p[r] = v[r];
+          for (int e = 0; e < 8; ++e)
+            if (n + e < a.N) p[e] = v[e];
         }
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before it is written again
+  }
+}
+
+// Rows that do not start on 16 bytes, copied to rows of whole steps with zeros behind them: M rows
+// of x, then N of the weights.  One launch and the bytes twice, against loads of 16 bytes at any
+// address in the tiles' loop ([777, 1025] x [2051, 1025]: 15.6 us and 13.5 us with words moved
+// into place).
+struct AlignArgs {
+  const int8_t *x, *w;
+  int64_t x_stride, w_stride;
+  int8_t *out;
+  int64_t M, rows;
+  int K, pitch;
+};
+
+__global__ __launch_bounds__(256) void linear_align(const AlignArgs a) {
+  const int pieces = a.pitch / 16;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= a.rows * pieces) return;
+  const int64_t row = i / pieces;
+  const int k = static_cast<int>(i % pieces) * 16;
+  const int8_t *p = row < a.M ? a.x + row * a.x_stride : a.w + (row - a.M) * a.w_stride;
+  *reinterpret_cast<uint4 *>(a.out + row * a.pitch + k) = load_piece(p, k, a.K);
 }
 
 // Adds the parts of K up and finishes four n of a row.
@@ -385,17 +395,16 @@ struct Plan {
   int splits, run;
 };
 
-// `whole`: rows of aligned 16-byte pieces; the others have fewer shapes.
-Plan plan_for(int64_t M, int64_t N, int64_t K, bool whole) {
+Plan plan_for(int64_t M, int64_t N, int64_t K) {
   if (M <= kFewRows) return {kFew, 1, 0};
   auto tiles = [&](int64_t tn, int64_t tm) { return cdiv(N, tn) * cdiv(M, tm); };
   if (M > 64) {
-    if (whole && tiles(256, 256) >= 256) return {k256x256, 1, 0};
-    if (whole && tiles(256, 128) >= 256) return {k256x128, 1, 0};
+    if (tiles(256, 256) >= 256) return {k256x256, 1, 0};
+    if (tiles(256, 128) >= 256) return {k256x128, 1, 0};
     if (tiles(128, 128) >= 256) return {k128x128, 1, 0};
-    if (whole && tiles(64, 128) >= 256) return {k64x128, 1, 0};
+    if (tiles(64, 128) >= 256) return {k64x128, 1, 0};
   }
-  Plan p{whole && M <= 32 ? k64x32 : k64x64, 1, 0};
+  Plan p{M <= 32 ? k64x32 : k64x64, 1, 0};
   const int64_t steps = K / kStep;
   int64_t splits = 256 / tiles(64, p.shape == k64x32 ? 32 : 64);
   if (splits > steps / 16) splits = steps / 16;
@@ -406,13 +415,23 @@ Plan plan_for(int64_t M, int64_t N, int64_t K, bool whole) {
   return p;
 }
 
+// Whether the rows can be read in aligned pieces of 16 bytes.
+bool aligned(const void *codes, int64_t codes_stride, const void *weight, int64_t weight_stride) {
+  return (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(weight) |
+          static_cast<uintptr_t>(codes_stride) | static_cast<uintptr_t>(weight_stride)) % 16 == 0;
+}
+
+int64_t pitch_of(int64_t K) { return cdiv(K, kStep) * kStep; }
+
+// Bytes of the parts' sums, behind which the copied rows lie.
+int64_t part_bytes(const Plan &p, int64_t M, int64_t N) {
+  return p.splits > 1 ? cdiv(p.splits * M * N * 4, 256) * 256 : 0;
+}
+
 template <typename T, int TN, int TM, int WN, int WM>
-void launch_tile(const LinArgs &a, bool whole, hipStream_t st) {
+void launch_tile(const LinArgs &a, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(cdiv(a.N, TN) * cdiv(a.M, TM)), a.splits);
-  if (whole)
-    linear_tile<T, TN, TM, WN, WM, true><<<grid, 64 * WN * WM, 0, st>>>(a);
-  else if constexpr (TN == TM && TN < 256)
-    linear_tile<T, TN, TM, WN, WM, false><<<grid, 64 * WN * WM, 0, st>>>(a);
+  linear_tile<T, TN, TM, WN, WM><<<grid, 64 * WN * WM, 0, st>>>(a);
 }
 
 }  // namespace
@@ -422,12 +441,15 @@ void launch_tile(const LinArgs &a, bool whole, hipStream_t st) {
 using namespace rxmet;
 using namespace rxmet::dec;
 
-extern "C" int64_t rxmet_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+extern "C" int64_t rxmet_linear_int8_workspace_bytes(const int8_t *codes, int64_t codes_stride,
+                                                     const int8_t *weight, int64_t weight_stride,
+                                                     int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  // the alignment is not known here: the larger of both ways
-  const Plan p = plan_for(M, N, K, true), q = plan_for(M, N, K, false);
-  const int splits = p.splits > q.splits ? p.splits : q.splits;
-  return splits > 1 ? splits * M * N * 4 : 0;
+  const Plan p = plan_for(M, N, K);
+  int64_t bytes = part_bytes(p, M, N);
+  if (p.shape != kFew && !aligned(codes, codes_stride, weight, weight_stride))
+    bytes += (M + N) * pitch_of(K);
+  return bytes;
 }
 
 extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, const float *scales,
@@ -447,28 +469,39 @@ extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, cons
   RXMET_CHECK_ARG(codes && scales && weight && weight_scales && y,
                   "codes, weight, their scales and y are needed");
   RXMET_CHECK_ARG(cdiv(M, 16) * cdiv(N, 64) <= INT32_MAX / 64, "too many outputs for one call");
-  const bool whole = (reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(weight) |
-                      static_cast<uintptr_t>(codes_stride) |
-                      static_cast<uintptr_t>(weight_stride)) % 16 == 0;
-  const Plan p = plan_for(M, N, K, whole);
-  RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
-  const LinArgs a{codes, weight, codes_stride, weight_stride, scales, weight_scales, bias,
-                  residual, residual_stride, y, M, N, static_cast<int>(K), activation,
-                  static_cast<int *>(workspace), p.splits, p.run};
+  const Plan p = plan_for(M, N, K);
+  const bool copy = p.shape != kFew && !aligned(codes, codes_stride, weight, weight_stride);
+  RXMET_CHECK_ARG((p.splits == 1 && !copy) || workspace, "this call needs a workspace");
+  RXMET_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
+  RXMET_CHECK_ARG(cdiv((M + N) * (pitch_of(K) / 16), 256) <= INT32_MAX, "too many rows for one call");
+  LinArgs a{codes, weight, codes_stride, weight_stride, scales, weight_scales, bias,
+            residual, residual_stride, y, M, N, static_cast<int>(K), activation,
+            static_cast<int *>(workspace), p.splits, p.run};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("linear_int8", st);
+  if (copy) {
+    const int64_t pitch = pitch_of(K);
+    int8_t *rows = static_cast<int8_t *>(workspace) + part_bytes(p, M, N);
+    const AlignArgs c{codes, weight, codes_stride, weight_stride, rows, M, M + N,
+                      static_cast<int>(K), static_cast<int>(pitch)};
+    linear_align<<<static_cast<unsigned>(cdiv((M + N) * (pitch / 16), 256)), 256, 0, st>>>(c);
+    a.x = rows;
+    a.w = rows + M * pitch;
+    a.x_stride = a.w_stride = pitch;
+    a.K = static_cast<int>(pitch);  // p was made for K: its last part takes what K's end adds
+  }
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
     switch (p.shape) {
       case kFew:
         linear_few<T><<<static_cast<unsigned>(cdiv(N, 16)), 64 * kFewWaves, 0, st>>>(a);
         break;
-      case k64x32: launch_tile<T, 64, 32, 2, 1>(a, whole, st); break;
-      case k64x64: launch_tile<T, 64, 64, 2, 2>(a, whole, st); break;
-      case k64x128: launch_tile<T, 64, 128, 2, 2>(a, whole, st); break;
-      case k128x128: launch_tile<T, 128, 128, 2, 2>(a, whole, st); break;
-      case k256x128: launch_tile<T, 256, 128, 4, 2>(a, whole, st); break;
-      case k256x256: launch_tile<T, 256, 256, 2, 4>(a, whole, st); break;
+      case k64x32: launch_tile<T, 64, 32, 2, 1>(a, st); break;
+      case k64x64: launch_tile<T, 64, 64, 2, 2>(a, st); break;
+      case k64x128: launch_tile<T, 64, 128, 2, 2>(a, st); break;
+      case k128x128: launch_tile<T, 128, 128, 2, 2>(a, st); break;
+      case k256x128: launch_tile<T, 256, 128, 4, 2>(a, st); break;
+      case k256x256: launch_tile<T, 256, 256, 2, 4>(a, st); break;
     }
     if (p.splits > 1)
       linear_join<T><<<static_cast<unsigned>(cdiv(M * cdiv(N, 4), 256)), 256, 0, st>>>(a);

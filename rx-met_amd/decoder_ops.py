@@ -229,7 +229,8 @@ def linear_int8(codes, scales, weight, weight_scales, bias=None, activation: Opt
     codes int8 [..., K] with scales float32 [...] (from ``rms_norm_quantize`` /
     ``quantize_rows``); weight int8 [N, K] with weight_scales float32 [N]; bias [N] and residual
     [..., N] in ``dtype``.  activation: None, "relu", "silu" or "gelu" (with the error function).
-    The sum over K is exact, the rest float32.  K is at most 131071.
+    The sum over K is exact, the rest float32.  K is at most 131071.  Rows that do not start on 16 bytes
+    (K no multiple of 16) are copied first where there are more than 16 rows of codes.
     """
     ext = _ext or _native()
     if ext and activation in ACTIVATIONS:
@@ -268,7 +269,8 @@ def linear_int8(codes, scales, weight, weight_scales, bias=None, activation: Opt
         _like(residual, "residual", dtype, dev, (*lead, N))
         r2, rs = _rows(residual)
     y = torch.empty((*lead, N), dtype=dtype, device=dev)
-    size = _rx.load().rxmet_linear_int8_workspace_bytes(M, N, K)
+    size = _rx.load().rxmet_linear_int8_workspace_bytes(x2.data_ptr(), xs, w2.data_ptr(),
+                                                           wst, M, N, K)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     with torch.cuda.device(dev):
         _rx.call("rxmet_linear_int8", x2.data_ptr(), xs, sx.data_ptr(), w2.data_ptr(), wst,

@@ -131,7 +131,7 @@ _SIGNATURES = {
     "rxmet_rms_quantize_backward": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, _i32,
                                             c_ptr, c_ptr, c_ptr, c_i64, c_i64, _i32, c_ptr,
                                             c_ptr]),
-    "rxmet_linear_int8_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "rxmet_linear_int8_workspace_bytes": (c_i64, [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_i64]),
     "rxmet_linear_int8": (c_int, [c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64,
                                   c_ptr, c_i64, c_i64, c_i64, _i32, _i32, c_ptr, c_ptr]),
     "rxmet_kv_append": (c_int, [_KVC, _KVT, c_ptr, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64,

@@ -202,7 +202,8 @@ py::object linear_int8(const Tensor &codes, const Tensor &scales, const Tensor &
     return py::none();
   const c10::DeviceGuard guard(codes.device());
   const Tensor y = at::empty(shape, codes.options().dtype(type));
-  const int64_t bytes = linear_bytes(M, N, K);
+  const int64_t bytes = linear_bytes(codes.const_data_ptr<int8_t>(), xs,
+                                     weight.const_data_ptr<int8_t>(), ws, M, N, K);
   Tensor work;
   if (bytes > 0) work = at::empty({bytes}, codes.options().dtype(at::kByte));
   check(linear(codes.const_data_ptr<int8_t>(), xs, scales.const_data_ptr<float>(),
