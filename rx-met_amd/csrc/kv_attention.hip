@@ -181,6 +181,7 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
     const Seen top = seen_by(a, seq.length, seq.n, rt * kRows / G);  // the tile's first and last query
     const int last = rt * kRows + kRows - 1 < rows ? rt * kRows + kRows - 1 : rows - 1;
     const Seen bot = seen_by(a, seq.length, seq.n, last / G);
+    const unsigned wide = me.hi > me.lo ? me.hi - me.lo : 0;
     const int begin = (top.lo & ~(kGroup - 1)) + split * a.chunk;
     const int end = split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
 
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int tok = tv + 4 * t + r;
-            s[t][r] = tok >= me.lo && tok < me.hi ? s[t][r] : -INFINITY;
+            s[t][r] = static_cast<unsigned>(tok - me.lo) < wide ? s[t][r] : -INFINITY;
           }
         if (tv + 16 <= me.lo || tv >= me.hi) vs = 0.0f;  // 0 times a hidden page's NaN is no 0
       }
@@ -343,9 +344,9 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many query rows: 128 rows of one cache head, 32 to a wave, on mfma 32x32x16 (lane = (col, h),
+// Many query rows: 32 W rows of one cache head, 32 to a wave, on mfma 32x32x16 (lane = (col, h),
 // col = lane % 32, h = lane / 32).  The workgroup brings 64 tokens at a time into LDS as fp16, so that the
-// codes are converted once for all 128 rows, while the next 64 are on their way.  As above,
+// codes are converted once for all the rows, while the next 64 are on their way.  As above,
 // S^T = K Q^T with row i of tile t standing for token 32 t + 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4, so that a lane holds
 // 16 consecutive tokens of one page a tile, and the weights are the second product's operand
 // where they are.  The weights are 2^(s f - m + log2(vs / R)): vs / R costs nothing for each weight, and l takes it
@@ -353,17 +354,17 @@ __global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
 // 8 above it, which leaves weights below 2^8 and spares most rescalings of the sums.
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr int kTileRows = 128;
-
 __device__ __forceinline__ v16f mfma32_f16(v8h a, v8h b, v16f c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArgs a) {
+template <typename T, int D, int W, bool WIDE>
+__global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const AttnArgs a) {
+  constexpr int tile = 32 * W, threads = 64 * W;
   constexpr int KC = D / 16, NU = D / 32;   // steps of the first product, tiles of the second
   constexpr int kp = kGroup + 1, vp = D + 1;  // pitches in units of 16 bytes
-  constexpr int pieces = D * kGroup / 16 / 256;  // of keys and of values for each thread
+  constexpr int all = D * kGroup / 16;        // pieces of 16 codes of the keys, and of the values
+  constexpr int pieces = (all + threads - 1) / threads;
   struct Stage {
     uint4 k[D / 8 * kp];  // [8 dimensions][row of the tiles]
     uint4 v[8 * vp];      // [8 tokens][dimension]
@@ -377,14 +378,24 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
   const Sequence seq = sequence_of(a, b);
   const int rows = seq.rows, slot = blockIdx.x / a.splits;
   const int32_t *ids = a.g.t.ids + b * a.g.t.stride;
+  // where a thread's pieces lie in a page: keys of token i / (D / 16), values of tokens 16 * (i % 4)
+  const int page_bytes = H * P * D;
+  unsigned kat[pieces], vat[pieces];
+#pragma unroll
+  for (int j = 0; j < pieces; ++j) {
+    const int i = tid + threads * j;
+    kat[j] = head * P * D + (i / (D / 16) & (P - 1)) * D + i % (D / 16) * 16;
+    vat[j] = head * P * D + i / 4 * P + (i % 4 * 16 & (P - 1));
+  }
   // the last rows see the most tokens: they go first
-  for (int rt = a.row_tiles - 1 - slot; rt * kTileRows < rows; rt += a.row_tiles) {
-    const int r0 = rt * kTileRows, w0 = r0 + wave * 32;
+  for (int rt = a.row_tiles - 1 - slot; rt * tile < rows; rt += a.row_tiles) {
+    const int r0 = rt * tile, w0 = r0 + wave * 32;
     auto seen = [&](int r) { return seen_by(a, seq.length, seq.n, (r < rows ? r : rows - 1) / G); };
-    const Seen top = seen(r0), bot = seen(r0 + kTileRows - 1), wtop = seen(w0), wbot = seen(w0 + 31);
+    const Seen top = seen(r0), bot = seen(r0 + tile - 1), wtop = seen(w0), wbot = seen(w0 + 31);
     const int row = w0 + col;
     const bool valid = row < rows;
     const Seen me = seen(row);
+    const unsigned wide = me.hi > me.lo ? me.hi - me.lo : 0;
     const int begin = (top.lo & ~(kGroup - 1)) + split * a.chunk;
     const int end = split == a.splits - 1 || bot.hi < begin + a.chunk ? bot.hi : begin + a.chunk;
 
@@ -407,64 +418,74 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
       for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
     float m = -INFINITY, l = 0.0f, ref = 1.0f, inv_ref = 1.0f;
 
-    // Staging.  Piece i = tid + 256 j: keys of token i / (D / 16), values of the 16 tokens i % 4.
+    // Staging.  Piece i = tid + threads * j.
     uint4 kw[pieces], vw[pieces];
     float ks = 0.0f, vs = 0.0f;
     int ik[pieces], iv;
     auto look_up = [&](int t0) {
+      if constexpr (WIDE) {
+        iv = page_id(a, ids, t0, end, shift);
+      } else {
 #pragma unroll
-      for (int j = 0; j < pieces; ++j)
-        ik[j] = page_id(a, ids, t0 + (tid + 256 * j) / (D / 16), end, shift);
-      iv = page_id(a, ids, t0 + tid % 4 * 16, end, shift);
+        for (int j = 0; j < pieces; ++j)
+          ik[j] = page_id(a, ids, t0 + (tid + threads * j) / (D / 16), end, shift);
+        iv = page_id(a, ids, t0 + tid % 4 * 16, end, shift);
+      }
     };
     auto fetch = [&](int t0) {
-      const int64_t vat = static_cast<int64_t>(in_cache(a, iv) ? iv : 0) * H + head;
-      const int tv = t0 + tid % 4 * 16;
+      const int in = t0 & (P - 1);
+      if constexpr (WIDE) iv = __builtin_amdgcn_readfirstlane(iv);
+      const int64_t pv = in_cache(a, iv) ? iv : 0;
+      const int8_t *kpage = a.g.c.k + pv * page_bytes + in * D;
+      const int8_t *vpage = a.g.c.v + pv * page_bytes + in;
 #pragma unroll
       for (int j = 0; j < pieces; ++j) {
-        const int i = tid + 256 * j, t = t0 + i / (D / 16);
-        const int64_t kat = static_cast<int64_t>(in_cache(a, ik[j]) ? ik[j] : 0) * H + head;
-        kw[j] = *reinterpret_cast<const uint4 *>(a.g.c.k + kat * P * D + (t & (P - 1)) * D +
-                                                 i % (D / 16) * 16);
-        vw[j] = *reinterpret_cast<const uint4 *>(a.g.c.v + vat * P * D + i / 4 * P + (tv & (P - 1)));
+        if (all % threads == 0 || tid + threads * j < all) {
+          if constexpr (!WIDE)
+            kpage = a.g.c.k + static_cast<int64_t>(in_cache(a, ik[j]) ? ik[j] : 0) * page_bytes;
+          kw[j] = *reinterpret_cast<const uint4 *>(kpage + kat[j]);
+          vw[j] = *reinterpret_cast<const uint4 *>(vpage + vat[j]);
+        }
       }
       if (tid < 4) {
-        ks = a.g.c.k_scale[vat];
-        vs = a.g.c.v_scale[vat];
+        ks = a.g.c.k_scale[pv * H + head];
+        vs = a.g.c.v_scale[pv * H + head];
         if (!in_cache(a, iv)) ks = vs = nanf32();
-        if (tv >= end) ks = vs = 0.0f;
+        if (t0 + 16 * tid >= end) ks = vs = 0.0f;
       }
     };
     auto put = [&](Stage &s) {
 #pragma unroll
       for (int j = 0; j < pieces; ++j) {
-        const int i = tid + 256 * j;
-        {
-          const int t = i / (D / 16), d = i % (D / 16) * 2;
+        const int i = tid + threads * j;
+        if (all % threads == 0 || i < all) {
+          const int t = i / (D / 16), dk = i % (D / 16) * 2;
           const int r = (t & 32) + (t >> 4 & 1) * 4 + (t >> 2 & 3) * 8 + (t & 3);
-          s.k[d * kp + r] = __builtin_bit_cast(uint4, codes_f16(kw[j].x, kw[j].y));
-          s.k[(d + 1) * kp + r] = __builtin_bit_cast(uint4, codes_f16(kw[j].z, kw[j].w));
-        }
-        {
-          const int c = i % 4 * 2, d = i / 4;
-          s.v[c * vp + d] = __builtin_bit_cast(uint4, codes_f16(vw[j].x, vw[j].y));
-          s.v[(c + 1) * vp + d] = __builtin_bit_cast(uint4, codes_f16(vw[j].z, vw[j].w));
+          s.k[dk * kp + r] = __builtin_bit_cast(uint4, codes_f16(kw[j].x, kw[j].y));
+          s.k[(dk + 1) * kp + r] = __builtin_bit_cast(uint4, codes_f16(kw[j].z, kw[j].w));
+          const int c = i % 4 * 2, dv = i / 4;
+          s.v[c * vp + dv] = __builtin_bit_cast(uint4, codes_f16(vw[j].x, vw[j].y));
+          s.v[(c + 1) * vp + dv] = __builtin_bit_cast(uint4, codes_f16(vw[j].z, vw[j].w));
         }
       }
       if (tid < 4) s.ks[tid] = ks, s.vs[tid] = vs;
     };
 
-    auto step = [&](int t0, const Stage &s) {  // one group of 64 tokens
-      v16f st[2];
+    v16f st[2];
+    auto scores = [&](const Stage &s) {  // one group of 64 tokens
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[t][r] = 0.0f;
+      // neighbouring products do not wait for each other's sums
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
           st[t] = mfma32_f16(__builtin_bit_cast(v8h, s.k[(2 * c + h) * kp + 32 * t + col]), q[c],
                              st[t]);
-      }
+    };
+    auto weigh = [&](int t0, const Stage &s) {
       float f[2], v[2], high = -INFINITY, big = 0.0f;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -479,7 +500,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
           const int t1 = t0 + 32 * t + 16 * h;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            st[t][r] = t1 + r >= me.lo && t1 + r < me.hi ? st[t][r] : -INFINITY;
+            st[t][r] = static_cast<unsigned>(t1 + r - me.lo) < wide ? st[t][r] : -INFINITY;
           if (t1 + 16 <= me.lo || t1 >= me.hi) f[t] = v[t] = 1.0f;  // a hidden page's may be NaN
         }
       }
@@ -527,9 +548,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
         l += sum * __builtin_amdgcn_rcpf(ratio);
       }
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int u = 0; u < NU; ++u) {
           // weights c: tokens 32 (c / 2) + 16 h + 8 (c % 2) + 0..7
           const int chunk = 4 * (c / 2) + 2 * h + c % 2;
           acc[u] = mfma32_f16(__builtin_bit_cast(v8h, s.v[chunk * vp + 32 * u + col]), p[c], acc[u]);
@@ -543,17 +564,18 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_tile(const AttnArg
       put(stage[0]);
     }
     __syncthreads();
-    int buf = 0;
-    for (int t0 = begin; t0 < end; t0 += kGroup, buf ^= 1) {
+    int now = 0;
+    for (int t0 = begin; t0 < end; t0 += kGroup, now ^= 1) {
       const bool more = t0 + kGroup < end;
       if (more) {
         fetch(t0 + kGroup);
         look_up(t0 + 2 * kGroup);
       }
       if (t0 < wbot.hi && t0 + kGroup > wtop.lo && w0 < rows) {
-        step(t0, stage[buf]);
+        scores(stage[now]);
+        weigh(t0, stage[now]);
       }
-      if (more) put(stage[buf ^ 1]);
+      if (more) put(stage[now ^ 1]);
       __syncthreads();
     }
 
@@ -639,23 +661,23 @@ __global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
 struct Plan {
   int64_t row_tiles, chunk;
   int splits;
-  bool tile;  // attn_tile, else attn_rows
+  int waves;  // of attn_tile; 0: attn_rows
 };
 
 // Chunks of the token axis: enough workgroups to fill the GPU (four for each of 256 CUs), each
 // with at least 512 tokens, eight groups, so that its start and its sums' join stay small beside them.
 Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t queries, int64_t max_query,
-              int64_t max_length, int64_t window) {
+              int64_t max_length, int64_t window, int32_t dim) {
   if (max_query > queries) max_query = queries;
   if (max_length > kMost) max_length = kMost;
   Plan p;
   const int64_t rows = (max_query < 1 ? 1 : max_query) * group;
-  p.tile = rows >= 64;
-  p.row_tiles = cdiv(rows, p.tile ? kTileRows : kRows);
+  p.waves = rows < 64 ? 0 : dim <= 128 && cdiv(rows, 256) * heads * seqs >= 256 ? 8 : 4;
+  p.row_tiles = cdiv(rows, p.waves ? 32 * p.waves : kRows);
   int64_t span = max_length;
   if (window > 0 && window + max_query + kGroup < span) span = window + max_query + kGroup;
   const int64_t tiles = p.row_tiles * heads * seqs;
-  int64_t splits = cdiv(1024, tiles < 1 ? 1 : tiles);
+  int64_t splits = cdiv(p.waves ? 2048 / p.waves : 1024, tiles < 1 ? 1 : tiles);
   if (splits > cdiv(span, 512)) splits = cdiv(span, 512);
   if (splits < 1) splits = 1;
   p.chunk = cdiv(cdiv(span, splits), kWaves * kGroup) * (kWaves * kGroup);
@@ -677,7 +699,7 @@ extern "C" int64_t rxmet_kv_attention_workspace_bytes(const rxmet_kv_cache *cach
                                                       int64_t window) {
   if (!cache || cache->heads < 1 || q_heads < cache->heads || queries <= 0 || seqs <= 0) return 0;
   const Plan p = plan_for(cache->heads, seqs, q_heads / cache->heads, queries, max_query,
-                          max_length, window);
+                          max_length, window, cache->dim);
   return p.splits == 1 ? 0 : p.splits * queries * q_heads * (cache->dim + 2) * 4;
 }
 
@@ -704,7 +726,8 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
   const int group = q_heads / cache->heads;
   int64_t cap = static_cast<int64_t>(table->cols) * cache->page_size;
   if (cap > kMost) cap = kMost;
-  const Plan p = plan_for(cache->heads, table->seqs, group, queries, max_query, max_length, window);
+  const Plan p = plan_for(cache->heads, table->seqs, group, queries, max_query, max_length, window,
+                          cache->dim);
   if (window > INT32_MAX) window = 0;  // hides nothing
   RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
   RXMET_CHECK_ARG(p.row_tiles * p.splits <= INT32_MAX, "too many query rows for one call");
@@ -721,10 +744,18 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
   prof::Scope scope("kv_attention", st);
   auto launch = [&](auto t, auto dim) {
     using T = decltype(t);
-    if (p.tile)
-      attn_tile<T, dim.value><<<grid, 256, 0, st>>>(a);
-    else
+    const bool wide = cache->page_size >= kGroup;
+    if (p.waves == 4) {
+      if (wide) attn_tile<T, dim.value, 4, true><<<grid, 256, 0, st>>>(a);
+      else attn_tile<T, dim.value, 4, false><<<grid, 256, 0, st>>>(a);
+    } else if (p.waves == 8) {
+      if constexpr (dim.value <= 128) {
+        if (wide) attn_tile<T, dim.value, 8, true><<<grid, 512, 0, st>>>(a);
+        else attn_tile<T, dim.value, 8, false><<<grid, 512, 0, st>>>(a);
+      }
+    } else {
       attn_rows<T, dim.value><<<grid, 256, 0, st>>>(a);
+    }
     if (p.splits > 8)
       attn_join<T, dim.value, kWaves><<<static_cast<unsigned>(rows), 256, 0, st>>>(a);
     else if (p.splits > 1)

@@ -268,6 +268,27 @@ def test_prompts(cuda, dim, page, group, causal, window, dtype):
                     max_query=max(new), max_length=max(totals))
 
 
+@pytest.mark.parametrize("dim,page,group", [(64, 64, 9), (128, 16, 8), (128, 128, 16), (256, 64, 8)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_many_prompts(cuda, dim, page, group, window):
+    """As many query rows as fill the GPU: the largest tiles.  Rows of a part of the sequences are
+    compared with the definition, all of them with single calls."""
+    seqs, new = 130, [33 - b % 5 for b in range(130)]
+    totals = [n + 17 * (b % 9) for b, n in enumerate(new)]
+    table, pages = table_for(totals, page, 1, cuda)
+    cache = fill(cuda, pages, 2, dim, page, 2)
+    q = queries(cuda, sum(new), 2 * group, dim, torch.bfloat16)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    out = ops.kv_cache_attention(q, cache, table, ints(totals, cuda), ints(starts, cuda),
+                                 max_query=max(new), max_length=max(totals), window=window)
+    for b in (0, 7, 129):
+        rows = slice(starts[b], starts[b + 1])
+        got = check_attention(cuda, cache, table[b:b + 1], totals[b:b + 1], new[b:b + 1], q[rows],
+                              window=window)
+        # another tile and other chunks: fp16 weights and bf16 results of both
+        assert torch.allclose(out[rows].float(), got.float(), rtol=2.0 ** -7, atol=4e-3 * float(got.float().abs().max()))
+
+
 def test_queries_before_the_first_token_see_nothing(cuda):
     """More queries than tokens: those that stand before the first token give 0."""
     table, pages = table_for([3], 64, 1, cuda)
