@@ -57,13 +57,55 @@ __device__ __forceinline__ void store8_part(T *p, int n, const float (&f)[8]) {
 
 // The code of v, |v| < 2^22, in the low byte: adding 1.5 * 2^23 rounds half to even into the last
 // bits of the sum.  A NaN gives 0.
-__device__ __forceinline__ unsigned code_byte(float v) {
-  return __builtin_bit_cast(unsigned, v + 12582912.0f) & 0xffu;
+__device__ __forceinline__ unsigned code_word(float v) {
+  return __builtin_bit_cast(unsigned, v + 12582912.0f);
 }
 
 __device__ __forceinline__ unsigned code_bytes4(float a, float b, float c, float d) {
-  return code_byte(a) | code_byte(b) << 8 | code_byte(c) << 16 | code_byte(d) << 24;
+  const unsigned lo = __builtin_amdgcn_perm(code_word(b), code_word(a), 0x0c0c0400u);
+  return lo | __builtin_amdgcn_perm(code_word(d), code_word(c), 0x04000c0cu);
 }
+
+// The largest magnitude as an integer: without their signs, floats are ordered as their bits are,
+// infinity above all numbers and NaN above infinity, so that a maximum of bits keeps a NaN.
+__device__ __forceinline__ unsigned magnitude(float v) {
+  return __builtin_bit_cast(unsigned, v) & 0x7fffffffu;
+}
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) {
+    const unsigned o = __shfl_xor(v, off, kWave);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// Largest magnitude of vectors of eight, as fp32 bits once asked for: two 16-bit values a step.
+template <typename T>
+struct Peak {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {0, 0};
+  __device__ __forceinline__ void add(const Vec8<T> &v) {
+    unsigned w[4];
+    __builtin_memcpy(w, &v, 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[k] & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ unsigned bits() const {
+    const unsigned short t = top[0] > top[1] ? top[0] : top[1];
+    return magnitude(static_cast<float>(__builtin_bit_cast(T, t)));
+  }
+};
+template <>
+struct Peak<float> {
+  unsigned top = 0;
+  __device__ __forceinline__ void add(const Vec8<float> &v) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = __builtin_elementwise_max(top, magnitude(v.v[k]));
+  }
+  __device__ __forceinline__ unsigned bits() const { return top; }
+};
 
 // Byte k of a word as a signed code.
 __device__ __forceinline__ float code_value(unsigned w, int k) {

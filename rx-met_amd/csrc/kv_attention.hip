@@ -193,7 +193,7 @@ __device__ __forceinline__ int load_query(const T *q, bool valid, At at, Join jo
 // Sixteen query rows of one cache head, one chunk of their tokens.  The waves take groups of 64
 // tokens in turn and join their sums in LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_rows(const AttnArgs a) {
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_rows(const AttnArgs a) {
   constexpr int NC = D / 64, NU = D / 16, pitch = D + 4;
   __shared__ float s_acc[kWaves][kRows][pitch];
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];

@@ -27,13 +27,14 @@ struct AppendArgs {
   int64_t stride_t[2], stride_h[2];
 };
 
-__device__ __forceinline__ float block_max(float v) {
-  __shared__ float s[4];
-  v = wave_max(v);
+__device__ __forceinline__ float block_max(unsigned v) {
+  __shared__ unsigned s[4];
+  v = wave_max_bits(v);
   __syncthreads();  // the last page's maxima have been read
   if (threadIdx.x % kWave == 0) s[threadIdx.x / kWave] = v;
   __syncthreads();
-  return nan_max(nan_max(s[0], s[1]), nan_max(s[2], s[3]));
+  const unsigned a = s[0] > s[1] ? s[0] : s[1], b = s[2] > s[3] ? s[2] : s[3];
+  return __builtin_bit_cast(float, a > b ? a : b);
 }
 
 // Four codes of an old page on its new grid.
@@ -74,7 +75,7 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
     int8_t *codes = pool + at * P * D;
     const float was = s0 > 0 ? scales[at] : 0.0f;
     Vec8<T> u[NU][4];
-    float top = 0.0f;
+    Peak<T> peak;
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
       const int i = tid + 256 * j, c = i % C, q = i / C * 4;
@@ -88,10 +89,8 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
 #pragma unroll
     for (int j = 0; j < NU; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int d = 0; d < 8; ++d) top = nan_max(top, fabsf(static_cast<float>(u[j][e].v[d])));
-    top = block_max(top);
+      for (int e = 0; e < 4; ++e) peak.add(u[j][e]);
+    const float top = block_max(peak.bits());
     // block_max's barriers stand between every thread's read of the old scale and this write
     const bool good = top <= 3.402823466e38f && was == was;
     const float fresh = fmaxf(top, kFloor) * kInv127;

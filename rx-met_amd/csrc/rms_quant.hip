@@ -28,23 +28,25 @@ struct RowArgs {
   float eps;
 };
 
-// Sum and NaN-keeping maximum over the TPR threads of a row.
+// Sum, and maximum of magnitudes as bits, over the TPR threads of a row.
 template <int TPR>
-__device__ __forceinline__ void row_reduce(float &sum, float &top) {
+__device__ __forceinline__ void row_reduce(float &sum, unsigned &top) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    sum += __shfl_xor(sum, off, kWave);
-    top = nan_max(top, __shfl_xor(top, off, kWave));
-  }
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+  top = wave_max_bits(top);
   if constexpr (TPR > kWave) {
     constexpr int waves = TPR / kWave;
-    __shared__ float s_sum[waves], s_top[waves];
+    __shared__ float s_sum[waves];
+    __shared__ unsigned s_top[waves];
     const int wave = threadIdx.x / kWave;
     if (threadIdx.x % kWave == 0) s_sum[wave] = sum, s_top[wave] = top;
     __syncthreads();
     sum = s_sum[0], top = s_top[0];
 #pragma unroll
-    for (int k = 1; k < waves; ++k) sum += s_sum[k], top = nan_max(top, s_top[k]);
+    for (int k = 1; k < waves; ++k) {
+      sum += s_sum[k];
+      top = s_top[k] > top ? s_top[k] : top;
+    }
   }
 }
 
@@ -58,7 +60,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
   const T *res = a.res ? static_cast<const T *>(a.res) + row * a.res_stride : nullptr;
   const W *w = static_cast<const W *>(a.w);
   float u[NV][8];
-  float sum = 0.0f, top = 0.0f;
+  float sum = 0.0f;
+  unsigned bits = 0;
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = (v * TPR + tid) * 8, n = a.cols - c;
@@ -94,9 +97,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = nan_max(top, fabsf(u[v][e]));
+    for (int e = 0; e < 8; ++e) bits = __builtin_elementwise_max(bits, magnitude(u[v][e]));
   }
-  row_reduce<TPR>(sum, top);
+  row_reduce<TPR>(sum, bits);
+  const float top = __builtin_bit_cast(float, bits);
   const float rstd = w ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : 1.0f;
   const bool good = top <= 3.402823466e38f;
   const float peak = fmaxf(top, kFloor);
@@ -158,7 +162,8 @@ __global__ __launch_bounds__(TPR) void rms_backward(const BackArgs a) {
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float rstd = a.rstd[row];
     float n[NV][8], dn[NV][8];
-    float dot = 0.0f, none = 0.0f;
+    float dot = 0.0f;
+    unsigned none = 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * TPR + tid) * 8, m = a.cols - c;
