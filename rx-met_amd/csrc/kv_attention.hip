@@ -763,7 +763,7 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
   if (window > INT32_MAX) window = 0;  // hides nothing
   RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
   const int64_t jobs = p.row_tiles * p.splits * cache->heads;
-  RXMET_CHECK_ARG(jobs <= INT32_MAX && jobs * table->seqs <= INT32_MAX, "too many query rows for one call");
+  RXMET_CHECK_ARG(jobs < 1 << 23 && jobs * table->seqs < 1 << 23, "too many query rows for one call");
   const int64_t rows = queries * q_heads;
   float *part = static_cast<float *>(workspace);
   const AttnArgs a{{*cache, *table}, lengths, cu_query, static_cast<int>(queries), query,

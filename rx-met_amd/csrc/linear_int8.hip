@@ -460,7 +460,7 @@ extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, cons
                                  void *workspace, void *stream) {
   RXMET_CHECK_ARG(M >= 0 && N >= 1 && K >= 1 && K <= RXMET_LINEAR_INT8_K_MAX,
                   "M must be >= 0, N >= 1 and K between 1 and 131071");
-  RXMET_CHECK_ARG(M <= INT32_MAX && N <= INT32_MAX, "M and N must be below 2^31");
+  RXMET_CHECK_ARG(M <= 1 << 26 && N <= 1 << 26, "M and N must be at most 2^26");
   RXMET_CHECK_ARG(activation >= RXMET_ACT_NONE && activation <= RXMET_ACT_GELU,
                   "unknown activation");
   RXMET_CHECK_ARG(dtype == RXMET_QDQ_F32 || dtype == RXMET_QDQ_F16 || dtype == RXMET_QDQ_BF16,
@@ -468,12 +468,12 @@ extern "C" int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, cons
   if (M == 0) return 0;
   RXMET_CHECK_ARG(codes && scales && weight && weight_scales && y,
                   "codes, weight, their scales and y are needed");
-  RXMET_CHECK_ARG(cdiv(M, 16) * cdiv(N, 64) <= INT32_MAX / 64, "too many outputs for one call");
+  RXMET_CHECK_ARG(cdiv(M, 32) * cdiv(N, 64) < 1 << 23, "too many outputs for one call");
   const Plan p = plan_for(M, N, K);
   const bool copy = p.shape != kFew && !aligned(codes, codes_stride, weight, weight_stride);
   RXMET_CHECK_ARG((p.splits == 1 && !copy) || workspace, "this call needs a workspace");
   RXMET_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
-  RXMET_CHECK_ARG(cdiv((M + N) * (pitch_of(K) / 16), 256) <= INT32_MAX, "too many rows for one call");
+  RXMET_CHECK_ARG(!copy || (M + N) * (pitch_of(K) / 16) < 1LL << 32, "too many rows to copy");
   LinArgs a{codes, weight, codes_stride, weight_stride, scales, weight_scales, bias,
             residual, residual_stride, y, M, N, static_cast<int>(K), activation,
             static_cast<int *>(workspace), p.splits, p.run};

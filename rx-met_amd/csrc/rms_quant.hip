@@ -23,7 +23,7 @@ struct RowArgs {
   int8_t *codes;
   void *y;
   float *scales, *rstd;
-  int64_t rows;
+  int64_t rows, row0;  // row0: of the tensors, where a launch takes a part of the rows
   int cols;
   float eps;
 };
@@ -53,9 +53,10 @@ __device__ __forceinline__ void row_reduce(float &sum, unsigned &top) {
 template <typename T, typename W, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowArgs a) {
   constexpr int block = TPR < 256 ? 256 : TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (block / TPR) + threadIdx.x / TPR;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (block / TPR) + threadIdx.x / TPR;
   const int tid = threadIdx.x % TPR;
-  if (row >= a.rows) return;  // whole waves (TPR = 64) or none: no barrier follows for them
+  if (at >= a.rows) return;  // whole waves (TPR = 64) or none: no barrier follows for them
+  const int64_t row = a.row0 + at;
   const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
   const T *res = a.res ? static_cast<const T *>(a.res) + row * a.res_stride : nullptr;
   const W *w = static_cast<const W *>(a.w);
@@ -304,14 +305,20 @@ extern "C" int rxmet_rms_quantize_forward(const void *x, int64_t x_stride, const
   RXMET_CHECK_ARG(x && scales && (codes || y), "x, scales and codes or y are needed");
   RXMET_CHECK_ARG(!residual || (weight && h), "a residual needs a weight and h");
   const RowArgs a{x, residual, weight, x_stride, residual_stride, h, codes, y, scales, rstd,
-                  rows, static_cast<int>(cols), eps};
+                  rows, 0, static_cast<int>(cols), eps};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("rms_quantize_forward", st);
   with_weight_type(dtype, weight_f32, [&](auto t, auto w) {
     with_row_shape(cols, [&](auto tpr, auto nv) {
       constexpr int block = tpr.value < 256 ? 256 : tpr.value;
-      const unsigned grid = static_cast<unsigned>(cdiv(rows, block / tpr.value));
-      rms_forward<decltype(t), decltype(w), tpr.value, nv.value><<<grid, block, 0, st>>>(a);
+      constexpr int64_t most = 1 << 21;  // rows of a launch, whose threads number below 2^32
+      for (int64_t r = 0; r < rows; r += most) {
+        RowArgs part = a;
+        part.rows = rows - r < most ? rows - r : most;
+        part.row0 = r;
+        const unsigned grid = static_cast<unsigned>(cdiv(part.rows, block / tpr.value));
+        rms_forward<decltype(t), decltype(w), tpr.value, nv.value><<<grid, block, 0, st>>>(part);
+      }
     });
   });
   RXMET_CHECK_LAUNCH();

@@ -183,6 +183,9 @@ def test_read_of_what_has_no_page(cuda):
     key, value = ops.kv_cache_read(cache, ints([[1, -1]], cuda), ints([14], cuda), ints([0, 30], cuda), 30)
     for t in (key, value):
         assert torch.isfinite(t[:2]).all() and torch.isnan(t[2:]).all()
+    key, value = ops.kv_cache_read(cache, ints([[1, 2]], cuda), ints([-20], cuda), ints([0, 30], cuda), 30)
+    for t in (key, value):
+        assert torch.isnan(t[:20]).all() and torch.isfinite(t[20:]).all()
 
 
 def test_round_trip_holds_half_a_step(cuda):
@@ -216,7 +219,7 @@ def check_attention(cuda, cache, table, totals, new, q, cu=True, causal=True, wi
         for h in range(heads):
             rows = slice(starts[b], starts[b + 1]), slice(h * G, (h + 1) * G)
             want, off = O.attention(qd[rows], k[:, h], ks[:, h], v[:, h], vs[:, h], total,
-                                    scale or 1 / math.sqrt(dim), causal, window or 0)
+                                    1 / math.sqrt(dim) if scale is None else scale, causal, window or 0)
             tol = off + HALF_ULP[dtype] * np.abs(want) + 2.0 ** -24
             most = torch.finfo(dtype).max  # what lies beyond it rounds to an infinity
             with np.errstate(invalid="ignore"):
@@ -344,6 +347,17 @@ def test_large_and_small_queries(cuda, dtype, size):
         q = q.clamp(-6e4, 6e4)
     q[0, 1] = 0
     check_attention(cuda, cache, table, totals, [1, 1], q.to(dtype), cu=False, scale=0.1 / size)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scale_of_zero_and_below(cuda, new, scale):
+    """All tokens alike, and the least alike first; partly hidden groups among them."""
+    totals = [100, 64]
+    table, pages = table_for(totals, 64, 1, cuda)
+    cache = fill(cuda, pages, 1, 64, 64, 2)
+    q = queries(cuda, 2 * new, 4, 64, torch.float16)
+    check_attention(cuda, cache, table, totals, [new, new], q, scale=scale)
 
 
 def test_not_finite_stays_where_it_is_seen(cuda):

@@ -178,6 +178,17 @@ def test_gradients_that_do_not_arrive(cuda):
     assert w.grad is None
 
 
+def test_more_rows_than_a_launch_takes(cuda):
+    """Rows beyond the 2^21 of one launch; the last ones as a call of their own gives them."""
+    rows = (1 << 21) + 37
+    x = torch.randn(rows, 8, generator=torch.Generator().manual_seed(1)).half().to(cuda)
+    codes, scales = ops.quantize_rows(x)
+    tail, tail_scales = ops.quantize_rows(x[-40:])
+    assert torch.equal(codes[-40:], tail) and torch.equal(scales[-40:], tail_scales)
+    exact, _ = O.quantize_rows(f64(x[:50]))
+    check_codes(codes[:50], exact)
+
+
 def test_side_stream_and_same_bits(cuda):
     """Tensors made on another stream than the call's; the same bits on every run."""
     x, r, w = make(64, 4099, torch.bfloat16, 11, cuda)
