@@ -349,11 +349,10 @@ struct AlignArgs {
 };
 
 __global__ __launch_bounds__(256) void linear_align(const AlignArgs a) {
-  const int pieces = a.pitch / 16;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const unsigned pieces = a.pitch / 16, i = blockIdx.x * 256 + threadIdx.x;  // below 2^32
   if (i >= a.rows * pieces) return;
   const int64_t row = i / pieces;
-  const int k = static_cast<int>(i % pieces) * 16;
+  const int k = i % pieces * 16;
   const int8_t *p = row < a.M ? a.x + row * a.x_stride : a.w + (row - a.M) * a.w_stride;
   *reinterpret_cast<uint4 *>(a.out + row * a.pitch + k) = load_piece(p, k, a.K);
 }
