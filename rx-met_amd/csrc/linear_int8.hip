@@ -254,20 +254,21 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
       xat[j][c] = (TN + row) * kStep + ((2 * c + h) ^ turn_x(row)) * 16;
     }
   }
-  auto compute = [&](const int8_t *buf) {
+  struct Half {  // the operands of half a step
+    v4i w[FN], x[FM];
+  };
+  auto load = [&](Half &f, const int8_t *buf, int c) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      v4i wf[FN], xf[FM];
+    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const v4i *>(buf + wat[i][c]);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) wf[i] = *reinterpret_cast<const v4i *>(buf + wat[i][c]);
+    for (int j = 0; j < FM; ++j) f.x[j] = *reinterpret_cast<const v4i *>(buf + xat[j][c]);
+  };
+  auto multiply = [&](const Half &f) {
 #pragma unroll
-      for (int j = 0; j < FM; ++j) xf[j] = *reinterpret_cast<const v4i *>(buf + xat[j][c]);
+    for (int i = 0; i < FN; ++i)
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
-    }
+      for (int j = 0; j < FM; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
   };
   auto issue = [&](int step, int slot) {
 #pragma unroll
@@ -277,12 +278,20 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
   if (whole > 0) {
     // past the end a step is read once more, so that the count of loads in flight holds
 #pragma unroll
-    for (int k = 0; k < ring - 1; ++k) issue(k < whole ? k : 0, k);
+    for (int k = 0; k < ring; ++k) issue(k < whole ? k : 0, k);
+    wait_loads<(ring - 1) * loads>();
+    meet();
+    // each half's operands are read from LDS while the half before is multiplied
+    Half even, odd;
+    load(even, s[0], 0);
     for (int k = 0; k < whole; ++k) {
+      load(odd, s[k % ring], 1);
+      multiply(even);
       wait_loads<(ring - 2) * loads>();
-      meet();  // step k is there for all, and step k - 1 has been read by all
-      issue(k + ring - 1 < whole ? k + ring - 1 : k, (k + ring - 1) % ring);
-      compute(s[k % ring]);
+      meet();  // step k + 1 is there for all, and step k has been read by all
+      issue(k + ring < whole ? k + ring : k, k % ring);
+      load(even, s[(k + 1) % ring], 0);
+      multiply(odd);
     }
     wait_loads<0>();
   }
@@ -295,7 +304,11 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
           load_piece(src[j] + whole * kStep - k, k, a.K - from * kStep);
     }
     __syncthreads();
-    compute(s[0]);
+    Half f;
+    load(f, s[0], 0);
+    multiply(f);
+    load(f, s[0], 1);
+    multiply(f);
     __syncthreads();
   }
 
