@@ -201,7 +201,7 @@ __device__ __forceinline__ int load_query(const T *q, bool valid, At at, Join jo
 // Sixteen query rows of one cache head, one chunk of their tokens.  The waves take groups of 64
 // tokens in turn and join their sums in LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attn_rows(const AttnArgs a) {
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArgs a) {
   constexpr int NC = D / 64, NU = D / 16, pitch = D + 4;
   __shared__ float s_acc[kWaves][kRows][pitch];
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
@@ -707,7 +707,8 @@ struct Plan {
 // Chunks of the token axis: for attn_rows eight workgroups for each of 256 CUs, so that ragged
 // lengths even out (64 sequences of up to 16384 tokens, 8 heads: 286 us, with four 297, with sixteen 284),
 // each with at least 512 tokens, eight groups, so that its start and its sums' join stay small
-// beside them; for attn_tile as many as are resident at once.
+// beside them; for attn_tile as many as are resident at once, with at least 256 tokens (385 queries
+// of three heads over 3256 tokens, dim 256: 51 us with 512, 40 with 256).
 //
 // From 64 query rows on attn_tile runs, which reads and converts each token once for 128 or 256 rows:
 // 8 heads, 6144 and 2217 tokens, 2048 and 1226 queries of 4 heads each: 235 us, attn_rows 741. 256 rows take turns
@@ -724,7 +725,8 @@ Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t queries, int64
   if (window > 0 && window + max_query + kGroup < span) span = window + max_query + kGroup;
   const int64_t tiles = p.row_tiles * heads * seqs;
   int64_t splits = cdiv(p.waves ? 2048 / p.waves : 2048, tiles < 1 ? 1 : tiles);
-  if (splits > cdiv(span, 512)) splits = cdiv(span, 512);
+  const int64_t least = p.waves ? 256 : 512;
+  if (splits > cdiv(span, least)) splits = cdiv(span, least);
   if (splits < 1) splits = 1;
   p.chunk = cdiv(cdiv(span, splits), kWaves * kGroup) * (kWaves * kGroup);
   if (p.chunk < 1) p.chunk = kWaves * kGroup;
