@@ -11,6 +11,8 @@
 // of two, which keeps all of its bits.  The weights are rounded to fp16 (11 bits) once, as p * vs / R:
 // R is a running reference near the scales of the pages at hand (within a factor of 8 above the
 // largest of each 64 tokens), so that pages of any scale keep their bits; the sums are in units of R.
+// Weights and l carry a common power of two (kLift) until the end: without it a weight 2^-25 of its
+// row's largest would round to 0 in fp16, and many such beside one large one make a sum that counts.
 //
 // Layout.  With mfma 16x16x32 (lane = (col, g), col = lane % 16, g = lane / 16) the first product is
 // taken as S^T = K Q^T on 64 tokens: row i of tile t stands for token 16 * (i / 4) + 4 t + i % 4, so that
@@ -40,6 +42,8 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 constexpr int kRows = 16;   // query rows of a workgroup: one column of the matrix instruction each
 constexpr int kGroup = 64;  // tokens that a wave takes at a time
 constexpr int kWaves = 4;
+// log2 of the weights' factor: the largest stays below 2^15 (attn_tile's may be 2^8 above its reference).
+constexpr float kLiftRows = 14.0f, kLiftTile = 7.0f;
 
 struct AttnArgs {
   Pages g;
@@ -290,7 +294,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
 #pragma unroll
         for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][r]);
       high = fmaxf(m, col_max(high));
-      const float base = high == -INFINITY ? 0.0f : high;
+      const float base = high == -INFINITY ? 0.0f : high, lifted = base - kLiftRows;
       const float alpha = exp2f(m - base);
       m = high;
       float fix = alpha;  // and the reference of the weights' rounding
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[t][r] - base);
+          const float e = __builtin_amdgcn_exp2f(s[t][r] - lifted);
           l += e;
           p[t / 2][4 * (t % 2) + r] = static_cast<_Float16>(e * ratio);
         }
@@ -336,7 +340,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
     }
 
     // the four waves' sums on one maximum
-    l = col_sum(l);
+    l = col_sum(l) * exp2f(-kLiftRows);
     if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
     __syncthreads();
     float all = s_m[0][col];
@@ -345,7 +349,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
     const float mine = exp2f(m - (all == -INFINITY ? 0.0f : all)) * ref;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
-      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = acc[u] * mine;
+      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = acc[u] * exp2f(-kLiftRows) * mine;
     __syncthreads();
     constexpr int per = D / 16;  // elements of a thread: 16 threads a row
     const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * per;
@@ -570,12 +574,12 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[u][r] *= fix;
       }
-      const float base = m == -INFINITY ? 0.0f : m;
+      const float base = (m == -INFINITY ? 0.0f : m) - kLiftTile;
       v8h p[4];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         float ratio = v[t] * inv_ref;
-        ratio = ratio < 0x1p-40f ? 0x1p-40f : ratio;  // below that: rounds to 0 anyway
+        ratio = ratio < 0x1p-48f ? 0x1p-48f : ratio;  // below that: rounds to 0 anyway
         const float c = __builtin_amdgcn_logf(ratio) - base;
         float sum = 0.0f;
 #pragma unroll
@@ -619,7 +623,8 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
       __syncthreads();
     }
 
-    l += __shfl_xor(l, 32, kWave);
+    l = (l + __shfl_xor(l, 32, kWave)) * exp2f(-kLiftTile);
+    ref *= exp2f(-kLiftTile);
     if (valid) {
       const int64_t place = static_cast<int64_t>(seq.q0 + row / G) * a.q_heads + head * G + row % G;
       const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;

@@ -336,6 +336,26 @@ def test_scales_far_apart(cuda):
     check_attention(cuda, small, table, totals, [1], q, cu=False)
 
 
+@pytest.mark.parametrize("group,lift", [(1, 14), (64, 7)])
+def test_many_small_weights_beside_a_large_one(cuda, group, lift):
+    """One token with the weight 1 and the value 0, and 65535 with 2^-26.5 and 100: what is kept of each is
+    2^-11 of itself or 2^-25 of the factor 2^lift that the weights carry; the result is rounded once more."""
+    n, w = 65536, 2.0 ** -26.5
+    table, pages = table_for([n], 64, 1, cuda)
+    k = torch.zeros(pages, 1, 64, 64, dtype=torch.int8, device=cuda)
+    k[table[0, 0].long(), 0, 0, 0] = 127
+    v = torch.full((pages, 1, 64, 64), 100, dtype=torch.int8, device=cuda)
+    v[table[0, 0].long(), 0, :, 0] = 0
+    ones = torch.ones(pages, 1, device=cuda)
+    q = torch.zeros(1, group, 64, dtype=torch.float16, device=cuda)
+    q[:, :, 0] = 1
+    out = ops.kv_cache_attention(q, ops.KVCache(k, v, ones, ones), table, ints([n], cuda), max_length=1,
+                                 scale=26.5 * math.log(2) / 127)
+    want = 100 * (n - 1) * w / (1 + (n - 1) * w)
+    tol = want * (2.0 ** -11 + 2.0 ** -11 + 2.0 ** -16) + 100 * n * 2.0 ** (-25 - lift)
+    assert np.abs(f64(out) - want).max() <= tol
+
+
 @pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 1e30), (torch.bfloat16, 1e-30), (torch.float16, 6e4)])
 def test_large_and_small_queries(cuda, dtype, size):
     """Rows outside fp16's range keep their bits; the scale brings the scores back."""
