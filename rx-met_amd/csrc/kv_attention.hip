@@ -25,7 +25,7 @@
 // tokens, 8 heads, 64 query heads: 1356 MB in 281 us (4.8 TB/s; a copy of 2 GiB reaches 4.9); two of 32768 and 16679 tokens,
 // 32 query heads: 101 MB in 24 us and 4.7 us for the join of 64 chunks.  attn_tile: the issue of a
 // SIMD's two waves, of whose time the matrix unit has 40 % and the vector unit 54 % (exponentials,
-// conversions): 204 GFLOP in 235 us, 867 TFLOP/s, where a large library product reaches 1385.  64 rows a
+// conversions): 204 GFLOP in 235 to 255 us by card, 867 to 800 TFLOP/s, where a large library product reaches 1385.  64 rows a
 // wave (half the LDS reads) spill and take 512 us; waves half a turn apart, a higher priority for the
 // products, and products placed among the exponentials by hand change nothing or cost 4 to 6 %.
 #include <type_traits>

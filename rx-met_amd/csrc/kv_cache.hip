@@ -11,7 +11,7 @@
 //
 // Bound: HBM traffic for prompts (each new token read once, its codes written), the launch and three dependent
 // reads (length, page, codes) for single tokens.  Measured, bf16, 8 heads of 128, pages of 64: 28098
-// tokens of 8 prompts in 41 us (173 MB, 4.2 TB/s), read back in 29 us (172 MB, 6.0 TB/s); one token for
+// tokens of 8 prompts in 41 us (173 MB, 4.2 TB/s; 50 us where the tokens come from HBM), read back in 29 us (172 MB, 6.0 TB/s); one token for
 // each of 64 sequences 7.5 us, their open pages read back in 8.8 us.
 #include <type_traits>
 
