@@ -11,8 +11,11 @@
 //
 // Bound: HBM traffic for prompts (each new token read once, its codes written), the launch and three dependent
 // reads (length, page, codes) for single tokens.  Measured, bf16, 8 heads of 128, pages of 64: 28098
-// tokens of 8 prompts in 41 us (173 MB, 4.2 TB/s; 50 us where the tokens come from HBM), read back in 29 us (172 MB, 6.0 TB/s); one token for
-// each of 64 sequences 7.5 us, their open pages read back in 8.8 us.
+// tokens of 8 prompts in 45 us (173 MB, 3.8 TB/s, the tokens in no cache), read back in 31 us (172 MB,
+// 5.5 TB/s); one token for each of 64 sequences 6.0 us, their open pages read back in 7.2 us.
+// Neighbouring workgroups have neighbouring heads, so that those at work together read whole rows of the
+// tokens (pages first: 50, 30, 6.8 and 9.4 us; 20 sequences of 500 to 1000 tokens, 3 heads of 64, pages of 16:
+// 24 and 13.5 us then, 20.5 and 12.4 so).
 #include <type_traits>
 
 #include "kv_cache.h"
@@ -54,7 +57,8 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
   constexpr int units = P / 4 * C, NU = (units + 255) / 256;
   constexpr int pitch = P / 4 + 1;                      // words of a dimension in LDS
   __shared__ unsigned s_v[D * pitch];
-  const int b = blockIdx.y, which = blockIdx.z & 1, head = blockIdx.z >> 1, tid = threadIdx.x;
+  const int heads = a.g.c.heads, b = blockIdx.z, which = static_cast<int>(blockIdx.x) >= heads, tid = threadIdx.x;
+  const int head = blockIdx.x - which * heads;
   const int64_t start = a.lengths[b];
   const int64_t row0 = a.cu ? a.cu[b] : b;
   int64_t count = a.cu ? a.cu[b + 1] - row0 : 1;
@@ -66,7 +70,7 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
   float *scales = which ? a.g.c.v_scale : a.g.c.k_scale;
   const int64_t stride = a.stride_t[which];
   const T *x = static_cast<const T *>(a.x[which]) + head * a.stride_h[which];
-  for (int64_t p = first + blockIdx.x; p <= last; p += gridDim.x) {
+  for (int64_t p = first + blockIdx.y; p <= last; p += gridDim.y) {
     const int64_t page = page_of(a.g, b, p);
     if (page < 0) continue;
     // new tokens stand in slots s0..s1-1, older ones below s0
@@ -173,7 +177,8 @@ struct ReadArgs {
 
 template <typename T, int D, int P>
 __global__ __launch_bounds__(256) void kv_read(const ReadArgs a) {
-  const int b = blockIdx.y, which = blockIdx.z & 1, head = blockIdx.z >> 1, tid = threadIdx.x;
+  const int heads = a.g.c.heads, b = blockIdx.z, which = static_cast<int>(blockIdx.x) >= heads, tid = threadIdx.x;
+  const int head = blockIdx.x - which * heads;
   const int64_t start = a.first[b], row0 = a.cu[b];
   int64_t count = a.cu[b + 1] - row0;
   if (row0 < 0) return;
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(256) void kv_read(const ReadArgs a) {
   const int64_t end = start + count, last = end > 0 ? (end - 1) / P : -((-end + P) / P);
   const int64_t pitch = static_cast<int64_t>(a.g.c.heads) * D;
   T *out = static_cast<T *>(a.out[which]) + head * D;
-  for (int64_t p = first + blockIdx.x; p <= last; p += gridDim.x) {
+  for (int64_t p = first + blockIdx.y; p <= last; p += gridDim.y) {
     const int64_t page = page_of(a.g, b, p);
     const int s0 = static_cast<int>(p == first ? start - p * P : 0);
     const int s1 = static_cast<int>(p == last ? end - p * P : P);
@@ -289,8 +294,8 @@ extern "C" int rxmet_kv_append(const rxmet_kv_cache *cache, const rxmet_kv_table
                      {key_stride_t, value_stride_t}, {key_stride_h, value_stride_h}};
   // n >= 1 tokens touch at most (n + P - 2) / P + 1 pages
   const int64_t pages = (max_new + cache->page_size - 2) / cache->page_size + 1;
-  const dim3 grid(static_cast<unsigned>(pages < 65536 ? pages : 65536), table->seqs,
-                  2 * cache->heads);
+  const dim3 grid(2 * cache->heads, static_cast<unsigned>(pages < 65535 ? pages : 65535),
+                  table->seqs);
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("kv_append", st);
   with_type(dtype, [&](auto t) {
@@ -314,8 +319,8 @@ extern "C" int rxmet_kv_read(const rxmet_kv_cache *cache, const rxmet_kv_table *
   RXMET_CHECK_ARG(first && cu && key && value, "first, cu, key and value are needed");
   const ReadArgs a{{*cache, *table}, first, cu, tokens, {key, value}};
   const int64_t pages = (max_tokens + cache->page_size - 2) / cache->page_size + 1;
-  const dim3 grid(static_cast<unsigned>(pages < 65536 ? pages : 65536), table->seqs,
-                  2 * cache->heads);
+  const dim3 grid(2 * cache->heads, static_cast<unsigned>(pages < 65535 ? pages : 65535),
+                  table->seqs);
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("kv_read", st);
   with_type(dtype, [&](auto t) {
