@@ -1,4 +1,4 @@
-"""Checker of the 8-bit decoder operators: their definitions in 64 bits, in numpy.
+"""Oracle of the 8-bit decoder operators: their definitions in 64 bits, in numpy.
 
 Inputs are arrays that hold the operators' inputs exactly (fp16 / bf16 / fp32 values as float64,
 int8 codes); nothing here knows tiles, splits or matrix instructions.

@@ -1,4 +1,4 @@
-"""The 8-bit decoder operators without a GPU: their checker against itself, and what the library
+"""The 8-bit decoder operators without a GPU: their oracle against itself, and what the library
 refuses before any device call."""
 import ctypes
 
@@ -11,7 +11,7 @@ import decoder_oracle as O
 import rxmet_lib
 
 
-def test_checker_gradient_is_the_smooth_norms_derivative():
+def test_oracle_gradient_is_the_smooth_norms_derivative():
     rng = np.random.default_rng(0)
     h, w, dy = rng.standard_normal((3, 17)), rng.standard_normal(17), rng.standard_normal((3, 17))
     dx, dw = O.rms_backward(h, w, 1e-3, dy, None)
@@ -21,8 +21,8 @@ def test_checker_gradient_is_the_smooth_norms_derivative():
         assert abs((f(t) - f(-t)) / (2 * t) - (dx * a).sum() - (dw * b).sum()) < 1e-7
 
 
-def test_checker_sees_a_planted_mistake():
-    """The comparison that the GPU tests make fails where the checker's own sums leave a term out."""
+def test_oracle_sees_a_planted_mistake():
+    """The comparison that the GPU tests make fails where the oracle's own sums leave a term out."""
     rng = np.random.default_rng(1)
     h, w, dy = rng.standard_normal((3, 40)), rng.standard_normal(40), rng.standard_normal((3, 40))
     dx, _ = O.rms_backward(h, w, 1e-6, dy, None)
@@ -31,7 +31,7 @@ def test_checker_sees_a_planted_mistake():
     assert np.abs(dx - without).max() > 1e-2
 
 
-def test_checker_codes_do_not_go_by_the_norm():
+def test_oracle_codes_do_not_go_by_the_norm():
     rng = np.random.default_rng(2)
     h, w = rng.standard_normal((4, 33)), rng.standard_normal(33)
     q, scale, rstd = O.rms_quantize(h, w, 1e-6)
@@ -39,7 +39,7 @@ def test_checker_codes_do_not_go_by_the_norm():
     assert np.allclose(np.abs(q).max(-1), 127)
 
 
-def test_checker_attention_on_one_token():
+def test_oracle_attention_on_one_token():
     v = np.arange(4.0)[None]
     out, _ = O.attention(np.ones((1, 2, 4)), np.ones((1, 4)), np.ones(1), v, np.full(1, 0.5), 1, 1.0,
                          True, 0)
