@@ -8,9 +8,11 @@
 //
 // Precision.  An int8 code is exact in fp16, so both products run on the fp16 matrix instruction
 // with the codes themselves and the scales stay outside.  A query row is brought to [-2, 2) by a power
-// of two, which keeps all of its bits.  The weights are rounded to fp16 (11 bits) once, as p * vs / R:
-// R is a running reference near the scales of the pages at hand (within a factor of 8 above the
-// largest of each 64 tokens), so that pages of any scale keep their bits; the sums are in units of R.
+// of two, which keeps all of its bits.  The weights are rounded to fp16 (11 bits) once, with their value
+// scales in them: as 2^(s - m) vs / 2^d, where 2^d is a running reference of the row's own, like m, that
+// follows the largest 2^(s - m) vs which the row has seen.  It never falls below what the sums hold, so
+// that they stay finite beside pages of any scale (a page of zeros has 2^-119), and pages that the
+// row does not see do not move it.  The weighted sums are in units of 2^d, l in units of 1.
 // Weights and l carry a common power of two (kLift) until the end: without it a weight 2^-25 of its
 // row's largest would round to 0 in fp16, and many such beside one large one make a sum that counts.
 //
@@ -42,8 +44,12 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 constexpr int kRows = 16;   // query rows of a workgroup: one column of the matrix instruction each
 constexpr int kGroup = 64;  // tokens that a wave takes at a time
 constexpr int kWaves = 4;
-// log2 of the weights' factor: the largest stays below 2^15 (attn_tile's may be 2^8 above its reference).
-constexpr float kLiftRows = 14.0f, kLiftTile = 7.0f;
+// log2 of the weights' factor: the largest stays below 2^15 (attn_tile's may be 2^8 above its reference;
+// attn_rows multiplies by a scale's mantissa below 1).
+constexpr float kLiftRows = 15.0f, kLiftTile = 7.0f;
+// Least reference d, below the exponent of every scale, and the least log2(vs) - d that is told apart: with
+// it a weight's rounding gives 0, and l, which takes the factor out again, keeps its bits.
+constexpr float kLeast = -200.0f, kApart = -48.0f;
 
 struct AttnArgs {
   Pages g;
@@ -243,7 +249,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
     v4f acc[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) acc[u] = v4f{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f, ref = 1.0f, inv_ref = 1.0f;
+    // maximum, largest weight times scale (log2, relative to m), and d, the next whole number above it
+    float m = -INFINITY, l = 0.0f, peak = -INFINITY, d = kLeast;
 
     auto step = [&](int t0, int ik, int iv) {  // one group of 64 tokens
       const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * g;
@@ -274,7 +281,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
         }
       }
       const float f = ks * q_scale;
-      const float big = col_max(vs == vs ? vs : 0.0f);
 #pragma unroll
       for (int t = 0; t < 4; ++t) s[t] *= f;
       if (t0 < bot.lo || t0 + kGroup > top.hi) {  // some row does not see all 64
@@ -288,38 +294,41 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
           }
         if (tv + 16 <= me.lo || tv >= me.hi) vs = 0.0f;  // 0 times a hidden page's NaN is no 0
       }
-      float high = -INFINITY;
+      // vs = mant * 2^ex; the lane's 16 tokens lie in one page
+      const float mant = __builtin_amdgcn_frexp_mantf(vs);
+      const float ex = vs == 0.0f ? kLeast : static_cast<float>(__builtin_amdgcn_frexp_expf(vs));
+      float own = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][r]);
-      high = fmaxf(m, col_max(high));
-      const float base = high == -INFINITY ? 0.0f : high, lifted = base - kLiftRows;
-      const float alpha = exp2f(m - base);
-      m = high;
-      float fix = alpha;  // and the reference of the weights' rounding
-      if (big > 0.0f && (big > ref || big * 8.0f < ref)) {
-        fix *= ref / big;
-        ref = big;
-        inv_ref = 1.0f / big;
-      }
-      if (__any(fix != 1.0f)) {
+        for (int r = 0; r < 4; ++r) own = fmaxf(own, s[t][r]);
+      if (__any(own > m || (own - m) + ex > d)) {  // a row's maximum or reference moves
+        const float high = fmaxf(m, col_max(own));
+        const float base = high == -INFINITY ? 0.0f : high, delta = m - base;
+        m = high;
+        peak = fmaxf(peak + delta, col_max((own - base) + ex));
+        const float next = fmaxf(ceilf(peak), kLeast);
+        const float fix = exp2f((d - next) + delta);
+        d = next;
+        l *= exp2f(delta);
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[u][r] *= fix;
       }
-      l *= alpha;
-      const float ratio = vs * inv_ref;
+      const float part = fmaxf(ex - d, kApart);  // whole: l loses nothing when it is taken out again
+      const float lifted = (m == -INFINITY ? 0.0f : m) - (kLiftRows + part);
+      float sum = 0.0f;
       v8h p[2];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float e = __builtin_amdgcn_exp2f(s[t][r] - lifted);
-          l += e;
-          p[t / 2][4 * (t % 2) + r] = static_cast<_Float16>(e * ratio);
+          sum += e;
+          p[t / 2][4 * (t % 2) + r] = static_cast<_Float16>(e * mant);
         }
+      l += __builtin_amdgcn_ldexpf(sum, -static_cast<int>(part));
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         acc[u] = mfma_f16(codes_f16(vw[u].x, vw[u].y), p[0], acc[u]);
@@ -341,15 +350,16 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
 
     // the four waves' sums on one maximum
     l = col_sum(l) * exp2f(-kLiftRows);
+    d -= kLiftRows;
     if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
     __syncthreads();
     float all = s_m[0][col];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) all = fmaxf(all, s_m[w][col]);
-    const float mine = exp2f(m - (all == -INFINITY ? 0.0f : all)) * ref;
+    const float mine = exp2f(d + (m - (all == -INFINITY ? 0.0f : all)));
 #pragma unroll
     for (int u = 0; u < NU; ++u)
-      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = acc[u] * exp2f(-kLiftRows) * mine;
+      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = acc[u] * mine;
     __syncthreads();
     constexpr int per = D / 16;  // elements of a thread: 16 threads a row
     const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * per;
@@ -392,9 +402,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
 // codes are converted once for all the rows, while the next 64 are on their way.  As above,
 // S^T = K Q^T with row i of tile t standing for token 32 t + 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4, so that a lane holds
 // 16 consecutive tokens of one page a tile, and the weights are the second product's operand
-// where they are.  The weights are 2^(s f - m + log2(vs / R)): vs / R costs nothing for each weight, and l takes it
-// out again once for 16 of them.  The reference m follows the maximum only when that is more than
-// 8 above it, which leaves weights below 2^8 and spares most rescalings of the sums.
+// where they are.  The weights are 2^(s f - m + log2(vs) - d): vs costs nothing for each weight, and l takes
+// it out again once for 16 of them.  The references m and d follow the largest only when that is more
+// than 8 above them, which leaves weights below 2^8 and spares most rescalings of the sums.
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ v16f mfma32_f16(v8h a, v8h b, v16f c) {
@@ -411,7 +421,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
   struct Stage {
     uint4 k[D / 8 * kp];  // [8 dimensions][row of the tiles]
     uint4 v[8 * vp];      // [8 tokens][dimension]
-    float ks[4], vs[4];   // of 16 tokens each
+    float ks[4], lv[4];   // of 16 tokens each: key scale, log2 of the value scale
   };
   __shared__ Stage stage[2];
   const int tid = threadIdx.x, lane = tid % kWave, wave = wave_id();
@@ -460,7 +470,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f, ref = 1.0f, inv_ref = 1.0f;
+    float m = -INFINITY, l = 0.0f, peak = -INFINITY, d = kLeast;  // as in attn_rows
 
     // Staging.  Piece i = tid + threads * j.
     uint4 kw[pieces], vw[pieces];
@@ -512,7 +522,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
           s.v[(c + 1) * vp + dv] = __builtin_bit_cast(uint4, codes_f16(vw[j].z, vw[j].w));
         }
       }
-      if (tid < 4) s.ks[tid] = ks, s.vs[tid] = vs;
+      if (tid < 4) s.ks[tid] = ks, s.lv[tid] = __builtin_amdgcn_logf(vs);
     };
 
     v16f st[2];
@@ -530,12 +540,12 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
                              st[t]);
     };
     auto weigh = [&](int t0, const Stage &s) {
-      float f[2], v[2], high = -INFINITY, big = 0.0f;
+      float f[2], v[2], x[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         f[t] = s.ks[2 * t + h] * q_scale;
         f[t] = f[t] < 0x1p-126f ? 0x1p-126f : f[t];  // so that -inf stays -inf
-        v[t] = s.vs[2 * t + h];
+        v[t] = s.lv[2 * t + h];
       }
       if (t0 < wbot.lo || t0 + kGroup > wtop.hi) {  // some row does not see all 64
         asm volatile("");  // stays a branch: few groups need it
@@ -545,30 +555,28 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             st[t][r] = static_cast<unsigned>(t1 + r - me.lo) < wide ? st[t][r] : -INFINITY;
-          if (t1 + 16 <= me.lo || t1 >= me.hi) f[t] = v[t] = 1.0f;  // a hidden page's may be NaN
+          if (t1 + 16 <= me.lo || t1 >= me.hi) f[t] = 1.0f, v[t] = 0.0f;  // a hidden page's may be NaN
         }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        float x = st[t][0];
+        x[t] = st[t][0];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) x = fmaxf(x, st[t][r]);
-        high = fmaxf(high, x * f[t]);
+        for (int r = 1; r < 16; ++r) x[t] = fmaxf(x[t], st[t][r]);
+        x[t] *= f[t];
       }
-      high = fmaxf(high, __shfl_xor(high, 32, kWave));
-#pragma unroll
-      for (int t = 0; t < 4; ++t) big = fmaxf(big, s.vs[t]);
-      const bool turn = big > 0.0f && (big > ref || big * 8.0f < ref);
-      if (__any(high > m + 8.0f) || turn) {
-        const float was = m;
-        m = fmaxf(m, high);
-        float fix = exp2f(was - (m == -INFINITY ? 0.0f : m));
-        l *= fix;
-        if (turn) {
-          fix *= ref / big;
-          ref = big;
-          inv_ref = 1.0f / big;
-        }
+      if (__any(fmaxf(x[0], x[1]) > m + 8.0f || fmaxf((x[0] - m) + v[0], (x[1] - m) + v[1]) > d + 8.0f)) {
+        float high = fmaxf(x[0], x[1]);
+        high = fmaxf(m, fmaxf(high, __shfl_xor(high, 32, kWave)));
+        const float base = high == -INFINITY ? 0.0f : high, delta = m - base;
+        m = high;
+        float up = fmaxf((x[0] - base) + v[0], (x[1] - base) + v[1]);
+        up = fmaxf(up, __shfl_xor(up, 32, kWave));
+        peak = fmaxf(peak + delta, up);
+        const float next = fmaxf(ceilf(peak), kLeast);
+        const float fix = exp2f((d - next) + delta);
+        d = next;
+        l *= exp2f(delta);
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -578,9 +586,9 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
       v8h p[4];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        float ratio = v[t] * inv_ref;
-        ratio = ratio < 0x1p-48f ? 0x1p-48f : ratio;  // below that: rounds to 0 anyway
-        const float c = __builtin_amdgcn_logf(ratio) - base;
+        float part = v[t] - d;
+        part = part < kApart ? kApart : part;  // a NaN stays one
+        const float c = part - base;
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -589,7 +597,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
           sum += e;
           p[2 * t + r / 8][r % 8] = static_cast<_Float16>(e);
         }
-        l += sum * __builtin_amdgcn_rcpf(ratio);
+        l += sum * __builtin_amdgcn_exp2f(-part);
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c)
@@ -624,7 +632,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
     }
 
     l = (l + __shfl_xor(l, 32, kWave)) * exp2f(-kLiftTile);
-    ref *= exp2f(-kLiftTile);
+    const float ref = exp2f(d - kLiftTile);
     if (valid) {
       const int64_t place = static_cast<int64_t>(seq.q0 + row / G) * a.q_heads + head * G + row % G;
       const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;
