@@ -13,7 +13,7 @@
 // follows the largest 2^(s - m) vs which the row has seen.  It never falls below what the sums hold, so
 // that they stay finite beside pages of any scale (a page of zeros has 2^-119), and pages that the
 // row does not see do not move it.  The weighted sums are in units of 2^d, l in units of 1.
-// Weights and l carry a common power of two (kLift) until the end: without it a weight 2^-25 of its
+// Weights and l carry a common power of two (kLift): without it a weight 2^-25 of its
 // row's largest would round to 0 in fp16, and many such beside one large one make a sum that counts.
 //
 // Layout.  With mfma 16x16x32 (lane = (col, g), col = lane % 16, g = lane / 16) the first product is
@@ -62,7 +62,7 @@ struct AttnArgs {
   int causal;
   int window, chunk, splits, row_tiles, cap;
   void *out;
-  float *part, *stats;  // [splits, queries * q_heads, D] and [.., 2]: used where splits > 1
+  float *part, *stats;  // [splits, queries * q_heads, D] and [.., 2]: averages, maxima and l, where splits > 1
 };
 
 // Eight codes (two words) as fp16: 0x6400 | u is 1024 + u, and u is the code + 128.
@@ -348,48 +348,55 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
       iv = nv;
     }
 
-    // the four waves' sums on one maximum
-    l = col_sum(l) * exp2f(-kLiftRows);
-    d -= kLiftRows;
+    // The four waves' sums on one maximum, as averages: each sum is divided by the row's whole l before
+    // anything is added to it, because values near the type's largest have no room for more.
+    l = col_sum(l);
     if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
     __syncthreads();
-    float all = s_m[0][col];
+    float all = s_m[0][col], total = 0.0f;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) all = fmaxf(all, s_m[w][col]);
-    const float mine = exp2f(d + (m - (all == -INFINITY ? 0.0f : all)));
+    const float base = all == -INFINITY ? 0.0f : all;
 #pragma unroll
-    for (int u = 0; u < NU; ++u)
-      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = acc[u] * mine;
+    for (int w = 0; w < kWaves; ++w) total += s_l[w][col] * __builtin_amdgcn_exp2f(s_m[w][col] - base);
+    const float unit = fmaxf(d + (m - base), -1000.0f);  // log2 of what this wave's sums count
+    // of row r's values in `out` or, for this chunk, in `part` and `stats`
+    auto place_of = [&](int r) {
+      return static_cast<int64_t>(seq.q0 + r / G) * a.q_heads + head * G + r % G;
+    };
+    const int64_t chunk0 = static_cast<int64_t>(split) * a.queries * a.q_heads;
+    if (a.splits > 1 && wave == 0 && g == 0 && valid) {
+      float *stats = a.stats + 2 * (chunk0 + place_of(row));
+      stats[0] = all, stats[1] = total;
+    }
+    const float whole = rintf(unit);
+    const float mine = total == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(unit - whole) / total;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      v4f o = acc[u] * mine;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = __builtin_amdgcn_ldexpf(o[r], static_cast<int>(whole));
+      *reinterpret_cast<v4f *>(&s_acc[wave][col][16 * u + 4 * g]) = o;
+    }
     __syncthreads();
     constexpr int per = D / 16;  // elements of a thread: 16 threads a row
     const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * per;
     const int orow = rt * kRows + r;
     if (orow < rows) {
-      float best = s_m[0][r], total = 0.0f;
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) best = fmaxf(best, s_m[w][r]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w)
-        total += s_l[w][r] * exp2f(s_m[w][r] - (best == -INFINITY ? 0.0f : best));
-      const int64_t place = static_cast<int64_t>(seq.q0 + orow / G) * a.q_heads + head * G + orow % G;
+      const int64_t place = place_of(orow);
       float o[per];
 #pragma unroll
       for (int e = 0; e < per; ++e)
         o[e] = s_acc[0][r][d0 + e] + s_acc[1][r][d0 + e] + s_acc[2][r][d0 + e] +
                s_acc[3][r][d0 + e];
       if (a.splits == 1) {
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         T *out = static_cast<T *>(a.out) + place * D + d0;
 #pragma unroll
-        for (int e = 0; e < per; ++e) out[e] = static_cast<T>(o[e] * inv);
-      } else {
-        const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;
-        if (d0 == 0) a.stats[2 * at] = best, a.stats[2 * at + 1] = total;
-        if (begin < end) {
-          float *part = a.part + at * D + d0;
+        for (int e = 0; e < per; ++e) out[e] = static_cast<T>(o[e]);
+      } else if (begin < end) {
+        float *part = a.part + (chunk0 + place) * D + d0;
 #pragma unroll
-          for (int e = 0; e < per; ++e) part[e] = o[e];
-        }
+        for (int e = 0; e < per; ++e) part[e] = o[e];
       }
     }
     __syncthreads();  // the next tile writes the LDS again
@@ -631,12 +638,12 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
       __syncthreads();
     }
 
-    l = (l + __shfl_xor(l, 32, kWave)) * exp2f(-kLiftTile);
-    const float ref = exp2f(d - kLiftTile);
+    l += __shfl_xor(l, 32, kWave);  // its lift is that of the sums
+    const int unit = static_cast<int>(d);
     if (valid) {
       const int64_t place = static_cast<int64_t>(seq.q0 + row / G) * a.q_heads + head * G + row % G;
       const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;
-      const float f = a.splits > 1 ? ref : l == 0.0f ? 0.0f : ref / l;
+      const float f = l == 0.0f ? 0.0f : 1.0f / l;
       if (a.splits > 1 && h == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
       if (a.splits == 1 || begin < end) {
 #pragma unroll
@@ -650,7 +657,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
             v4f w;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              w[e] = acc[u][4 * k + e] * f;
+              w[e] = __builtin_amdgcn_ldexpf(acc[u][4 * k + e] * f, unit);
               o.v[e] = static_cast<T>(w[e]);
             }
             if (a.splits > 1)
@@ -663,8 +670,9 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
   }
 }
 
-// Joins the chunks of a row in the chunks' order: W waves take every W-th chunk, lane by lane of
-// the row.  A chunk in which the row sees nothing has l = 0 and its sums were never written.
+// Joins the chunks of a row, averages with their maxima and sums l, in the chunks' order: W waves take
+// every W-th chunk, lane by lane of the row.  A chunk in which the row sees nothing has l = 0 and its
+// averages were never written.
 template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
   constexpr int E = D / 64;
@@ -683,11 +691,12 @@ __global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, kWave);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   float o[E] = {};
 #pragma unroll 4
   for (int s = W == 1 ? 0 : wave; s < a.splits; s += W) {
     const int64_t at = s * rows + row;
-    const float l = a.stats[2 * at + 1], f = exp2f(a.stats[2 * at] - base);
+    const float l = a.stats[2 * at + 1], f = l * exp2f(a.stats[2 * at] - base) * inv;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float v = a.part[at * D + 64 * e + lane];
@@ -705,10 +714,9 @@ __global__ __launch_bounds__(256) void attn_join(const AttnArgs a) {
 #pragma unroll
       for (int w = 1; w < W; ++w) o[e] += s_o[w][64 * e + lane];
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   T *out = static_cast<T *>(a.out) + row * D + lane;
 #pragma unroll
-  for (int e = 0; e < E; ++e) out[64 * e] = static_cast<T>(o[e] * inv);
+  for (int e = 0; e < E; ++e) out[64 * e] = static_cast<T>(o[e]);
 }
 
 struct Plan {

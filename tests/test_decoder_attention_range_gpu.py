@@ -149,3 +149,16 @@ def test_a_light_loud_page_beside_a_heavy_quiet_one(cuda, n, group):
                                  scale=math.log(2))
     want = f64(cache.v[0, 0]).mean(1)  # page 1 adds 2^-100 * 2^60 * 127 at most
     assert np.abs(f64(out[-1]) - want).max() <= 2.0 ** -7 * 127
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("total", [100, 5000])
+@pytest.mark.parametrize("exponent", [120, -119])
+def test_values_at_the_ends_of_the_range(cuda, exponent, total, n, group):
+    """Averages near the largest and the least values, whose sums lie beyond fp32."""
+    pages = -(-total // 64)
+    cache = codes_cache(cuda, pages, 1, 128, 64)
+    cache.v.copy_(cache.v.abs().clamp(min=100))  # all of one sign: nothing cancels
+    cache.v_scale.fill_(2.0 ** exponent)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+    check(cuda, cache, table, total, n, queries(cuda, n, group, 128, torch.bfloat16))
