@@ -8,7 +8,10 @@
 //
 // Precision.  An int8 code is exact in fp16, so both products run on the fp16 matrix instruction
 // with the codes themselves and the scales stay outside.  A query row is brought to [-2, 2) by a power
-// of two, which keeps all of its bits.  The weights are rounded to fp16 (11 bits) once, with their value
+// of two and keeps all bits of the elements down to 2^-14 of its largest.  What fp16 drops of smaller
+// ones decides nothing but where the keys' codes are 0 at the large ones; where it could change a score
+// by more than 2^-14, an eighth of the weights' rounding, the tokens are taken again with further products
+// that add it (Rest).  The weights are rounded to fp16 (11 bits) once, with their value
 // scales in them: as 2^(s - m) vs / 2^d, where 2^d is a running reference of the row's own, like m, that
 // follows the largest 2^(s - m) vs which the row has seen.  It never falls below what the sums hold, so
 // that they stay finite beside pages of any scale (a page of zeros has 2^-119), and pages that the
@@ -31,6 +34,7 @@
 // wave (half the LDS reads) spill and take 512 us; waves half a turn apart, a higher priority for the
 // products, and products placed among the exponentials by hand change nothing or cost 4 to 6 %.
 #include <type_traits>
+#include <utility>
 
 #include "mfma_frag.h"
 
@@ -208,10 +212,67 @@ __device__ __forceinline__ int load_query(const T *q, bool valid, At at, Join jo
   return e2;
 }
 
+// What fp16 drops of query rows.  A pass over the tokens keeps the largest factor f from products to
+// scores; only if it could matter with f is it found what the rows did lose, and only if that does are the
+// tokens taken a second time, with the lost part as further products: in levels, each at 2^24 times the size
+// of the one before, so that four of them reach 2^-121 of a row's largest element.  The rows and, for attn_rows, the
+// codes are read again for it: it is rare, and registers are not.
+template <typename T, int D>
+struct Rest {
+  static constexpr float kMissed = 0x1p-14f;  // log2 units of a score
+  static constexpr int kLevels = 4, kStep = 24;
+  static constexpr float kUnit = 1 << kStep;
+
+  // Whether scores of up to f times a product need it.  q: pieces of the lane's row at at(c), c < n;
+  // join: as in load_query, over `sharing` lanes.
+  template <typename At, typename Join>
+  __device__ __forceinline__ static bool counts(float f, const T *q, int e2, bool valid, int n, At at, int sharing,
+                                                Join join) {
+    if (!__any(127.0f * D * 0x1p-25f * f > kMissed)) return false;  // D subnormal elements
+    float lost = 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < n; ++c) {
+      float x[8];
+      load8(q + at(c), x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_amdgcn_ldexpf(x[e], -e2);
+        lost += fabsf(v - static_cast<float>(static_cast<_Float16>(v)));
+      }
+    }
+    // a row that is not finite has NaN here, and NaN in its products
+    return __any(valid && 127.0f * sharing * join(lost) * f > kMissed);
+  }
+
+  // How many levels a group of tokens needs: an element leaves at most 2^-25 of the last level's unit.
+  __device__ __forceinline__ static int levels(float f) {
+    int level = 0;
+    while (level < kLevels && __any(__builtin_amdgcn_ldexpf(127.0f * D * f, -25 - kStep * level) > kMissed)) ++level;
+    return level;
+  }
+
+  // Eight elements at q as the operand of a level; level 0: the row as load_query gives it.
+  __device__ __forceinline__ static v8h operand(const T *q, int e2, int level) {
+    float f[8];
+    load8(q, f);
+    v8h r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v = __builtin_amdgcn_ldexpf(f[e], -e2);
+      v += 0.0f * v;  // an infinity becomes NaN
+#pragma unroll 1
+      for (int k = 0; k < level; ++k)
+        v = (v - static_cast<float>(static_cast<_Float16>(v))) * kUnit;
+      r[e] = static_cast<_Float16>(v);
+    }
+    return r;
+  }
+};
+
 // Sixteen query rows of one cache head, one chunk of their tokens.  The waves take groups of 64
 // tokens in turn and join their sums in LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArgs a) {
+__global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) void attn_rows(const AttnArgs a) {
   constexpr int NC = D / 64, NU = D / 16, pitch = D + 4;
   __shared__ float s_acc[kWaves][kRows][pitch];
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
@@ -247,12 +308,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
     const float q_scale = __builtin_amdgcn_ldexpf(a.scale, e2);
 
     v4f acc[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u) acc[u] = v4f{0, 0, 0, 0};
     // maximum, largest weight times scale (log2, relative to m), and d, the next whole number above it
-    float m = -INFINITY, l = 0.0f, peak = -INFINITY, d = kLeast;
+    float m, l, peak, d;
+    float f_most;  // largest factor from products to scores
+    auto rest_at = [](int c) { return 32 * (c & ~1) + 8 * (c & 1); };
 
-    auto step = [&](int t0, int ik, int iv) {  // one group of 64 tokens
+    auto step = [&](auto all_bits, int t0, int ik, int iv) {  // one group of 64 tokens
       const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * g;
       const int64_t kat = static_cast<int64_t>(in_cache(a, ik) ? ik : 0) * H + head;
       const int64_t vat = static_cast<int64_t>(in_cache(a, iv) ? iv : 0) * H + head;
@@ -270,17 +331,40 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
       if (!in_cache(a, iv)) ks = vs = nanf32();
       if (tv >= bot.hi) ks = vs = 0.0f;
 
+      const float f = ks * q_scale;
       v4f s[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        s[t] = v4f{0, 0, 0, 0};
+      for (int t = 0; t < 4; ++t) s[t] = v4f{0, 0, 0, 0};
+      if constexpr (all_bits.value) {
+        const int levels = Rest<T, D>::levels(fabsf(f));
+#pragma unroll 1
+        for (int level = 0; level <= levels; ++level) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          s[t] = mfma_f16(codes_f16(kw[t][c].x, kw[t][c].y), q[2 * c], s[t]);
-          s[t] = mfma_f16(codes_f16(kw[t][c].z, kw[t][c].w), q[2 * c + 1], s[t]);
+          for (int t = 0; t < 4; ++t) s[t] *= Rest<T, D>::kUnit;
+#pragma unroll 1
+          for (int c = 0; c < 2 * NC; ++c) {
+            const v8h r = Rest<T, D>::operand(qp + 16 * g + rest_at(c), e2, level);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint2 w = *reinterpret_cast<const uint2 *>(kp + 4 * t * D + rest_at(c));
+              s[t] = mfma_f16(codes_f16(w.x, w.y), r, s[t]);
+            }
+          }
         }
+#pragma unroll 1
+        for (int level = 1; level <= levels; ++level)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) s[t] *= 1.0f / Rest<T, D>::kUnit;
+      } else {
+        f_most = fmaxf(f_most, fabsf(f));
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            s[t] = mfma_f16(codes_f16(kw[t][c].x, kw[t][c].y), q[2 * c], s[t]);
+            s[t] = mfma_f16(codes_f16(kw[t][c].z, kw[t][c].w), q[2 * c + 1], s[t]);
+          }
       }
-      const float f = ks * q_scale;
 #pragma unroll
       for (int t = 0; t < 4; ++t) s[t] *= f;
       if (t0 < bot.lo || t0 + kGroup > top.hi) {  // some row does not see all 64
@@ -335,18 +419,28 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void attn_rows(const AttnArg
         acc[u] = mfma_f16(codes_f16(vw[u].z, vw[u].w), p[1], acc[u]);
       }
     };
-    // the ids of a group's pages are on their way while the group before is computed
-    const int t_first = begin + wave * kGroup;
-    int ik = page_id(a, ids, t_first + 16 * (col >> 2), end, shift);
-    int iv = page_id(a, ids, t_first + 16 * g, end, shift);
-    for (int t0 = t_first; t0 < end; t0 += kWaves * kGroup) {
-      const int t1 = t0 + kWaves * kGroup;
-      const int nk = page_id(a, ids, t1 + 16 * (col >> 2), end, shift);
-      const int nv = page_id(a, ids, t1 + 16 * g, end, shift);
-      step(t0, ik, iv);
-      ik = nk;
-      iv = nv;
-    }
+    auto pass = [&](auto all_bits) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u) acc[u] = v4f{0, 0, 0, 0};
+      m = peak = -INFINITY;
+      l = f_most = 0.0f;
+      d = kLeast;
+      // the ids of a group's pages are on their way while the group before is computed
+      const int t_first = begin + wave * kGroup;
+      int ik = page_id(a, ids, t_first + 16 * (col >> 2), end, shift);
+      int iv = page_id(a, ids, t_first + 16 * g, end, shift);
+      for (int t0 = t_first; t0 < end; t0 += kWaves * kGroup) {
+        const int t1 = t0 + kWaves * kGroup;
+        const int nk = page_id(a, ids, t1 + 16 * (col >> 2), end, shift);
+        const int nv = page_id(a, ids, t1 + 16 * g, end, shift);
+        step(all_bits, t0, ik, iv);
+        ik = nk;
+        iv = nv;
+      }
+    };
+    pass(std::false_type{});
+    if (Rest<T, D>::counts(f_most, qp + 16 * g, e2, valid, 2 * NC, rest_at, 4, [](float v) { return col_max(v); }))
+      pass(std::true_type{});
 
     // The four waves' sums on one maximum, as averages: each sum is divided by the row's whole l before
     // anything is added to it, because values near the type's largest have no room for more.
@@ -418,19 +512,39 @@ __device__ __forceinline__ v16f mfma32_f16(v8h a, v8h b, v16f c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+// Waves of a SIMD, least and most: with room for more the compiler saves registers that buy nothing.
+constexpr int tile_waves(int dim) { return dim <= 64 ? 3 : dim <= 128 ? 2 : 1; }
+
+// Products, each with an operand from LDS that is read AHEAD products before: load(i) and multiply(i, operand),
+// i a constant.  The order is pinned: left to itself the compiler reads, waits and multiplies one by one where
+// the rest of a kernel needs many registers ([2048 + 1226 queries]: 257 us, so 237).
+template <int AHEAD, int... I, typename Load, typename Multiply>
+__device__ __forceinline__ void feed_products(std::integer_sequence<int, I...>, Load load, Multiply multiply) {
+  v8h next[AHEAD];
+  auto fill = [&](auto i) {
+    if constexpr (i.value < static_cast<int>(sizeof...(I))) next[i.value % AHEAD] = load(i);
+  };
+  (((void)(I < AHEAD ? (fill(std::integral_constant<int, I>{}), 0) : 0)), ...);
+  ((multiply(std::integral_constant<int, I>{}, next[I % AHEAD]), fill(std::integral_constant<int, I + AHEAD>{}),
+    __builtin_amdgcn_sched_barrier(0)), ...);
+}
+
 template <typename T, int D, int W, bool WIDE>
-__global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const AttnArgs a) {
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(tile_waves(D), tile_waves(D)))) void attn_tile(
+    const AttnArgs a) {
   constexpr int tile = 32 * W, threads = 64 * W;
   constexpr int KC = D / 16, NU = D / 32;   // steps of the first product, tiles of the second
   constexpr int kp = kGroup + 1, vp = D + 1;  // pitches in units of 16 bytes
   constexpr int all = D * kGroup / 16;        // pieces of 16 codes of the keys, and of the values
   constexpr int pieces = (all + threads - 1) / threads;
+  constexpr int ahead = D <= 64 ? 2 : 4;      // operands that are read before they are needed
   struct Stage {
     uint4 k[D / 8 * kp];  // [8 dimensions][row of the tiles]
     uint4 v[8 * vp];      // [8 tokens][dimension]
     float ks[4], lv[4];   // of 16 tokens each: key scale, log2 of the value scale
   };
   __shared__ Stage stage[2];
+  __shared__ int s_again[W];
   const int tid = threadIdx.x, lane = tid % kWave, wave = wave_id();
   const int col = lane % 32, h = lane / 32;
   const Job job = job_of(a);
@@ -473,17 +587,14 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
     const float q_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale), e2);
 
     v16f acc[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
-    float m = -INFINITY, l = 0.0f, peak = -INFINITY, d = kLeast;  // as in attn_rows
+    float m, l, peak, d, f_most;  // as in attn_rows
+    auto rest_at = [](int c) { return 16 * c; };
 
     // Staging.  Piece i = tid + threads * j.
     uint4 kw[pieces], vw[pieces];
     float ks = 0.0f, vs = 0.0f;
     int ik[pieces], iv;
-    auto look_up = [&](int t0) {
+    auto look_up = [&](int t0) __attribute__((always_inline)) {
       if constexpr (WIDE) {
         iv = page_id(a, ids, t0, end, shift);
       } else {
@@ -493,7 +604,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
         iv = page_id(a, ids, t0 + tid % 4 * 16, end, shift);
       }
     };
-    auto fetch = [&](int t0) {
+    auto fetch = [&](int t0) __attribute__((always_inline)) {
       const int in = t0 & (P - 1);
       if constexpr (WIDE) iv = __builtin_amdgcn_readfirstlane(iv);
       const int64_t pv = in_cache(a, iv) ? iv : 0;
@@ -515,7 +626,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
         if (t0 + 16 * tid >= end) ks = vs = 0.0f;
       }
     };
-    auto put = [&](Stage &s) {
+    auto put = [&](Stage &s) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < pieces; ++j) {
         const int i = tid + threads * j;
@@ -533,20 +644,45 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
     };
 
     v16f st[2];
-    auto scores = [&](const Stage &s) {  // one group of 64 tokens
+    auto scores = [&](auto all_bits, const Stage &s) __attribute__((always_inline)) {  // one group of 64 tokens
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[t][r] = 0.0f;
-      // neighbouring products do not wait for each other's sums
+      auto keys = [&](int c, int t) {
+        return __builtin_bit_cast(v8h, s.k[(2 * c + h) * kp + 32 * t + col]);
+      };
+      if constexpr (all_bits.value) {
+        const int levels = Rest<T, D>::levels(fmaxf(s.ks[h], s.ks[2 + h]) * q_scale);
+#pragma unroll 1
+        for (int level = 0; level <= levels; ++level) {
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          st[t] = mfma32_f16(__builtin_bit_cast(v8h, s.k[(2 * c + h) * kp + 32 * t + col]), q[c],
-                             st[t]);
+            for (int r = 0; r < 16; ++r) st[t][r] *= Rest<T, D>::kUnit;
+#pragma unroll 1
+          for (int c = 0; c < KC; ++c) {
+            v8h r = Rest<T, D>::operand(qp + 8 * h + rest_at(c), e2, level);
+            if (a.scale < 0.0f) r = -r;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) st[t] = mfma32_f16(keys(c, t), r, st[t]);
+          }
+        }
+#pragma unroll 1
+        for (int level = 1; level <= levels; ++level)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[t][r] *= 1.0f / Rest<T, D>::kUnit;
+      } else {
+        // neighbouring products do not wait for each other's sums
+        feed_products<ahead>(
+            std::make_integer_sequence<int, 2 * KC>{},
+            [&](auto i) { return keys(i.value / 2, i.value % 2); },
+            [&](auto i, v8h k) { st[i.value % 2] = mfma32_f16(k, q[i.value / 2], st[i.value % 2]); });
+      }
     };
-    auto weigh = [&](int t0, const Stage &s) {
+    auto weigh = [&](int t0, const Stage &s) __attribute__((always_inline)) {
       float f[2], v[2], x[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -554,6 +690,7 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
         f[t] = f[t] < 0x1p-126f ? 0x1p-126f : f[t];  // so that -inf stays -inf
         v[t] = s.lv[2 * t + h];
       }
+      f_most = fmaxf(f_most, fmaxf(f[0], f[1]));
       if (t0 < wbot.lo || t0 + kGroup > wtop.hi) {  // some row does not see all 64
         asm volatile("");  // stays a branch: few groups need it
 #pragma unroll
@@ -606,37 +743,55 @@ __global__ __launch_bounds__(64 * W, D <= 128 ? 2 : 1) void attn_tile(const Attn
         }
         l += sum * __builtin_amdgcn_exp2f(-part);
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          // weights c: tokens 32 (c / 2) + 16 h + 8 (c % 2) + 0..7
-          const int chunk = 4 * (c / 2) + 2 * h + c % 2;
-          acc[u] = mfma32_f16(__builtin_bit_cast(v8h, s.v[chunk * vp + 32 * u + col]), p[c], acc[u]);
-        }
+      // weights c: tokens 32 (c / 2) + 16 h + 8 (c % 2) + 0..7
+      feed_products<ahead>(
+          std::make_integer_sequence<int, 4 * NU>{},
+          [&](auto i) {
+            constexpr int c = i.value / NU;
+            const int chunk = 4 * (c / 2) + 2 * h + c % 2;
+            return __builtin_bit_cast(v8h, s.v[chunk * vp + 32 * (i.value % NU) + col]);
+          },
+          [&](auto i, v8h v) { acc[i.value % NU] = mfma32_f16(v, p[i.value / NU], acc[i.value % NU]); });
     };
-
-    if (begin < end) {
-      look_up(begin);
-      fetch(begin);
-      look_up(begin + kGroup);
-      put(stage[0]);
-    }
-    __syncthreads();
-    int now = 0;
-    for (int t0 = begin; t0 < end; t0 += kGroup, now ^= 1) {
-      const bool more = t0 + kGroup < end;
-      if (more) {
-        fetch(t0 + kGroup);
-        look_up(t0 + 2 * kGroup);
+    auto pass = [&](auto all_bits) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
+      m = peak = -INFINITY;
+      l = f_most = 0.0f;
+      d = kLeast;
+      if (begin < end) {
+        look_up(begin);
+        fetch(begin);
+        look_up(begin + kGroup);
+        put(stage[0]);
       }
-      if (t0 < wbot.hi && t0 + kGroup > wtop.lo && w0 < rows) {
-        scores(stage[now]);
-        weigh(t0, stage[now]);
-      }
-      if (more) put(stage[now ^ 1]);
       __syncthreads();
-    }
+      int now = 0;
+      for (int t0 = begin; t0 < end; t0 += kGroup, now ^= 1) {
+        const bool more = t0 + kGroup < end;
+        if (more) {
+          fetch(t0 + kGroup);
+          look_up(t0 + 2 * kGroup);
+        }
+        if (t0 < wbot.hi && t0 + kGroup > wtop.lo && w0 < rows) {
+          scores(all_bits, stage[now]);
+          weigh(t0, stage[now]);
+        }
+        if (more) put(stage[now ^ 1]);
+        __syncthreads();
+      }
+    };
+    pass(std::false_type{});
+    const bool again = Rest<T, D>::counts(f_most, qp + 8 * h, e2, valid, KC, rest_at, 2,
+                                          [](float v) { return fmaxf(v, __shfl_xor(v, 32, kWave)); });
+    if (lane == 0) s_again[wave] = again;
+    __syncthreads();
+    bool any = false;  // the waves of a workgroup stay together
+#pragma unroll
+    for (int w = 0; w < W; ++w) any |= s_again[w] != 0;
+    if (any) pass(std::true_type{});
 
     l += __shfl_xor(l, 32, kWave);  // its lift is that of the sums
     const int unit = static_cast<int>(d);

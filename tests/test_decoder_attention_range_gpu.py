@@ -162,3 +162,35 @@ def test_values_at_the_ends_of_the_range(cuda, exponent, total, n, group):
     cache.v_scale.fill_(2.0 ** exponent)
     table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
     check(cuda, cache, table, total, n, queries(cuda, n, group, 128, torch.bfloat16))
+
+
+@pytest.mark.parametrize("n,group", ROWS)
+@pytest.mark.parametrize("dtype,apart,loud", [(torch.bfloat16, 20, 1), (torch.bfloat16, 24, 30),
+                                              (torch.bfloat16, 40, 1), (torch.bfloat16, 100, 5),
+                                              (torch.float16, 20, 1), (torch.float16, 21, 30)])
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128)])
+def test_quiet_channels_beside_loud_ones(cuda, page, dim, dtype, apart, loud, n, group):
+    """Query channels 2^apart above the others meet key codes of 0: the quiet ones decide."""
+    total = 200
+    pages = -(-total // page)
+    cache = codes_cache(cuda, pages, 1, dim, page)
+    cache.k[..., :loud] = 0
+    quiet = 2.0 ** -6 if dtype == torch.float16 else 1.0
+    cache.k_scale.fill_(1 / 60 / quiet)
+    q = queries(cuda, n, group, dim, torch.float32) * quiet
+    q[..., :loud] = quiet * 2.0 ** apart
+    q[0, 0, :loud] = 0  # a row without them
+    check(cuda, cache, torch.arange(pages, dtype=torch.int32, device=cuda)[None], total, n, q.to(dtype))
+
+
+@pytest.mark.parametrize("n,group", [(1, 1), (16, 8)])
+def test_quiet_channels_with_a_scale_below_zero(cuda, n, group):
+    """As above, with the least alike first: against the same call with the keys' signs turned."""
+    cache = codes_cache(cuda, 4, 1, 128, 64)
+    cache.k[..., 0] = 0
+    q = queries(cuda, n, group, 128, torch.bfloat16)
+    q[..., 0] = 2.0 ** 24
+    table, total = ints([[0, 1, 2, 3]], cuda), 256
+    out = ops.kv_cache_attention(q, cache, table, ints([total], cuda), ints([0, n], cuda), scale=-128 ** -0.5)
+    turned = cache._replace(k=-cache.k)
+    assert torch.equal(out, check(cuda, turned, table, total, n, q))
