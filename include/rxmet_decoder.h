@@ -29,7 +29,8 @@ extern "C" {
 
 /*
  * Rows to int8.  With a weight: h = round_dtype(x + residual) (h = x without a residual),
- * rstd = 1 / sqrt(mean(h^2) + eps), u = h * weight, a = max(max|u|, 2^-112),
+ * rstd = 1 / sqrt(mean(h^2) + eps), u = h * weight (fp32; a product beyond it is an infinity),
+ * a = max(max|u|, 2^-112),
  * codes = rint(u * (127 / a)), scales = a / 127 * rstd.  The codes do not go by rstd, so they do not go by the
  * order of the mean's sum.  Without a weight (NULL): u = x, rstd = 1.
  *   x, residual   [rows, cols], row strides x_stride / residual_stride

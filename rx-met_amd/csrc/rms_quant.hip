@@ -5,7 +5,8 @@
 // normalised row is n = u * rstd and its symmetric grid has the scale max|n| / 127.  rstd is positive, so
 // it cancels out of n / scale = u * 127 / max|u|: the codes follow from u alone (bit for bit, whatever the
 // order in which the mean was summed), and rstd enters the scale only.  The sum and the maximum are
-// taken in one pass over a row that stays in registers.
+// taken in one pass over a row that stays in registers.  Rows whose squares leave fp32's range are
+// summed again in 64 bits.
 //
 // Bound: HBM traffic, one read of each input and one write of each output, and for few rows the launch and one
 // trip to memory.  A workgroup of 256 threads has a row of up to 8192 elements (a wave up to 1024, 1024
@@ -53,6 +54,35 @@ __device__ __forceinline__ void row_reduce(float &sum, unsigned &top) {
       top = s_top[k] > top ? s_top[k] : top;
     }
   }
+}
+
+constexpr float kLargest = 3.402823466e38f;
+
+// 1 / sqrt(mean(h^2) + eps) in 64 bits, of rows whose squares leave fp32's range.  One element at a time,
+// those that the thread has written itself: it is rare, and the usual rows need the registers.
+template <typename T, int TPR, int NV>
+__device__ __forceinline__ double rstd_beyond_range(const T *h, int cols, float eps) {
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = 0; i < 8 * NV; ++i) {
+    const int c = (i / 8 * TPR + threadIdx.x % TPR) * 8 + i % 8;
+    if (c < cols) {
+      const double v = static_cast<double>(static_cast<float>(h[c]));
+      sum += v * v;
+    }
+  }
+#pragma unroll 1
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+  if constexpr (TPR > kWave) {
+    constexpr int waves = TPR / kWave;
+    __shared__ double s_sum[waves];
+    if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll 1
+    for (int k = 0; k < waves; ++k) sum += s_sum[k];
+  }
+  return 1.0 / sqrt(sum / cols + eps);
 }
 
 template <typename T, typename W, int TPR, int NV>
@@ -107,11 +137,19 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
   }
   row_reduce<TPR>(sum, bits);
   const float top = __builtin_bit_cast(float, bits);
-  const float rstd = w ? 1.0f / sqrtf(sum / static_cast<float>(a.cols) + a.eps) : 1.0f;
-  const bool good = top <= 3.402823466e38f;
+  const bool good = top <= kLargest;
   const float peak = fmaxf(top, kFloor);
+  const float mean = sum / static_cast<float>(a.cols) + a.eps;
+  float rstd = w ? 1.0f / sqrtf(mean) : 1.0f, scale = peak * kInv127 * rstd;
+  // squares below 2^-126 lose bits, which count where they are the mean; all threads of a row agree
+  if (w && (mean > kLargest || mean < 0x1p-100f)) {
+    const double r = rstd_beyond_range<T, TPR, NV>(
+        res ? static_cast<const T *>(a.h) + row * a.cols : x, a.cols, a.eps);
+    rstd = static_cast<float>(r);
+    scale = static_cast<float>(static_cast<double>(peak) / 127.0 * r);
+  }
+  if (!good) scale = nanf32();
   const float inv = good ? 127.0f / peak : 0.0f;
-  const float scale = good ? peak * kInv127 * rstd : nanf32();
   if (tid == 0) {
     a.scales[row] = scale;
     if (a.rstd) a.rstd[row] = rstd;
