@@ -880,6 +880,9 @@ struct Plan {
   int waves;  // of attn_tile; 0: attn_rows
 };
 
+// Workgroups of a launch, whose threads number below 2^32.
+constexpr int64_t kMostJobs = (1 << 23) - 1;
+
 // Chunks of the token axis: for attn_rows eight workgroups for each of 256 CUs, so that ragged
 // lengths even out (64 sequences of up to 16384 tokens, 8 heads: 286 us, with four 297, with sixteen 284),
 // each with at least 512 tokens, eight groups, so that its start and its sums' join stay small
@@ -907,6 +910,9 @@ Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t queries, int64
   p.chunk = cdiv(cdiv(span, splits), kWaves * kGroup) * (kWaves * kGroup);
   if (p.chunk < 1) p.chunk = kWaves * kGroup;
   p.splits = static_cast<int>(span < 1 ? 1 : cdiv(span, p.chunk));
+  // max_query may be all rows of many sequences: a workgroup takes several row tiles then
+  const int64_t others = static_cast<int64_t>(heads) * seqs * p.splits;
+  if (p.row_tiles * others > kMostJobs) p.row_tiles = kMostJobs / others > 1 ? kMostJobs / others : 1;
   return p;
 }
 
@@ -955,7 +961,7 @@ extern "C" int rxmet_kv_attention(const rxmet_kv_cache *cache, const rxmet_kv_ta
   if (window > INT32_MAX) window = 0;  // hides nothing
   RXMET_CHECK_ARG(p.splits == 1 || workspace, "this call needs a workspace");
   const int64_t jobs = p.row_tiles * p.splits * cache->heads;
-  RXMET_CHECK_ARG(jobs < 1 << 23 && jobs * table->seqs < 1 << 23, "too many query rows for one call");
+  RXMET_CHECK_ARG(jobs * table->seqs <= kMostJobs, "too many sequences and heads for one call");
   const int64_t rows = queries * q_heads;
   float *part = static_cast<float *>(workspace);
   const AttnArgs a{{*cache, *table}, lengths, cu_query, static_cast<int>(queries), query,
