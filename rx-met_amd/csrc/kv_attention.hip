@@ -906,7 +906,8 @@ Plan plan_for(int32_t heads, int32_t seqs, int32_t group, int64_t queries, int64
   int64_t splits = cdiv(p.waves ? 2048 / p.waves : 2048, tiles < 1 ? 1 : tiles);
   const int64_t least = p.waves ? 256 : 512;
   if (splits > cdiv(span, least)) splits = cdiv(span, least);
-  if (splits < 1) splits = 1;
+  // rows that fill the GPU by themselves; the join's threads stay below 2^32 so
+  if (splits < 1 || queries * group * heads >= 1 << 24) splits = 1;
   p.chunk = cdiv(cdiv(span, splits), kWaves * kGroup) * (kWaves * kGroup);
   if (p.chunk < 1) p.chunk = kWaves * kGroup;
   p.splits = static_cast<int>(span < 1 ? 1 : cdiv(span, p.chunk));
