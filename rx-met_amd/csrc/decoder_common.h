@@ -73,14 +73,15 @@ __device__ __forceinline__ void store8_part(T *p, int n, const float (&f)[8]) {
 }
 
 // The code of v, |v| < 2^22, in the low byte: adding 1.5 * 2^23 rounds half to even into the last
-// bits of the sum.  A NaN gives 0.
+// bits of the sum.  A NaN gives a byte of its payload: groups that hold one are cleared with `keep` of
+// code_bytes4, 0 there and ~0 elsewhere.
 __device__ __forceinline__ unsigned code_word(float v) {
   return __builtin_bit_cast(unsigned, v + 12582912.0f);
 }
 
-__device__ __forceinline__ unsigned code_bytes4(float a, float b, float c, float d) {
+__device__ __forceinline__ unsigned code_bytes4(float a, float b, float c, float d, unsigned keep = ~0u) {
   const unsigned lo = __builtin_amdgcn_perm(code_word(b), code_word(a), 0x0c0c0400u);
-  return lo | __builtin_amdgcn_perm(code_word(d), code_word(c), 0x04000c0cu);
+  return (lo | __builtin_amdgcn_perm(code_word(d), code_word(c), 0x04000c0cu)) & keep;
 }
 
 // The largest magnitude as an integer: without their signs, floats are ordered as their bits are,

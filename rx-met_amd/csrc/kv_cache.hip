@@ -103,6 +103,7 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
     const float scale = good ? fmaxf(fresh, was) : nanf32();
     const float inv = good ? 1.0f / scale : 0.0f;
     const float ratio = good ? was * inv : 0.0f;
+    const unsigned keep = good ? ~0u : 0u;
     const bool moves = s0 > 0 && !(scale == was);
     if (tid == 0) scales[at] = scale;
     if (which == 0) {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
             w[k] = code_bytes4(static_cast<float>(u[j][e].v[4 * k]) * inv,
                                static_cast<float>(u[j][e].v[4 * k + 1]) * inv,
                                static_cast<float>(u[j][e].v[4 * k + 2]) * inv,
-                               static_cast<float>(u[j][e].v[4 * k + 3]) * inv);
+                               static_cast<float>(u[j][e].v[4 * k + 3]) * inv, keep);
           *reinterpret_cast<uint2 *>(codes + (q + e) * D + 8 * c) = make_uint2(w[0], w[1]);
         }
       }
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
           for (int d = 0; d < 8; ++d)
             s_v[(8 * c + d) * pitch + q] = code_bytes4(
                 static_cast<float>(u[j][0].v[d]) * inv, static_cast<float>(u[j][1].v[d]) * inv,
-                static_cast<float>(u[j][2].v[d]) * inv, static_cast<float>(u[j][3].v[d]) * inv);
+                static_cast<float>(u[j][2].v[d]) * inv, static_cast<float>(u[j][3].v[d]) * inv, keep);
         }
       }
       __syncthreads();

@@ -150,6 +150,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
   }
   if (!good) scale = nanf32();
   const float inv = good ? 127.0f / peak : 0.0f;
+  const unsigned keep = good ? ~0u : 0u;
   if (tid == 0) {
     a.scales[row] = scale;
     if (a.rstd) a.rstd[row] = rstd;
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_forward(const RowAr
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         b[k] = code_bytes4(u[v][4 * k] * inv, u[v][4 * k + 1] * inv, u[v][4 * k + 2] * inv,
-                           u[v][4 * k + 3] * inv);
+                           u[v][4 * k + 3] * inv, keep);
       int8_t *p = a.codes + row * a.cols + c;
       if (n >= 8) {
         __builtin_memcpy(p, b, 8);
