@@ -56,6 +56,12 @@ def _native():
     return _ext
 
 
+def _not_traced(name):
+    """A trace would hold the outputs' allocations without the kernel that fills them."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{name} cannot be traced; rms_norm_quantize_dequantize can")
+
+
 def _float_type(t, name):
     if t.dtype not in _DTYPE:
         raise RuntimeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
@@ -108,10 +114,12 @@ def _check_rows(x, weight, residual):
 def _row_forward(x, weight, residual, eps, codes, y, keep_rstd):
     """(codes or None, y or None, scales, rstd or None, h)."""
     code = _check_rows(x, weight, residual)
-    shape, dev = x.shape, x.device
+    # (sizes are tensors while a trace records the training form)
+    shape, dev = torch.Size(int(n) for n in x.shape), x.device
     x2, xs = _rows(x)
-    rows, cols = x2.shape
+    rows, cols, xs = int(x2.shape[0]), int(x2.shape[1]), int(xs)
     r2, rs = _rows(residual) if residual is not None else (None, 0)
+    rs = int(rs)
     w = weight.contiguous() if weight is not None else None
     h = torch.empty(shape, dtype=x.dtype, device=dev) if residual is not None else None
     out = torch.empty(shape, dtype=torch.int8, device=dev) if codes else None
@@ -142,6 +150,7 @@ def rms_norm_quantize(x, weight, residual=None, eps: float = 1e-6
         out = ext.rms_norm_quantize(x, weight, residual, eps)
         if out is not None:
             return out
+    _not_traced("rms_norm_quantize")
     codes, _, scales, _, h = _row_forward(x, weight, residual, eps, True, False, False)
     return codes, scales, h
 
@@ -154,6 +163,7 @@ def quantize_rows(x) -> Tuple[torch.Tensor, torch.Tensor]:
         out = ext.quantize_rows(x)
         if out is not None:
             return out
+    _not_traced("quantize_rows")
     codes, _, scales, _, _ = _row_forward(x, None, None, 0.0, True, False, False)
     return codes, scales
 
@@ -211,7 +221,9 @@ def rms_norm_quantize_dequantize(x, weight, residual=None, eps: float = 1e-6
     if weight is None:
         raise RuntimeError("rms_norm_quantize_dequantize needs a weight")
     ext = _ext or _native()
-    if ext:
+    # tracing records the Python function, transforms and compilation meet or refuse it
+    if (ext and torch._C._get_tracing_state() is None
+            and not torch._C._are_functorch_transforms_active() and not torch.compiler.is_compiling()):
         out = ext.rms_norm_quantize_dequantize(x, weight, residual, eps)
         if out is not None:
             return out
@@ -238,6 +250,7 @@ def linear_int8(codes, scales, weight, weight_scales, bias=None, activation: Opt
                               residual, dtype)
         if out is not None:
             return out
+    _not_traced("linear_int8")
     _on_gpu(codes, "codes")
     dev = codes.device
     if dtype not in _DTYPE:
@@ -364,6 +377,7 @@ def kv_cache_append(cache: KVCache, key, value, block_table, lengths, cu_new=Non
     ext = _ext or _native()
     if ext and ext.kv_append(*cache, key, value, block_table, lengths, cu_new, max_new):
         return
+    _not_traced("kv_cache_append")
     seqs = block_table.shape[0] if block_table.dim() else 0
     c, t, dev = _cache_args(cache, block_table, ("lengths", lengths, seqs),
                             ("cu_new", cu_new, seqs + 1))
@@ -399,6 +413,7 @@ def kv_cache_read(cache: KVCache, block_table, first, cu_tokens, tokens: int,
         out = ext.kv_read(*cache, block_table, first, cu_tokens, tokens, max_tokens, dtype)
         if out is not None:
             return out
+    _not_traced("kv_cache_read")
     seqs = block_table.shape[0] if block_table.dim() else 0
     c, t, dev = _cache_args(cache, block_table, ("first", first, seqs),
                             ("cu_tokens", cu_tokens, seqs + 1))
@@ -436,6 +451,7 @@ def kv_cache_attention(query, cache: KVCache, block_table, lengths, cu_query=Non
                                scale, causal, window)
         if out is not None:
             return out
+    _not_traced("kv_cache_attention")
     seqs = block_table.shape[0] if block_table.dim() else 0
     c, t, dev = _cache_args(cache, block_table, ("lengths", lengths, seqs),
                             ("cu_query", cu_query, seqs + 1))

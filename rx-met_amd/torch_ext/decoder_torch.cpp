@@ -4,10 +4,12 @@
 // A single token's norm or projection takes 5 - 7 us of kernel; decoder_ops.py's checks and its
 // call through ctypes take the host 14 - 18 us.  These functions take the calls that need no copy
 // and refuse nothing: they return None for everything else (a wrong type, shape, device or stride, a tensor
-// subclass), and decoder_ops.py then goes its own way, which copies or raises.
+// subclass, a trace, which would record the allocations without the kernels), and decoder_ops.py then
+// goes its own way, which copies or raises.
 #include "rxmet_torch.h"
 
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <optional>
@@ -47,7 +49,9 @@ int type_code(at::ScalarType t) {
   }
 }
 
-bool plain(const Tensor &t) { return t.is_cuda() && !at::isTensorSubclassLike(t); }
+bool plain(const Tensor &t) {
+  return t.is_cuda() && !at::isTensorSubclassLike(t) && !torch::jit::tracer::isTracing();
+}
 
 bool is(const Tensor &t, at::ScalarType type, const Tensor &like) {
   return t.scalar_type() == type && plain(t) && t.device() == like.device();

@@ -1,0 +1,70 @@
+"""The decoder operators under tracing, saved-tensor hooks, changed operands and second derivatives, through
+the node in C++ and through the Python function."""
+import pytest
+import torch
+
+import decoder_ops as ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["c++", "python"])
+def path(request, monkeypatch):
+    if request.param == "python":
+        monkeypatch.setattr(ops, "_ext", False)
+    else:
+        assert ops._native(), "the module rxmet_torch is missing"
+    return request.param
+
+
+def make(cuda, rows=6, cols=200, seed=0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g).to(dtype).to(cuda).requires_grad_()
+    r = torch.randn(rows, cols, generator=g).to(dtype).to(cuda).requires_grad_()
+    w = (1 + 0.2 * torch.randn(cols, generator=g)).to(dtype).to(cuda).requires_grad_()
+    return x, w, r
+
+
+# ---------------------------------------------------------------------------------
+# Tracing
+# ---------------------------------------------------------------------------------
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("with_residual", [True, False])
+def test_traced_training_form_runs_on_other_inputs(cuda, path, with_residual):
+    x, w, r = (t.detach() for t in make(cuda))
+    f = (lambda x, w, r: ops.rms_norm_quantize_dequantize(x, w, r)) if with_residual else \
+        (lambda x, w, r: ops.rms_norm_quantize_dequantize(x, w))
+    traced = torch.jit.trace(f, (x, w, r), check_trace=False)
+    for seed in (1, 2):
+        args = [t.detach() for t in make(cuda, seed=seed)]
+        for a, b in zip(traced(*args), f(*args)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_serving_calls_refuse_a_trace(cuda, path):
+    x, w, _ = (t.detach() for t in make(cuda, cols=64))
+    codes, scales = ops.quantize_rows(x)
+    cache = ops.KVCache.empty(1, 1, 64, 16, device=cuda)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)
+    table, zero = ints(0)[None], ints(0)
+    q = x[:1, None].half()
+    ops.kv_cache_append(cache, q, q, table, zero)
+    for f in (lambda x: ops.rms_norm_quantize(x, w)[1], lambda x: ops.quantize_rows(x)[1],
+              lambda x: ops.linear_int8(codes, scales, codes, scales, dtype=torch.float32) + x[0, 0],
+              lambda x: ops.kv_cache_append(cache, x[:1, None], x[:1, None], table, zero) or x,
+              lambda x: ops.kv_cache_read(cache, table, zero, ints(0, 1), 1)[0] + x[0, 0],
+              lambda x: ops.kv_cache_attention(x[:1, None].half(), cache, table, zero + 1)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+        f(x)  # outside a trace as ever
+
+
+def test_transforms_are_refused(cuda, path):
+    x, w, r = make(cuda)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: ops.rms_norm_quantize_dequantize(x, w.detach())[0])(x.detach()[None])
+    import torch.autograd.forward_ad as fwAD
+    with fwAD.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        ops.rms_norm_quantize_dequantize(fwAD.make_dual(x.detach().requires_grad_(), torch.ones_like(x)), w)
