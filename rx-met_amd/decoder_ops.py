@@ -175,6 +175,7 @@ class _RmsQuantDequant(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps):
         _, y, _, rstd, h = _row_forward(x, weight, residual, eps, False, True, True)
         ctx.has_residual = residual is not None
+        ctx.packed = x.dtype, weight.dtype, x.device, tuple(x.shape)
         if residual is None:
             h = h.view_as(h)
         ctx.save_for_backward(h, weight, rstd)
@@ -183,6 +184,15 @@ class _RmsQuantDequant(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy, dh):
         h, weight, rstd = ctx.saved_tensors
+        # unpack hooks may hand back other tensors than were packed
+        dtype, weight_dtype, dev, shape = ctx.packed
+        _like(h, "the saved h", dtype, dev, shape)
+        _like(weight, "the saved weight", weight_dtype, dev, shape[-1:])
+        _like(rstd, "the saved rstd", torch.float32, dev, (math.prod(shape[:-1]),))
+        for g in (dy, dh):
+            if g is not None:
+                _like(g, "a gradient", dtype, dev, shape)
+        rstd = rstd.contiguous()
         dx, dw = _row_backward(dy, dh, h, weight, rstd, ctx.needs_input_grad[1])
         return dx, dw, dx if ctx.has_residual else None, None
 

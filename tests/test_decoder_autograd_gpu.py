@@ -68,3 +68,55 @@ def test_transforms_are_refused(cuda, path):
     import torch.autograd.forward_ad as fwAD
     with fwAD.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
         ops.rms_norm_quantize_dequantize(fwAD.make_dual(x.detach().requires_grad_(), torch.ones_like(x)), w)
+
+
+# ---------------------------------------------------------------------------------
+# Saved tensors
+# ---------------------------------------------------------------------------------
+
+def gradients(y, h, inputs):
+    return torch.autograd.grad([y, h], inputs, [torch.ones_like(y) * 0.5, torch.ones_like(h)])
+
+
+def test_hooks_that_keep_the_values(cuda, path):
+    """Saved tensors on the host, or strided, in the meantime: the same gradients."""
+    x, w, r = make(cuda)
+    inputs = (x, w, r)
+    ref = gradients(*ops.rms_norm_quantize_dequantize(*inputs), inputs)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(
+            lambda t: (seen.append(tuple(t.shape)), t.cpu())[1], lambda t: t.to(cuda)):
+        out = ops.rms_norm_quantize_dequantize(*inputs)
+    assert seen == [(6, 200), (200,), (6,)]
+    assert all(torch.equal(a, b) for a, b in zip(gradients(*out, inputs), ref))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t, t], -1)[..., 0]):
+        out = ops.rms_norm_quantize_dequantize(*inputs)
+    assert all(torch.equal(a, b) for a, b in zip(gradients(*out, inputs), ref))
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])  # h, weight, rstd
+@pytest.mark.parametrize("change", [lambda t: t.cpu(), lambda t: t.double(), lambda t: t.half(),
+                                    lambda t: t[:-1], lambda t: t[..., None], lambda t: t.new_zeros(())],
+                         ids=["host", "double", "half", "short", "axis", "scalar"])
+def test_hooks_that_give_back_something_else(cuda, path, which, change):
+    """Another device, type or shape is refused before anything is read."""
+    inputs = make(cuda)
+    count = iter(range(100))
+    with torch.autograd.graph.saved_tensors_hooks(
+            lambda t: (next(count), t), lambda p: change(p[1]) if p[0] == which else p[1]):
+        out = ops.rms_norm_quantize_dequantize(*inputs)
+    with pytest.raises(RuntimeError, match="saved"):
+        gradients(*out, inputs)
+
+
+def test_changed_operands_and_second_backward_are_refused(cuda, path):
+    x, w, r = make(cuda)
+    out = ops.rms_norm_quantize_dequantize(x, w, r)
+    gradients(*out, (x, w, r))
+    with pytest.raises(RuntimeError, match="second time"):
+        gradients(*out, (x, w, r))
+    out = ops.rms_norm_quantize_dequantize(x, w)
+    with torch.no_grad():
+        x.mul_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        gradients(*out, (x, w))
