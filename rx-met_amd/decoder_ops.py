@@ -194,6 +194,11 @@ class _RmsQuantDequant(torch.autograd.Function):
                 _like(g, "a gradient", dtype, dev, shape)
         rstd = rstd.contiguous()
         dx, dw = _row_backward(dy, dh, h, weight, rstd, ctx.needs_input_grad[1])
+        if torch.is_grad_enabled():
+            # create_graph: the kernel's gradients have no graph, so going through them has to fail
+            fail = torch._C._functions.DelayedError(
+                b"rms_norm_quantize_dequantize cannot be differentiated twice", 2)
+            dx, dw = fail(*(None if t is None else t.detach().requires_grad_() for t in (dx, dw)))
         return dx, dw, dx if ctx.has_residual else None, None
 
 

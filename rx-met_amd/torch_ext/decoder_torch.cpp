@@ -9,6 +9,7 @@
 #include "rxmet_torch.h"
 
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
@@ -189,6 +190,15 @@ struct RmsQuantDequant : torch::autograd::Function<RmsQuantDequant> {
                        cols, type_code(h.scalar_type()), need_w ? ws.mutable_data_ptr() : nullptr,
                        stream_of(h)),
           "rxmet_rms_quantize_backward");
+    if (at::GradMode::is_enabled()) {
+      // create_graph: the kernel's gradients have no graph, so going through them has to fail
+      auto leaf = [](const Tensor &t) { return t.defined() ? t.detach().requires_grad_() : t; };
+      const auto outs = std::make_shared<torch::autograd::DelayedError>(
+                            "rms_norm_quantize_dequantize cannot be differentiated twice", 2)
+                            ->apply({leaf(dx), leaf(dw)});
+      dx = outs[0];
+      dw = outs[1];
+    }
     return {dx, dw, ctx->saved_data["residual"].toBool() ? dx : Tensor(), Tensor()};
   }
 };

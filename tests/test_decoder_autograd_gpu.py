@@ -120,3 +120,35 @@ def test_changed_operands_and_second_backward_are_refused(cuda, path):
         x.mul_(1.0)
     with pytest.raises(RuntimeError, match="inplace"):
         gradients(*out, (x, w))
+
+
+# ---------------------------------------------------------------------------------
+# Second derivatives
+# ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("with_residual", [True, False])
+def test_second_derivatives_are_refused(cuda, path, with_residual):
+    """A penalty on the gradient raises, alone and beside a term that has a gradient, whatever input it is
+    taken in; the gradients themselves are those of an ordinary backward."""
+    x, w, r = make(cuda)
+    inputs = (x, w, r) if with_residual else (x, w)
+    ref = torch.autograd.grad(ops.rms_norm_quantize_dequantize(*inputs)[0].square().sum(), inputs)
+    for k in range(len(inputs)):
+        y, _ = ops.rms_norm_quantize_dequantize(*inputs)
+        grads = torch.autograd.grad(y.square().sum(), inputs, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(grads, ref))
+        with pytest.raises(RuntimeError, match="twice"):
+            (y.sum() + grads[k].square().sum()).backward()
+    y, _ = ops.rms_norm_quantize_dequantize(*inputs)
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)  # an incoming gradient without one of its own
+    with pytest.raises(RuntimeError, match="twice"):
+        (y.sum() + g.square().sum()).backward()
+
+
+def test_second_derivative_of_a_frozen_weight(cuda, path):
+    x, w, _ = make(cuda)
+    w = w.detach()
+    y, _ = ops.rms_norm_quantize_dequantize(x, w)
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
