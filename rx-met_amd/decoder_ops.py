@@ -141,7 +141,7 @@ def rms_norm_quantize(x, weight, residual=None, eps: float = 1e-6
 
     x [..., C] float32, float16 or bfloat16; weight [C] of x's type or float32; residual like x.
     codes int8 [..., C], scales float32 [...].  A row with a NaN or an infinity has scale NaN and
-    codes 0.  For inference: nothing here carries a gradient.
+    codes 0.  For inference: nothing here carries a gradient, h neither.
     """
     if weight is None:
         raise RuntimeError("rms_norm_quantize needs a weight (quantize_rows has none)")
@@ -152,7 +152,7 @@ def rms_norm_quantize(x, weight, residual=None, eps: float = 1e-6
             return out
     _not_traced("rms_norm_quantize")
     codes, _, scales, _, h = _row_forward(x, weight, residual, eps, True, False, False)
-    return codes, scales, h
+    return codes, scales, h.detach() if h.requires_grad else h
 
 
 def quantize_rows(x) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -256,6 +256,7 @@ def linear_int8(codes, scales, weight, weight_scales, bias=None, activation: Opt
     codes int8 [..., K] with scales float32 [...] (from ``rms_norm_quantize`` /
     ``quantize_rows``); weight int8 [N, K] with weight_scales float32 [N]; bias [N] and residual
     [..., N] in ``dtype``.  activation: None, "relu", "silu" or "gelu" (with the error function).
+    For inference: bias and residual get no gradient.
     The sum over K is exact, the rest float32.  K is at most 131071.  Rows that do not start on 16 bytes
     (K no multiple of 16) are copied first where there are more than 16 rows of codes.
     """
@@ -454,7 +455,8 @@ def kv_cache_attention(query, cache: KVCache, block_table, lengths, cu_query=Non
     Rows ``cu_query[b]..cu_query[b + 1]`` (without ``cu_query``: row b) are the last ones of sequence b's
     ``lengths[b]`` tokens, which the cache holds already.  With ``causal`` a query sees the tokens up to its
     own, with ``window`` only the last ``window`` of them; a query that sees nothing gives 0.
-    ``scale`` defaults to ``1 / sqrt(dim)``.
+    ``scale`` defaults to ``1 / sqrt(dim)``.  Rows that no sequence covers are undefined.  For inference: query
+    gets no gradient.
 
     ``max_query`` and ``max_length`` (the most queries and tokens of a sequence) size the launch; they
     default to all rows and to the table's width.  Larger values in the device vectors are computed

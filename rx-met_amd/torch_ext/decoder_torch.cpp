@@ -123,7 +123,7 @@ py::object rms_norm_quantize(const Tensor &x, const Tensor &weight, const OptTen
                              double eps) {
   Rows r;
   if (!row_forward(x, weight, residual, eps, true, false, r)) return py::none();
-  return py::make_tuple(r.codes, r.scales, r.h);
+  return py::make_tuple(r.codes, r.scales, r.h.requires_grad() ? r.h.detach() : r.h);
 }
 
 py::object quantize_rows(const Tensor &x) {

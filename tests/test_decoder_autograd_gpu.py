@@ -152,3 +152,17 @@ def test_second_derivative_of_a_frozen_weight(cuda, path):
     (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="twice"):
         g.sum().backward()
+
+
+# ---------------------------------------------------------------------------------
+# Serving
+# ---------------------------------------------------------------------------------
+
+def test_serving_outputs_carry_no_gradient(cuda, path):
+    """h is detached with a residual and without; it is x itself where that carries none."""
+    x, w, r = make(cuda)
+    for res in (None, r):
+        codes, scales, h = ops.rms_norm_quantize(x, w, res)
+        assert not (codes.requires_grad or scales.requires_grad or h.requires_grad)
+    assert torch.equal(ops.rms_norm_quantize(x, w)[2], x.detach())
+    assert ops.rms_norm_quantize(x.detach(), w)[2].data_ptr() == x.data_ptr()
