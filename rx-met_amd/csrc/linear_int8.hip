@@ -57,16 +57,21 @@ __device__ __forceinline__ uint4 load_piece(const int8_t *row, int k, int K) {
 
 __device__ __forceinline__ v4i as_v4i(uint4 u) { return __builtin_bit_cast(v4i, u); }
 
-// Finishes and writes C consecutive n of row m: as vectors, and one by one at N's end.
-template <typename T, int C>
+// The sum times such a row scale may leave fp32 where the result does not: the weight's scale goes first.
+__device__ __forceinline__ bool is_large(float sx) { return fabsf(sx) > 0x1p90f; }
+
+// Finishes and writes C consecutive n of row m: as vectors, and one by one at N's end.  LARGE: some rows
+// may be large (asked for each output, that costs 1.5 % of [8192, 8192] x [8192, 8192]).
+template <typename T, int C, bool LARGE = true>
 __device__ __forceinline__ void finish(const LinArgs &a, int64_t m, int64_t n0, const int (&acc)[C]) {
   if (m >= a.M || n0 >= a.N) return;
   const float sx = a.sx[m];
   const T *bias = a.bias ? static_cast<const T *>(a.bias) + n0 : nullptr;
   const T *res = a.res ? static_cast<const T *>(a.res) + m * a.res_stride + n0 : nullptr;
   T *y = static_cast<T *>(a.y) + m * a.N + n0;
+  const bool large = LARGE && is_large(sx);
   auto value = [&](int acc, float sw, T b, T r) {
-    float v = static_cast<float>(acc) * sx * sw;
+    float v = static_cast<float>(acc) * (large ? sw : sx) * (large ? sx : sw);
     if (bias) v += static_cast<float>(b);
     v = activate(v, a.act);
     if (res) v += static_cast<float>(r);
@@ -320,6 +325,9 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
   // side.  Chunk c of row m lies at c ^ turn, for the banks.
   auto turn = [](int m) { return CH >= 16 ? m & 15 : m >> 1 & 7; };
   v4i *part = reinterpret_cast<v4i *>(&s[0][0]) + wave * 32 * CH;
+  bool large = false;
+  for (int r = lane; r < TM / WM; r += kWave) large |= m0 + wm + r < a.M && is_large(a.sx[m0 + wm + r]);
+  large = __any(large);
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
 #pragma unroll
@@ -336,7 +344,10 @@ __global__ __launch_bounds__(64 * WN * WM) void linear_tile(const LinArgs a) {
       const int v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       const int64_t m = m0 + wm + 32 * j + r, n = n0 + wn + 4 * c;
       if (a.splits == 1) {
-        finish<T, 8>(a, m, n, v);
+        if (large)
+          finish<T, 8, true>(a, m, n, v);
+        else
+          finish<T, 8, false>(a, m, n, v);
       } else if (m < a.M) {
         int *p = a.part + (split * a.M + m) * a.N + n;
         if (n + 8 <= a.N) {
