@@ -269,7 +269,8 @@ int check_cache(const rxmet_kv_cache *c, const rxmet_kv_table *t) {
   RXMET_CHECK_ARG((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 == 0,
                   "the cache's codes must be aligned to 16 bytes");
   RXMET_CHECK_ARG(t->seqs >= 0 && t->seqs <= 65535, "at most 65535 sequences");
-  RXMET_CHECK_ARG(t->cols >= 1 && t->ids, "the block table is empty");
+  // a tensor without elements has no address: no sequences need no ids
+  RXMET_CHECK_ARG(t->cols >= 1 && (t->ids || t->seqs == 0), "the block table is empty");
   return 0;
 }
 
