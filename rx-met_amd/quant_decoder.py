@@ -97,14 +97,14 @@ class QuantDecoderLayer(nn.Module):
         """x [tokens, width] -> the same; the tokens' keys and values go into the cache."""
         n, d = x.shape[0], self.head_dim
         codes, scales, _ = ops.rms_norm_quantize(x, self.norm1, eps=self.eps)
-        qkv = self._linear("qkv", codes, scales).view(n, -1, d)
+        qkv = self._linear("qkv", codes, scales).view(n, self.heads + 2 * self.kv_heads, d)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)
         if rotate is not None:
             q, k = rotate(q, k, step.positions(n))
         ops.kv_cache_append(cache, k, v, step.block_table, step.lengths, step.cu_new, step.max_new)
         a = ops.kv_cache_attention(q, cache, step.block_table, step.after(), cu_query=step.cu_new,
                                    max_query=step.max_new, max_length=step.max_length)
-        codes, scales = ops.quantize_rows(a.view(n, -1))
+        codes, scales = ops.quantize_rows(a.view(n, self.heads * d))
         a = self._linear("o", codes, scales)
         codes, scales, h = ops.rms_norm_quantize(a, self.norm2, x, eps=self.eps)
         codes, scales = ops.quantize_rows(
