@@ -59,6 +59,10 @@ class QuantDecoderLayer(nn.Module):
         super().__init__()
         if heads % kv_heads:
             raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
+        # later it would fail behind the append, with the pass's tokens in the cache
+        if dtype not in (torch.float16, torch.bfloat16) or head_dim not in ops.HEAD_DIMS:
+            raise ValueError("a layer needs dtype float16 or bfloat16 and a head dimension of "
+                             f"{ops.HEAD_DIMS}, not {dtype} and {head_dim}")
         self.width, self.heads, self.kv_heads, self.head_dim = width, heads, kv_heads, head_dim
         self.activation, self.eps, self.dtype = activation, eps, dtype
         qkv = (heads + 2 * kv_heads) * head_dim
