@@ -94,7 +94,7 @@ int rxmet_linear_int8(const int8_t *codes, int64_t codes_stride, const float *sc
  */
 typedef struct rxmet_kv_cache {
   int8_t *k, *v;
-  float *k_scale, *v_scale; /* [pages, heads] */
+  float *k_scale, *v_scale; /* [pages, heads], positive as append makes them */
   int64_t pages;
   int32_t heads, page_size, dim, reserved; /* dim: 64, 128, 192 or 256; reserved 0 */
 } rxmet_kv_cache;

@@ -15,7 +15,9 @@
 // scales in them: as 2^(s - m) vs / 2^d, where 2^d is a running reference of the row's own, like m, that
 // follows the largest 2^(s - m) vs which the row has seen.  It never falls below what the sums hold, so
 // that they stay finite beside pages of any scale (a page of zeros has 2^-119), and pages that the
-// row does not see do not move it.  The weighted sums are in units of 2^d, l in units of 1.
+// row does not see do not move it.  The heaviest weight is a power of two so, and not rounded: fp16 results are
+// 3 to 11 % further from 64 bits than fp32 weights leave them, with 2^d a whole power 24 to 84 %.  The weighted
+// sums are in units of 2^d, l in units of 1.
 // Weights and l carry a common power of two (kLift): without it a weight 2^-25 of its
 // row's largest would round to 0 in fp16, and many such beside one large one make a sum that counts.
 //
@@ -48,11 +50,10 @@ typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 constexpr int kRows = 16;   // query rows of a workgroup: one column of the matrix instruction each
 constexpr int kGroup = 64;  // tokens that a wave takes at a time
 constexpr int kWaves = 4;
-// log2 of the weights' factor: the largest stays below 2^15 (attn_tile's may be 2^8 above its reference;
-// attn_rows multiplies by a scale's mantissa below 1).
+// log2 of the weights' factor: the largest is 2^15 (attn_tile's may be 2^8 above its reference).
 constexpr float kLiftRows = 15.0f, kLiftTile = 7.0f;
-// Least reference d, below the exponent of every scale, and the least log2(vs) - d that is told apart: with
-// it a weight's rounding gives 0, and l, which takes the factor out again, keeps its bits.
+// Least reference d, below log2 of every scale, and the least log2(vs) - d that is told apart: with it a
+// weight's rounding gives 0, and l, which takes the factor out again, keeps its bits.
 constexpr float kLeast = -200.0f, kApart = -48.0f;
 
 struct AttnArgs {
@@ -308,8 +309,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) void attn_rows
     const float q_scale = __builtin_amdgcn_ldexpf(a.scale, e2);
 
     v4f acc[NU];
-    // maximum, largest weight times scale (log2, relative to m), and d, the next whole number above it
-    float m, l, peak, d;
+    float m, l, d;  // maximum, sum, and log2 of the largest weight times scale, relative to m
     float f_most;  // largest factor from products to scores
     auto rest_at = [](int c) { return 32 * (c & ~1) + 8 * (c & 1); };
 
@@ -378,20 +378,17 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) void attn_rows
           }
         if (tv + 16 <= me.lo || tv >= me.hi) vs = 0.0f;  // 0 times a hidden page's NaN is no 0
       }
-      // vs = mant * 2^ex; the lane's 16 tokens lie in one page
-      const float mant = __builtin_amdgcn_frexp_mantf(vs);
-      const float ex = vs == 0.0f ? kLeast : static_cast<float>(__builtin_amdgcn_frexp_expf(vs));
+      const float lv = __builtin_amdgcn_logf(fabsf(vs));  // the lane's 16 tokens lie in one page
       float own = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) own = fmaxf(own, s[t][r]);
-      if (__any(own > m || (own - m) + ex > d)) {  // a row's maximum or reference moves
+      if (__any(own > m || (own - m) + lv > d)) {  // a row's maximum or reference moves
         const float high = fmaxf(m, col_max(own));
         const float base = high == -INFINITY ? 0.0f : high, delta = m - base;
         m = high;
-        peak = fmaxf(peak + delta, col_max((own - base) + ex));
-        const float next = fmaxf(ceilf(peak), kLeast);
+        const float next = fmaxf(fmaxf(d + delta, col_max((own - base) + lv)), kLeast);
         const float fix = exp2f((d - next) + delta);
         d = next;
         l *= exp2f(delta);
@@ -400,7 +397,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) void attn_rows
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[u][r] *= fix;
       }
-      const float part = fmaxf(ex - d, kApart);  // whole: l loses nothing when it is taken out again
+      float part = lv - d;
+      part = part < kApart ? kApart : part;  // a NaN stays one
       const float lifted = (m == -INFINITY ? 0.0f : m) - (kLiftRows + part);
       float sum = 0.0f;
       v8h p[2];
@@ -410,9 +408,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) void attn_rows
         for (int r = 0; r < 4; ++r) {
           const float e = __builtin_amdgcn_exp2f(s[t][r] - lifted);
           sum += e;
-          p[t / 2][4 * (t % 2) + r] = static_cast<_Float16>(e * mant);
+          p[t / 2][4 * (t % 2) + r] = static_cast<_Float16>(e);
         }
-      l += __builtin_amdgcn_ldexpf(sum, -static_cast<int>(part));
+      l += sum * __builtin_amdgcn_exp2f(-part);
+      if (__any(vs < 0.0f)) {  // such scales come from elsewhere than the append
+        if (vs < 0.0f) p[0] = -p[0], p[1] = -p[1];
+      }
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         acc[u] = mfma_f16(codes_f16(vw[u].x, vw[u].y), p[0], acc[u]);
@@ -422,7 +423,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 3 : 2) void attn_rows
     auto pass = [&](auto all_bits) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) acc[u] = v4f{0, 0, 0, 0};
-      m = peak = -INFINITY;
+      m = -INFINITY;
       l = f_most = 0.0f;
       d = kLeast;
       // the ids of a group's pages are on their way while the group before is computed
@@ -587,7 +588,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(tile_wav
     const float q_scale = __builtin_amdgcn_ldexpf(fabsf(a.scale), e2);
 
     v16f acc[NU];
-    float m, l, peak, d, f_most;  // as in attn_rows
+    float m, l, d, f_most;  // as in attn_rows
     auto rest_at = [](int c) { return 16 * c; };
 
     // Staging.  Piece i = tid + threads * j.
@@ -716,8 +717,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(tile_wav
         m = high;
         float up = fmaxf((x[0] - base) + v[0], (x[1] - base) + v[1]);
         up = fmaxf(up, __shfl_xor(up, 32, kWave));
-        peak = fmaxf(peak + delta, up);
-        const float next = fmaxf(ceilf(peak), kLeast);
+        const float next = fmaxf(fmaxf(d + delta, up), kLeast);
         const float fix = exp2f((d - next) + delta);
         d = next;
         l *= exp2f(delta);
@@ -758,7 +758,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(tile_wav
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[u][r] = 0.0f;
-      m = peak = -INFINITY;
+      m = -INFINITY;
       l = f_most = 0.0f;
       d = kLeast;
       if (begin < end) {
@@ -794,11 +794,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(tile_wav
     if (any) pass(std::true_type{});
 
     l += __shfl_xor(l, 32, kWave);  // its lift is that of the sums
-    const int unit = static_cast<int>(d);
+    const float unit = rintf(d);
     if (valid) {
       const int64_t place = static_cast<int64_t>(seq.q0 + row / G) * a.q_heads + head * G + row % G;
       const int64_t at = static_cast<int64_t>(split) * a.queries * a.q_heads + place;
-      const float f = l == 0.0f ? 0.0f : 1.0f / l;
+      const float f = l == 0.0f ? 0.0f : exp2f(d - unit) / l;
       if (a.splits > 1 && h == 0) a.stats[2 * at] = m, a.stats[2 * at + 1] = l;
       if (a.splits == 1 || begin < end) {
 #pragma unroll
@@ -812,7 +812,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(tile_wav
             v4f w;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              w[e] = __builtin_amdgcn_ldexpf(acc[u][4 * k + e] * f, unit);
+              w[e] = __builtin_amdgcn_ldexpf(acc[u][4 * k + e] * f, static_cast<int>(unit));
               o.v[e] = static_cast<T>(w[e]);
             }
             if (a.splits > 1)

@@ -194,3 +194,23 @@ def test_quiet_channels_with_a_scale_below_zero(cuda, n, group):
     out = ops.kv_cache_attention(q, cache, table, ints([total], cuda), ints([0, n], cuda), scale=-128 ** -0.5)
     turned = cache._replace(k=-cache.k)
     assert torch.equal(out, check(cuda, turned, table, total, n, q))
+
+
+@pytest.mark.parametrize("n,group", [(1, 1), (1, 64)])
+@pytest.mark.parametrize("total,heavy", [(1, 0), (300, 0), (300, 200), (300, 299)])
+def test_one_heavy_token_is_rounded_once(cuda, total, heavy, n, group):
+    """The result is the token's value, whatever its page's scale: the weight adds no rounding of its own.
+    Exponential, logarithm, quotient and scale: 2^-18 at most; the result's rounding to fp16."""
+    pages = -(-total // 16)
+    cache = codes_cache(cuda, pages, 8, 64, 16)
+    cache.v_scale.copy_(torch.exp(torch.randn(pages, 8, generator=torch.Generator().manual_seed(heavy)) * 0.5))
+    cache.k.zero_()
+    cache.k[heavy // 16, :, heavy % 16, 0], cache.k_scale[:] = 127, 1.0
+    q = torch.zeros(n, 8 * group, 64, dtype=torch.float16, device=cuda)
+    q[..., 0] = 1
+    table = torch.arange(pages, dtype=torch.int32, device=cuda)[None]
+    out = ops.kv_cache_attention(q, cache, table, ints([total], cuda), scale=60 * math.log(2) / 127)
+    page = heavy // 16
+    want = f64(cache.v[page, :, :, heavy % 16]) * f64(cache.v_scale[page])[:, None]
+    got = f64(out).reshape(8, group, 64)
+    assert (np.abs(got - want[:, None]) <= (2.0 ** -11 + 2.0 ** -18) * np.abs(want[:, None]) + 2.0 ** -25).all()
