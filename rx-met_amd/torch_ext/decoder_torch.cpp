@@ -143,36 +143,32 @@ struct RmsQuantDequant : torch::autograd::Function<RmsQuantDequant> {
     ctx->save_for_backward({r.h, weight, r.rstd});
     ctx->set_materialize_grads(false);
     ctx->saved_data["residual"] = residual.has_value();
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
-    ctx->saved_data["weight_type"] = static_cast<int64_t>(weight.scalar_type());
-    ctx->saved_data["device"] = x.device();
     return {r.y, r.h};
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    // unpack hooks may hand back other tensors than were packed
-    const auto shape = ctx->saved_data["shape"].toIntVector();
-    const int64_t cols = shape.back();
-    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
-    const auto weight_type = static_cast<at::ScalarType>(ctx->saved_data["weight_type"].toInt());
-    const at::Device device = ctx->saved_data["device"].toDevice();
-    int64_t rows = 1;
-    for (size_t k = 0; k + 1 < shape.size(); ++k) rows *= shape[k];
-    auto is_packed = [&](const Tensor &t, at::ScalarType want, at::IntArrayRef sizes) {
+    // Unpack hooks may hand back other tensors than were packed.  The engine has held the gradients
+    // against the outputs, which are like x.
+    const Tensor &like = grads[0].defined() ? grads[0] : grads[1];
+    if (!like.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const at::ScalarType type = like.scalar_type();
+    const at::Device device = like.device();
+    const int64_t cols = like.size(-1), rows = like.numel() / cols;
+    auto fits = [&](const Tensor &t, at::ScalarType want, at::IntArrayRef sizes) {
       return t.defined() && t.device() == device && t.scalar_type() == want && t.sizes() == sizes;
     };
-    TORCH_CHECK(is_packed(saved[0], type, shape) && is_packed(saved[1], weight_type, {cols}) &&
-                    is_packed(saved[2], at::kFloat, {rows}),
+    TORCH_CHECK(type_code(type) >= 0 && like.is_cuda() && fits(saved[0], type, like.sizes()) &&
+                    (fits(saved[1], type, {cols}) || fits(saved[1], at::kFloat, {cols})) &&
+                    fits(saved[2], at::kFloat, {rows}),
                 "rms_norm_quantize_dequantize: the saved tensors are not those of the forward pass");
     const c10::DeviceGuard guard(device);
     const Tensor h = saved[0].contiguous(), weight = saved[1].contiguous(), rstd = saved[2].contiguous();
     auto gradient = [&](const Tensor &g) {
-      TORCH_CHECK(g.device() == device && g.sizes() == at::IntArrayRef(shape),
-                  "rms_norm_quantize_dequantize: a gradient has another shape or device");
-      return g.to(type).contiguous();
+      TORCH_CHECK(fits(g, type, like.sizes()),
+                  "rms_norm_quantize_dequantize: a gradient has another shape, type or device");
+      return g.contiguous();
     };
     const Tensor dy = grads[0].defined() ? gradient(grads[0]) : at::zeros_like(h);
     Tensor dh;
