@@ -26,18 +26,20 @@
 // lane (col, g) gets the scores of query col for the 16 consecutive tokens 16 g..16 g + 15.  The second
 // product is O^T = V^T P^T; its operand from P is what the lane holds already, and its operand
 // from V is 16 consecutive bytes, as values lie dimension by dimension.  Nothing crosses lanes but the row maximum.
-#include "kv_cache.h"
 //
-// Bound and measured (bf16 queries, dim 128, pages of 64).  attn_rows: HBM, the cache's bytes: 64 sequences of 0 to 16384
-// tokens, 8 heads, 64 query heads: 1356 MB in 281 us (4.8 TB/s; a copy of 2 GiB reaches 4.9); two of 32768 and 16679 tokens,
-// 32 query heads: 101 MB in 24 us and 4.7 us for the join of 64 chunks.  attn_tile: the issue of a
-// SIMD's two waves, of whose time the matrix unit has 40 % and the vector unit 54 % (exponentials,
-// conversions): 204 GFLOP in 235 to 255 us by card, 867 to 800 TFLOP/s, where a large library product reaches 1385.  64 rows a
-// wave (half the LDS reads) spill and take 512 us; waves half a turn apart, a higher priority for the
-// products, and products placed among the exponentials by hand change nothing or cost 4 to 6 %.
+// Bound and measured (bf16 queries, dim 128, pages of 64).  attn_rows: HBM, the cache's bytes: 64 sequences
+// of 0 to 16384 tokens, 8 heads, 64 query heads: 1356 MB in 283 us (4.8 TB/s; a copy of 2 GiB reaches 4.9); two
+// of 32768 and 16679 tokens, 32 query heads: 101 MB in 25 us and 4.7 us for the join of 64 chunks.  attn_tile: the issue of a
+// SIMD's two waves: counted over the whole launch, its ends with it, the matrix unit is busy for 35 % and the
+// vector unit (exponentials, conversions) for 46 % of the time: 204 GFLOP in 237 to 258 us by card, 860 to 790
+// TFLOP/s, where a large library product reaches 1385.  64 rows a wave (half the LDS reads) spill and take 512 us;
+// waves half a turn apart, a higher priority for the products, and products placed among the
+// exponentials by hand change nothing or cost 4 to 6 %; weights as two fp16 numbers, which keep 22 bits, cost
+// 32 % (and 2 % in attn_rows).
 #include <type_traits>
 #include <utility>
 
+#include "kv_cache.h"
 #include "mfma_frag.h"
 
 namespace rxmet {

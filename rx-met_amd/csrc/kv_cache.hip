@@ -57,7 +57,8 @@ __global__ __launch_bounds__(256) void kv_append(const AppendArgs a) {
   constexpr int units = P / 4 * C, NU = (units + 255) / 256;
   constexpr int pitch = P / 4 + 1;                      // words of a dimension in LDS
   __shared__ unsigned s_v[D * pitch];
-  const int heads = a.g.c.heads, b = blockIdx.z, which = static_cast<int>(blockIdx.x) >= heads, tid = threadIdx.x;
+  const int tid = threadIdx.x, heads = a.g.c.heads, b = blockIdx.z;
+  const int which = static_cast<int>(blockIdx.x) >= heads;  // 0: keys, 1: values
   const int head = blockIdx.x - which * heads;
   const int64_t start = a.lengths[b];
   const int64_t row0 = a.cu ? a.cu[b] : b;
@@ -178,7 +179,8 @@ struct ReadArgs {
 
 template <typename T, int D, int P>
 __global__ __launch_bounds__(256) void kv_read(const ReadArgs a) {
-  const int heads = a.g.c.heads, b = blockIdx.z, which = static_cast<int>(blockIdx.x) >= heads, tid = threadIdx.x;
+  const int tid = threadIdx.x, heads = a.g.c.heads, b = blockIdx.z;
+  const int which = static_cast<int>(blockIdx.x) >= heads;  // 0: keys, 1: values
   const int head = blockIdx.x - which * heads;
   const int64_t start = a.first[b], row0 = a.cu[b];
   int64_t count = a.cu[b + 1] - row0;

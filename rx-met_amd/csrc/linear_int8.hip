@@ -6,9 +6,9 @@
 // Layout.  The matrix instruction's rows are weight rows (n), its columns are token rows (m), so
 // that a lane holds several consecutive n of one m.
 //
-// Bound and measured.  Few rows: the weights' bytes ([16, 4096] x [4096, 4096] 6.9 us, [16, 8192] x [8192, 8192] 19 us =
-// 3.5 TB/s).  Many: the matrix unit, which is busy half of the time: [8192, 8192] x [8192, 8192] 566 us, 1.94 POP/s, where the
-// library's int8 product without an epilogue reaches 2.1.
+// Bound and measured.  Few rows: the weights' bytes ([16, 4096] x [4096, 4096] 6.9 us, [16, 8192] x
+// [8192, 8192] 19 us = 3.5 TB/s).  Many: the matrix unit, which is busy for 51 % of the time: [8192, 8192] x [8192, 8192] 568 to 650 us by
+// card, 1.94 to 1.69 POP/s, where the library's int8 product without an epilogue reaches 2.1.
 #include <type_traits>
 
 #include "decoder_common.h"
@@ -159,7 +159,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void linear_few(const LinArgs a) {
 //
 // K goes through LDS in steps of 64 bytes, memory -> LDS without registers, three steps ahead in
 // a ring of four.  A row's four 16-byte pieces lie at the places piece ^ f(row), so that 16 lanes
-// that read one piece of 16 rows meet 16 different bank groups (no conflicts counted).  Row i of a wave's
+// that read one piece of 16 rows meet 16 different bank groups (none of the 256 x 256
+// tiles' LDS accesses counts a conflict, 9 % of the 64 x 64 ones' do).  Row i of a wave's
 // 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) + i % 4: a lane holds 16 consecutive n of
 // one m.  Rows have to start on 16 bytes; others are copied first (linear_align).  Twice the ring for the
 // smallest tiles, or two steps of them to a barrier, changes nothing.
