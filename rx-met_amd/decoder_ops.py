@@ -236,9 +236,10 @@ def rms_norm_quantize_dequantize(x, weight, residual=None, eps: float = 1e-6
     if weight is None:
         raise RuntimeError("rms_norm_quantize_dequantize needs a weight")
     ext = _ext or _native()
-    # tracing records the Python function, transforms and compilation meet or refuse it
+    # tracing records the Python function, transforms refuse it; a compiled program calls the C++ one
+    # between its graphs
     if (ext and torch._C._get_tracing_state() is None
-            and not torch._C._are_functorch_transforms_active() and not torch.compiler.is_compiling()):
+            and not torch._C._are_functorch_transforms_active()):
         out = ext.rms_norm_quantize_dequantize(x, weight, residual, eps)
         if out is not None:
             return out

@@ -166,3 +166,28 @@ def test_serving_outputs_carry_no_gradient(cuda, path):
         assert not (codes.requires_grad or scales.requires_grad or h.requires_grad)
     assert torch.equal(ops.rms_norm_quantize(x, w)[2], x.detach())
     assert ops.rms_norm_quantize(x.detach(), w)[2].data_ptr() == x.data_ptr()
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_programs(cuda, backend):
+    """Operators between the graphs of a compiled program give what they give without it."""
+    assert ops._native(), "the module rxmet_torch is missing"
+    x, w, _ = make(cuda, cols=64)
+    codes, scales = ops.quantize_rows(x.detach())
+
+    def train(x, w):
+        y, h = ops.rms_norm_quantize_dequantize(x * 2, w)
+        return (y * h).sum()
+
+    def serve(x):
+        c, s, h = ops.rms_norm_quantize(x * 2, w)
+        return ops.linear_int8(c, s, codes, scales) * 2 + ops.quantize_rows(h)[1][0]
+
+    torch._dynamo.reset()
+    got, want = torch.compile(train, backend=backend)(x, w), train(x, w)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, (x, w)), torch.autograd.grad(want, (x, w))):
+        assert torch.equal(a, b)
+    assert torch.equal(torch.compile(serve, backend=backend)(x.detach()), serve(x.detach()))
+    torch._dynamo.reset()
