@@ -1,0 +1,482 @@
+// expert_linear.hip — int8 product with a weight for each expert, rows gathered or in the experts' order.
+//
+// Mathematics.  Of place i of expert e, with r its row of codes: acc[n] = sum_k x[r, k] w[e, n, k] exact in
+// int32, y[i, n] = act(acc * sx[r] * sw[e, n] + b[e, n]); gated: act(gate) * value, the gate from weight
+// row n and the value from row N + n, both in the same lane's hands.  The epilogue is fp32 and rounds once.
+//
+// The experts' rows are known on the device alone: a launch is sized for the most tiles that the entries
+// can need, and each workgroup finds its tile in the offsets.
+#include <type_traits>
+
+#include "../../include/rxmet_experts.h"
+#include "int8_tile.h"
+
+namespace rxmet {
+namespace dec {
+namespace {
+
+struct ExpertArgs {
+  const int32_t *offsets, *entries;
+  int64_t tokens, rows;  // rows: places, tokens * top_k
+  int top_k, experts, grouped;
+  const int8_t *x, *w;
+  int64_t x_stride, w_stride, e_stride;
+  const float *sx, *sw;
+  const void *bias;
+  void *y;
+  int64_t N;
+  int K, gated, act, dtype;
+};
+
+// The places of expert e, kept inside the rows whatever the offsets hold.
+__device__ __forceinline__ void places_of(const ExpertArgs &a, int e, int64_t &from, int64_t &to) {
+  const int64_t lo = a.offsets[e], hi = a.offsets[e + 1];
+  from = lo < 0 ? 0 : lo < a.rows ? lo : a.rows;
+  to = hi < from ? from : hi < a.rows ? hi : a.rows;
+}
+
+// The row of codes of place i.
+__device__ __forceinline__ int64_t row_of(const ExpertArgs &a, int64_t i) {
+  if (a.grouped) return i;
+  const int64_t t = a.entries[i] / a.top_k;
+  return t < 0 ? 0 : t < a.tokens ? t : a.tokens - 1;
+}
+
+// Finishes and writes C consecutive n of place i; v: the sums of the values where gated.
+template <typename T, int C, bool LARGE>
+__device__ __forceinline__ void finish(const ExpertArgs &a, int e, int64_t i, float sx, int64_t n0,
+                                       const int (&acc)[C], const int (&val)[C]) {
+  const int64_t first = static_cast<int64_t>(e) * a.N * (1 + a.gated) + n0;
+  const float *sw = a.sw + first;
+  const T *bias = a.bias ? static_cast<const T *>(a.bias) + first : nullptr;
+  T *y = static_cast<T *>(a.y) + i * a.N + n0;
+  const bool large = LARGE && is_large(sx);
+  auto scaled = [&](int acc, float w, T b) {
+    const float v = static_cast<float>(acc) * (large ? w : sx) * (large ? sx : w);
+    return bias ? v + static_cast<float>(b) : v;
+  };
+  struct Vec {
+    T v[C];
+  };
+  if (n0 + C <= a.N) {
+    Vec out, b = {}, bv = {};
+    float w[C], wv[C];
+    __builtin_memcpy(w, sw, sizeof(w));
+    if (bias) __builtin_memcpy(&b, bias, sizeof(b));
+    if (a.gated) {
+      __builtin_memcpy(wv, sw + a.N, sizeof(wv));
+      if (bias) __builtin_memcpy(&bv, bias + a.N, sizeof(bv));
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float v = activate(scaled(acc[c], w[c], b.v[c]), a.act);
+      if (a.gated) v *= scaled(val[c], wv[c], bv.v[c]);
+      out.v[c] = static_cast<T>(v);
+    }
+    __builtin_memcpy(y, &out, sizeof(out));
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (n0 + c < a.N) {
+        float v = activate(scaled(acc[c], sw[c], bias ? bias[c] : static_cast<T>(0.0f)), a.act);
+        if (a.gated) v *= scaled(val[c], sw[a.N + c], bias ? bias[a.N + c] : static_cast<T>(0.0f));
+        y[c] = static_cast<T>(v);
+      }
+  }
+}
+
+template <int C, bool LARGE = true>
+__device__ __forceinline__ void finish_as(const ExpertArgs &a, int e, int64_t i, float sx, int64_t n0,
+                                          const int (&acc)[C], const int (&val)[C]) {
+  if (a.dtype == RXMET_QDQ_BF16)
+    finish<bf16, C, LARGE>(a, e, i, sx, n0, acc, val);
+  else if (a.dtype == RXMET_QDQ_F16)
+    finish<f16, C, LARGE>(a, e, i, sx, n0, acc, val);
+  else
+    finish<float, C, LARGE>(a, e, i, sx, n0, acc, val);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows of an expert: a workgroup takes 16 weight rows of one expert (gated: 8 gates and their 8
+// values) and all of K, its eight waves take runs of 128 of K in turn; the weights go from memory
+// into the matrix instruction with no stop in LDS, for 16 rows of codes at a time.  The eight sums meet in LDS.
+constexpr int kFewWaves = 8;
+
+__global__ __launch_bounds__(64 * kFewWaves) void experts_few(const ExpertArgs a) {
+  __shared__ int s[kFewWaves][16][20];
+  const int tiles = static_cast<int>((a.N + (a.gated ? 7 : 15)) / (a.gated ? 8 : 16));
+  const int e = blockIdx.x / tiles;
+  int64_t from, to;
+  places_of(a, e, from, to);
+  if (from >= to) return;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int col = lane % 16, g = lane / 16;
+  const int width = a.gated ? 8 : 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x % tiles) * width;
+  const int64_t n = n0 + col % width;
+  const int8_t *w = a.w + e * a.e_stride + ((n < a.N ? n : a.N - 1) + (col >= width ? a.N : 0)) * a.w_stride;
+  for (int64_t m0 = from; m0 < to; m0 += 16) {
+    const int8_t *x = a.x + row_of(a, m0 + col < to ? m0 + col : to - 1) * a.x_stride;
+    v4i acc = {0, 0, 0, 0};
+    constexpr int turn = kFewWaves * 128;  // from a wave's run of K to its next
+    auto runs = [&](auto N, int k0) {      // N of them, all their loads before the first product
+      v4i wf[N.value][2], xf[N.value][2];
+#pragma unroll
+      for (int i = 0; i < N.value; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int k = k0 + turn * i + 64 * c + 16 * g;
+          __builtin_memcpy(&wf[i][c], w + k, 16);
+          __builtin_memcpy(&xf[i][c], x + k, 16);
+        }
+#pragma unroll
+      for (int i = 0; i < N.value; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc = mfma_i8(wf[i][c], xf[i][c], acc);
+    };
+    int k0 = wave * 128;
+    for (; k0 + turn + 128 <= a.K; k0 += 2 * turn) runs(std::integral_constant<int, 2>{}, k0);
+    for (; k0 + 128 <= a.K; k0 += turn) runs(std::integral_constant<int, 1>{}, k0);
+    if (k0 < a.K) {  // K ends in this run
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int k = k0 + 64 * c + 16 * g;
+        acc = mfma_i8(as_v4i(load_piece(w, k, a.K)), as_v4i(load_piece(x, k, a.K)), acc);
+      }
+    }
+    *reinterpret_cast<v4i *>(&s[wave][col][4 * g]) = acc;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < 16 * width / 4) {
+      const int m = threadIdx.x / (width / 4), c = threadIdx.x % (width / 4) * 4;
+      auto sum = [&](int at) {
+        v4i t = *reinterpret_cast<const v4i *>(&s[0][m][at]);
+#pragma unroll
+        for (int v = 1; v < kFewWaves; ++v) t += *reinterpret_cast<const v4i *>(&s[v][m][at]);
+        return t;
+      };
+      const v4i p = sum(c), q = a.gated ? sum(8 + c) : p;
+      const int acc4[4] = {p[0], p[1], p[2], p[3]}, val4[4] = {q[0], q[1], q[2], q[3]};
+      if (m0 + m < to && n0 + c < a.N)
+        finish_as<4>(a, e, m0 + m, a.sx[row_of(a, m0 + m)], n0 + c, acc4, val4);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Tiles of TN weight rows x TM places of one expert on mfma 32x32x32; WN x WM waves take equal parts.
+// Where gated, a wave's weight rows are gates in their first half and the same columns' values in the
+// second.  K goes through LDS in steps of 64 bytes, memory -> LDS without registers, three steps ahead in
+// a ring of four; pieces of a row and rows of a wave lie as in linear_int8.hip.  Rows that do not start
+// on 16 bytes (ALIGNED false) go through registers, one step ahead.
+template <int TN, int TM, int WN, int WM, bool ALIGNED>
+__global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a) {
+  constexpr int threads = 64 * WN * WM;
+  constexpr int FN = TN / WN / 32, FM = TM / WM / 32;
+  constexpr int bytes = (TN + TM) * kStep;
+  constexpr int ring = 4;
+  constexpr int loads = bytes / 16 / threads;  // pieces of a thread in a step
+  constexpr int CH = 8 * FN;                   // chunks of four weight rows of a wave (epilogue)
+  static_assert(loads * 16 * threads == bytes, "a step is whole pieces of all threads");
+  static_assert(WN * WM * 32 * CH * 16 <= ring * bytes, "the epilogue fits the ring");
+  static_assert(RXMET_EXPERTS_MAX * 4 + 64 <= ring * bytes, "the experts' first tiles fit the ring");
+  __shared__ __attribute__((aligned(16))) int8_t s[ring][bytes];
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int col = lane % 32, h = lane / 32;
+  const int wide = a.gated ? TN / 2 : TN;  // columns of y
+  const int tiles_n = static_cast<int>((a.N + wide - 1) / wide);
+
+  // tiles of the experts before each one
+  int *first = reinterpret_cast<int *>(&s[0][0]), *sums = first + RXMET_EXPERTS_MAX;
+  int before = 0;
+  for (int base = 0; base < a.experts; base += threads) {
+    const int e = base + tid;
+    int n = 0;
+    if (e < a.experts) {
+      int64_t lo, hi;
+      places_of(a, e, lo, hi);
+      n = static_cast<int>((hi - lo + TM - 1) / TM);
+    }
+    int up = n;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_up(up, d, kWave);
+      if (lane >= d) up += o;
+    }
+    if (lane == kWave - 1) sums[wave] = up;
+    __syncthreads();
+    int add = before;
+#pragma unroll
+    for (int v = 0; v < WN * WM; ++v) {
+      const int t = sums[v];
+      if (v < wave) add += t;
+      before += t;
+    }
+    if (e < a.experts) first[e] = add + up - n;
+    __syncthreads();
+  }
+  // Workgroups go to the eight XCDs in turn: each XCD gets a run of the tiles' order, in which bands of
+  // four tiles of places go through the weights together, so that its L2 holds what they share.
+  const int64_t total = static_cast<int64_t>(before) * tiles_n;
+  const int xcd = blockIdx.x % 8;
+  const int64_t per = total / 8, rest = total % 8, at = blockIdx.x / 8;
+  if (at >= per + (xcd < rest)) return;
+  const int64_t id = xcd * per + (xcd < rest ? xcd : rest) + at;
+  const int band = static_cast<int>(id / (4 * tiles_n)) * 4, in = static_cast<int>(id - static_cast<int64_t>(band) * tiles_n);
+  const int high = before - band < 4 ? before - band : 4;
+  const int tm = band + in % high, tn = in / high;
+  int e = 0;
+  for (int d = RXMET_EXPERTS_MAX / 2; d > 0; d >>= 1)
+    if (e + d < a.experts && first[e + d] <= tm) e += d;
+  e = __builtin_amdgcn_readfirstlane(e);
+  int64_t m0, end;
+  places_of(a, e, m0, end);
+  const int within = tm - __builtin_amdgcn_readfirstlane(first[e]);
+  m0 += static_cast<int64_t>(within) * TM;
+  if (within < 0 || m0 >= end) return;  // offsets that do not rise
+  const int64_t n0 = static_cast<int64_t>(tn) * wide;
+  __syncthreads();
+
+  // piece j of a thread lies at place tid + threads * j of the step, which holds this piece of a row
+  const int8_t *src[loads];
+  auto piece_at = [&](int j) {
+    const int p = tid + threads * j, row = p / 4;
+    return (p % 4) ^ (row < TN ? turn_w(row) : turn_x(row - TN));
+  };
+#pragma unroll
+  for (int j = 0; j < loads; ++j) {
+    const int row = (tid + threads * j) / 4;
+    if (row < TN) {
+      constexpr int part = 32 * FN;  // weight rows of a wave
+      int64_t n = n0 + row, up = 0;
+      if (a.gated) {
+        n = n0 + row / part * (part / 2) + row % (part / 2);
+        up = row % part >= part / 2 ? a.N : 0;
+      }
+      src[j] = a.w + e * a.e_stride + ((n < a.N ? n : a.N - 1) + up) * a.w_stride;
+    } else {
+      const int64_t i = m0 + row - TN;
+      src[j] = a.x + row_of(a, i < end ? i : end - 1) * a.x_stride;
+    }
+  }
+  v16i acc[FN][FM];
+#pragma unroll
+  for (int i = 0; i < FN; ++i)
+#pragma unroll
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+  const int wn = wave % WN * (TN / WN), wm = wave / WN * (TM / WM);
+  int wat[FN][2], xat[FM][2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int row = wn + 32 * i + 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
+      wat[i][c] = row * kStep + ((2 * c + h) ^ turn_w(row)) * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+      const int row = wm + 32 * j + col;
+      xat[j][c] = (TN + row) * kStep + ((2 * c + h) ^ turn_x(row)) * 16;
+    }
+  }
+  struct Half {  // the operands of half a step
+    v4i w[FN], x[FM];
+  };
+  auto load = [&](Half &f, const int8_t *buf, int c) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const v4i *>(buf + wat[i][c]);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) f.x[j] = *reinterpret_cast<const v4i *>(buf + xat[j][c]);
+  };
+  auto multiply = [&](const Half &f) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+  };
+  const int whole = a.K / kStep;
+  if constexpr (ALIGNED) {
+    auto issue = [&](int step, int slot) {
+#pragma unroll
+      for (int j = 0; j < loads; ++j)
+        load_to_lds(src[j] + piece_at(j) * 16 + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
+    };
+    if (whole > 0) {
+      // past the end a step is read once more, so that the count of loads in flight holds
+#pragma unroll
+      for (int k = 0; k < ring; ++k) issue(k < whole ? k : 0, k);
+      wait_loads<(ring - 1) * loads>();
+      meet();
+      // each half's operands are read from LDS while the half before is multiplied
+      Half even, odd;
+      load(even, s[0], 0);
+      for (int k = 0; k < whole; ++k) {
+        load(odd, s[k % ring], 1);
+        multiply(even);
+        wait_loads<(ring - 2) * loads>();
+        meet();  // step k + 1 is there for all, and step k has been read by all
+        issue(k + ring < whole ? k + ring : k, k % ring);
+        load(even, s[(k + 1) % ring], 0);
+        multiply(odd);
+      }
+      wait_loads<0>();
+    }
+  } else {
+    uint4 piece[loads];
+    auto fetch = [&](int step) {
+#pragma unroll
+      for (int j = 0; j < loads; ++j) __builtin_memcpy(&piece[j], src[j] + piece_at(j) * 16 + step * kStep, 16);
+    };
+    auto put = [&](int slot) {
+#pragma unroll
+      for (int j = 0; j < loads; ++j) *reinterpret_cast<uint4 *>(&s[slot][16 * (tid + threads * j)]) = piece[j];
+    };
+    if (whole > 0) {
+      fetch(0);
+      put(0);
+      __syncthreads();
+    }
+    for (int k = 0; k < whole; ++k) {
+      if (k + 1 < whole) fetch(k + 1);
+      Half f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        load(f, s[k % 2], c);
+        multiply(f);
+      }
+      if (k + 1 < whole) put((k + 1) % 2);
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  if (whole * kStep < a.K) {  // the step that K ends in
+#pragma unroll
+    for (int j = 0; j < loads; ++j)
+      *reinterpret_cast<uint4 *>(&s[0][16 * (tid + threads * j)]) =
+          load_piece(src[j], whole * kStep + 16 * piece_at(j), a.K);
+    __syncthreads();
+    Half f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      load(f, s[0], c);
+      multiply(f);
+    }
+    __syncthreads();
+  }
+
+  // 32 places at a time the wave's sums go through its own part of the LDS, from where a lane finishes
+  // eight consecutive n of a place and neighbouring lanes write what lies side by side.  Chunk c of
+  // place m lies at c ^ turn, for the banks.
+  auto turn = [](int m) { return CH >= 16 ? m & 15 : m >> 1 & 7; };
+  v4i *part = reinterpret_cast<v4i *>(&s[0][0]) + wave * 32 * CH;
+  const int chunks = a.gated ? CH / 2 : CH;  // of four columns
+  const int64_t nw = n0 + (a.gated ? wn / 2 : wn);
+  bool large = false;
+  for (int r = lane; r < TM / WM; r += kWave) large |= m0 + wm + r < end && is_large(a.sx[row_of(a, m0 + wm + r)]);
+  large = __any(large);
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        part[col * CH + ((8 * i + 4 * h + k) ^ turn(col))] =
+            v4i{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+#pragma unroll 1
+    for (int at = lane; at < 16 * chunks; at += kWave) {
+      const int r = at / (chunks / 2), c = at % (chunks / 2) * 2;
+      auto eight = [&](int c, int (&v)[8]) {
+        const v4i lo = part[r * CH + (c ^ turn(r))], hi = part[r * CH + ((c + 1) ^ turn(r))];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = lo[k], v[4 + k] = hi[k];
+      };
+      int v[8], u[8];
+      eight(c, v);
+      if (a.gated)
+        eight(chunks + c, u);
+      else
+        eight(c, u);
+      const int64_t i = m0 + wm + 32 * j + r, n = nw + 4 * c;
+      if (i >= end || n >= a.N) continue;
+      const float sx = a.sx[row_of(a, i)];
+      if (large)
+        finish_as<8, true>(a, e, i, sx, n, v, u);
+      else
+        finish_as<8, false>(a, e, i, sx, n, v, u);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before it is written again
+  }
+}
+
+// Whether the rows can be read in aligned pieces of 16 bytes.
+bool aligned(const ExpertArgs &a) {
+  return (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) |
+          static_cast<uintptr_t>(a.x_stride) | static_cast<uintptr_t>(a.w_stride) |
+          static_cast<uintptr_t>(a.e_stride)) % 16 == 0;
+}
+
+template <int TN, int TM, int WN, int WM>
+void launch_tile(const ExpertArgs &a, hipStream_t st) {
+  // an expert's last tile may be partly filled; a run of an XCD is rounded up
+  const int64_t tiles_m = a.rows / TM + (a.experts < a.rows ? a.experts : a.rows);
+  const int64_t tiles = cdiv(a.N, a.gated ? TN / 2 : TN) * tiles_m;
+  const unsigned grid = static_cast<unsigned>(cdiv(tiles, 8) * 8);
+  if (aligned(a))
+    experts_tile<TN, TM, WN, WM, true><<<grid, 64 * WN * WM, 0, st>>>(a);
+  else
+    experts_tile<TN, TM, WN, WM, false><<<grid, 64 * WN * WM, 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace dec
+}  // namespace rxmet
+
+using namespace rxmet;
+using namespace rxmet::dec;
+
+extern "C" int rxmet_experts_linear_int8(const rxmet_expert_groups *g, int32_t grouped,
+                                         const int8_t *codes, int64_t codes_stride,
+                                         const float *scales, const int8_t *weight,
+                                         int64_t weight_stride, int64_t expert_stride,
+                                         const float *weight_scales, const void *bias, void *y,
+                                         int64_t N, int64_t K, int32_t gated, int32_t activation,
+                                         int32_t dtype, void *stream) {
+  RXMET_CHECK_ARG(g != nullptr, "the groups are missing");
+  RXMET_CHECK_ARG(g->experts >= 1 && g->experts <= RXMET_EXPERTS_MAX, "there must be 1 to 1024 experts");
+  RXMET_CHECK_ARG(g->top_k >= 1 && g->top_k <= RXMET_TOP_K_MAX, "top_k must be between 1 and 64");
+  RXMET_CHECK_ARG(g->tokens >= 0 && g->tokens <= 1 << 24, "there must be at most 2^24 tokens");
+  RXMET_CHECK_ARG(N >= 1 && N <= 1 << 24 && K >= 1 && K <= RXMET_LINEAR_INT8_K_MAX,
+                  "N must be between 1 and 2^24 and K between 1 and 131071");
+  RXMET_CHECK_ARG(activation >= RXMET_ACT_NONE && activation <= RXMET_ACT_GELU, "unknown activation");
+  RXMET_CHECK_ARG(dtype == RXMET_QDQ_F32 || dtype == RXMET_QDQ_F16 || dtype == RXMET_QDQ_BF16,
+                  "element type must be fp32, fp16 or bf16");
+  const int64_t rows = g->tokens * g->top_k;
+  if (rows == 0) return 0;
+  RXMET_CHECK_ARG(g->offsets && (grouped || g->entries), "the groups' offsets and entries are needed");
+  RXMET_CHECK_ARG(codes && scales && weight && weight_scales && y,
+                  "codes, weight, their scales and y are needed");
+  const ExpertArgs a{g->offsets, g->entries, g->tokens, rows, g->top_k, g->experts, grouped != 0,
+                     codes, weight, codes_stride, weight_stride, expert_stride, scales, weight_scales,
+                     bias, y, N, static_cast<int>(K), gated != 0, activation, dtype};
+  const int64_t few = cdiv(N, gated ? 8 : 16) * g->experts;
+  RXMET_CHECK_ARG(rows < 1 << 26 && few < 1 << 22 &&
+                      cdiv(N, gated ? 32 : 64) * (rows / 64 + g->experts) < 1 << 22,
+                  "too many outputs for one call");
+  auto st = static_cast<hipStream_t>(stream);
+  prof::Scope scope("experts_linear_int8", st);
+  if (rows <= 16LL * g->experts)
+    experts_few<<<static_cast<unsigned>(few), 64 * kFewWaves, 0, st>>>(a);
+  else if (rows <= 64LL * g->experts)
+    launch_tile<64, 64, 2, 2>(a, st);
+  else if (rows <= 256LL * g->experts)
+    launch_tile<128, 128, 2, 2>(a, st);
+  else
+    launch_tile<256, 256, 2, 4>(a, st);
+  RXMET_CHECK_LAUNCH();
+  return 0;
+}

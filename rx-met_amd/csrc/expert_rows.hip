@@ -1,0 +1,332 @@
+// expert_rows.hip — the entries in the experts' order, a token's rows added up, and the gradient of that.
+#include "../../include/rxmet_experts.h"
+#include "decoder_common.h"
+
+namespace rxmet {
+namespace dec {
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Order by expert: a counting sort that keeps the entries' order.  A workgroup has kChunk entries; its
+// counts go to memory, and a second launch adds up the counts of the chunks before, ranks the entries of
+// its chunk and writes both directions.  Up to kAlone entries one workgroup does it all in one launch.
+struct GroupArgs {
+  const int32_t *experts;
+  int64_t count;
+  int E, chunks;
+  int32_t *offsets, *entries, *places;
+  int32_t *counts;  // [chunks, E + 1]
+};
+
+constexpr int kChunk = 1024, kGroupWaves = kChunk / kWave;
+constexpr int64_t kAlone = 4096;
+constexpr int kBins = RXMET_EXPERTS_MAX + 1;  // the last one: entries of no expert
+
+__device__ __forceinline__ int bin_of(const GroupArgs &a, int64_t i) {
+  const int32_t e = a.experts[i];
+  return e >= 0 && e < a.E ? e : a.E;
+}
+
+__global__ __launch_bounds__(kChunk) void group_count(const GroupArgs a) {
+  __shared__ int s_count[kBins];
+  for (int b = threadIdx.x; b <= a.E; b += kChunk) s_count[b] = 0;
+  __syncthreads();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kChunk + threadIdx.x;
+  if (i < a.count) atomicAdd(&s_count[bin_of(a, i)], 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b <= a.E; b += kChunk)
+    a.counts[static_cast<int64_t>(blockIdx.x) * (a.E + 1) + b] = s_count[b];
+}
+
+// ALONE: one workgroup has all entries and counts them first.
+template <bool ALONE>
+__global__ __launch_bounds__(kChunk) void group_place(const GroupArgs a) {
+  __shared__ int s_all[kBins], s_at[kBins];  // entries of a bin; where its next one goes
+  __shared__ unsigned short s_wave[kGroupWaves][kBins];
+  __shared__ int s_sum[kGroupWaves];
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, bins = a.E + 1;
+  for (int b = tid; b < bins; b += kChunk) s_all[b] = s_at[b] = 0;
+  __syncthreads();
+  if (ALONE) {
+    for (int64_t i = tid; i < a.count; i += kChunk) atomicAdd(&s_all[bin_of(a, i)], 1);
+  } else {
+    // each bin's column of counts by as many threads as there are
+    const int columns = bins < kChunk ? bins : kChunk, share = kChunk / columns;
+    if (tid < columns * share)
+      for (int b = tid % columns; b < bins; b += columns) {
+        int all = 0, mine = 0;
+        for (int c = tid / columns; c < a.chunks; c += share) {
+          const int n = a.counts[static_cast<int64_t>(c) * bins + b];
+          all += n;
+          mine += c < static_cast<int>(blockIdx.x) ? n : 0;
+        }
+        atomicAdd(&s_all[b], all);
+        atomicAdd(&s_at[b], mine);
+      }
+  }
+  __syncthreads();
+  // places before each bin; bins beyond the threads go around again
+  int before = 0;
+  for (int base = 0; base < bins; base += kChunk) {
+    const int b = base + tid, n = b < bins ? s_all[b] : 0;
+    int up = n;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int o = __shfl_up(up, d, kWave);
+      if (lane >= d) up += o;
+    }
+    if (lane == kWave - 1) s_sum[wave] = up;
+    __syncthreads();
+    int first = before + up - n;
+    for (int v = 0; v < kGroupWaves; ++v) {
+      if (v < wave) first += s_sum[v];
+      before += s_sum[v];
+    }
+    if (b < bins) {
+      s_at[b] += first;
+      if (blockIdx.x == 0) a.offsets[b] = first;  // of the last bin: where the experts' entries end
+    }
+    __syncthreads();
+  }
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * kChunk, to = ALONE ? a.count : from + 1;
+  for (int64_t base = from; base < to; base += kChunk) {
+    for (int b = lane; b < bins; b += kWave) s_wave[wave][b] = 0;
+    const int64_t i = base + tid;
+    const int bin = i < a.count ? bin_of(a, i) : bins;  // lanes behind the end stand apart
+    // lanes of the same bin
+    unsigned long long same = ~0ull;
+    for (int bit = 1; bit <= bins; bit <<= 1) {
+      const unsigned long long set = __ballot((bin & bit) != 0);
+      same &= bin & bit ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    __syncthreads();
+    if (bin < bins && rank == 0) s_wave[wave][bin] = static_cast<unsigned short>(__popcll(same));
+    __syncthreads();
+    for (int b = tid; b < bins; b += kChunk) {  // counts of the waves before; the bin moves on
+      int n = 0;
+      for (int v = 0; v < kGroupWaves; ++v) {
+        const int c = s_wave[v][b];
+        s_wave[v][b] = static_cast<unsigned short>(n);
+        n += c;
+      }
+      s_all[b] = s_at[b];
+      s_at[b] += n;
+    }
+    __syncthreads();
+    if (bin < bins) {
+      const int place = s_all[bin] + s_wave[wave][bin] + rank;
+      a.entries[place] = static_cast<int32_t>(i);
+      a.places[i] = bin < a.E ? place : -1;
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Rows added up: a run of threads has a token's row, eight columns a thread, and adds the rows of
+// its entries in fp32 in their order.  Bound: the rows' bytes.
+struct CombineArgs {
+  const int32_t *offsets, *places;
+  int64_t tokens, rows;
+  int top_k, experts;
+  const void *y, *res, *d_out;
+  int64_t y_stride, res_stride, d_stride;
+  const float *weights;
+  void *out, *d_y;
+  float *d_weights;
+  int64_t N;
+  int shift;  // 2^shift threads have a row
+};
+
+template <typename T>
+__device__ __forceinline__ void load_any(const T *p, int64_t left, float (&f)[8]) {
+  if (left >= 8)
+    load8(p, f);
+  else
+    load8_part(p, static_cast<int>(left), f);
+}
+template <typename T>
+__device__ __forceinline__ void store_any(T *p, int64_t left, const float (&f)[8]) {
+  if (left >= 8)
+    store8(p, f);
+  else
+    store8_part(p, static_cast<int>(left), f);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_rows(const CombineArgs a) {
+  const int width = 1 << a.shift, lane = threadIdx.x & (width - 1);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (256 >> a.shift) + (threadIdx.x >> a.shift);
+  if (t >= a.tokens) return;
+  const int32_t *place = a.places + t * a.top_k;
+  const float *w = a.weights + t * a.top_k;
+  for (int64_t n = 8 * lane; n < a.N; n += 8 * width) {
+    const int64_t left = a.N - n;
+    float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+    for (int j = 0; j < a.top_k; ++j) {
+      const int64_t p = place[j];
+      if (p < 0 || p >= a.rows) continue;
+      float v[8];
+      load_any(static_cast<const T *>(a.y) + p * a.y_stride + n, left, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] = __builtin_fmaf(w[j], v[e], sum[e]);
+    }
+    if (a.res) {
+      float v[8];
+      load_any(static_cast<const T *>(a.res) + t * a.res_stride + n, left, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    }
+    store_any(static_cast<T *>(a.out) + t * a.N + n, left, sum);
+  }
+}
+
+// The gradient: a workgroup has a token, reads its gradient once for up to kTogether of its rows,
+// writes theirs and adds up their products with y.  Rows of no expert are cleared by all workgroups.
+constexpr int kTogether = 4;
+
+template <typename T>
+__global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
+  __shared__ float s_dot[4][kTogether];
+  const int64_t t = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int32_t *place = a.places + t * a.top_k;
+  for (int j0 = 0; j0 < a.top_k; j0 += kTogether) {
+    int64_t p[kTogether];
+    float w[kTogether], dot[kTogether];
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j) {
+      p[j] = j0 + j < a.top_k ? place[j0 + j] : -1;
+      if (p[j] >= a.rows) p[j] = -1;
+      w[j] = j0 + j < a.top_k ? a.weights[t * a.top_k + j0 + j] : 0.0f;
+      dot[j] = 0;
+    }
+    for (int64_t n = 8 * tid; n < a.N; n += 8 * 256) {
+      const int64_t left = a.N - n;
+      float g[8];
+      load_any(static_cast<const T *>(a.d_out) + t * a.d_stride + n, left, g);
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+        if (p[j] < 0) continue;
+        if (a.d_weights) {
+          float v[8];
+          load_any(static_cast<const T *>(a.y) + p[j] * a.y_stride + n, left, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot[j] = __builtin_fmaf(g[e], v[e], dot[j]);
+        }
+        if (a.d_y) {
+          float d[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = w[j] * g[e];
+          store_any(static_cast<T *>(a.d_y) + p[j] * a.N + n, left, d);
+        }
+      }
+    }
+    if (a.d_weights) {
+#pragma unroll
+      for (int j = 0; j < kTogether; ++j) {
+#pragma unroll
+        for (int d = kWave / 2; d > 0; d >>= 1) dot[j] += __shfl_xor(dot[j], d, kWave);
+        if (lane == 0) s_dot[wave][j] = dot[j];
+      }
+      __syncthreads();
+      if (tid < kTogether && j0 + tid < a.top_k)
+        a.d_weights[t * a.top_k + j0 + tid] = s_dot[0][tid] + s_dot[1][tid] + s_dot[2][tid] + s_dot[3][tid];
+      __syncthreads();
+    }
+  }
+  if (!a.d_y) return;
+  const int64_t held = a.offsets[a.experts];
+  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int64_t i = (held < 0 ? 0 : held) + t; i < a.rows; i += a.tokens)
+    for (int64_t n = 8 * tid; n < a.N; n += 8 * 256)
+      store_any(static_cast<T *>(a.d_y) + i * a.N + n, a.N - n, zero);
+}
+
+int check_groups(const rxmet_expert_groups *g, int64_t N, int32_t dtype) {
+  RXMET_CHECK_ARG(g != nullptr, "the groups are missing");
+  RXMET_CHECK_ARG(g->experts >= 1 && g->experts <= RXMET_EXPERTS_MAX, "there must be 1 to 1024 experts");
+  RXMET_CHECK_ARG(g->top_k >= 1 && g->top_k <= RXMET_TOP_K_MAX, "top_k must be between 1 and 64");
+  RXMET_CHECK_ARG(g->tokens >= 0 && g->tokens <= 1 << 23, "there must be at most 2^23 tokens");
+  RXMET_CHECK_ARG(N >= 1 && N <= 1 << 24, "N must be between 1 and 2^24");
+  RXMET_CHECK_ARG(dtype == RXMET_QDQ_F32 || dtype == RXMET_QDQ_F16 || dtype == RXMET_QDQ_BF16,
+                  "element type must be fp32, fp16 or bf16");
+  return 0;
+}
+
+}  // namespace
+}  // namespace dec
+}  // namespace rxmet
+
+using namespace rxmet;
+using namespace rxmet::dec;
+
+extern "C" int64_t rxmet_group_experts_workspace_bytes(int64_t count, int32_t num_experts) {
+  if (count <= kAlone || num_experts < 1) return 0;
+  return cdiv(count, kChunk) * (num_experts + 1) * 4;
+}
+
+extern "C" int rxmet_group_experts(const int32_t *experts, int64_t count, int32_t num_experts,
+                                   int32_t *offsets, int32_t *entries, int32_t *places,
+                                   void *workspace, void *stream) {
+  RXMET_CHECK_ARG(num_experts >= 1 && num_experts <= RXMET_EXPERTS_MAX, "there must be 1 to 1024 experts");
+  RXMET_CHECK_ARG(count >= 0 && count <= 1 << 26, "there must be at most 2^26 entries");
+  RXMET_CHECK_ARG(offsets != nullptr, "offsets are needed");
+  RXMET_CHECK_ARG(count == 0 || (experts && entries && places), "experts, entries and places are needed");
+  RXMET_CHECK_ARG(count <= kAlone || workspace, "this call needs a workspace");
+  auto st = static_cast<hipStream_t>(stream);
+  prof::Scope scope("group_experts", st);
+  const int chunks = static_cast<int>(cdiv(count, kChunk));
+  const GroupArgs a{experts, count, num_experts, chunks, offsets, entries, places,
+                    static_cast<int32_t *>(workspace)};
+  if (count <= kAlone) {
+    group_place<true><<<1, kChunk, 0, st>>>(a);
+  } else {
+    group_count<<<chunks, kChunk, 0, st>>>(a);
+    group_place<false><<<chunks, kChunk, 0, st>>>(a);
+  }
+  RXMET_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int rxmet_experts_combine(const rxmet_expert_groups *g, const void *y, int64_t y_stride,
+                                     const float *weights, const void *residual,
+                                     int64_t residual_stride, void *out, int64_t N, int32_t dtype,
+                                     void *stream) {
+  if (const int rc = check_groups(g, N, dtype)) return rc;
+  if (g->tokens == 0) return 0;
+  RXMET_CHECK_ARG(g->places && y && weights && out, "places, y, weights and out are needed");
+  int shift = 0;
+  while (shift < 8 && (8LL << shift) < N) ++shift;
+  const CombineArgs a{g->offsets, g->places, g->tokens, g->tokens * g->top_k, g->top_k, g->experts, y,
+                      residual, nullptr, y_stride, residual_stride, 0, weights, out, nullptr, nullptr, N, shift};
+  auto st = static_cast<hipStream_t>(stream);
+  prof::Scope scope("experts_combine", st);
+  with_type(dtype, [&](auto t) {
+    combine_rows<decltype(t)><<<static_cast<unsigned>(cdiv(g->tokens, 256 >> shift)), 256, 0, st>>>(a);
+  });
+  RXMET_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int rxmet_experts_combine_backward(const rxmet_expert_groups *g, const void *d_out,
+                                              int64_t d_out_stride, const void *y, int64_t y_stride,
+                                              const float *weights, void *d_y, float *d_weights,
+                                              int64_t N, int32_t dtype, void *stream) {
+  if (const int rc = check_groups(g, N, dtype)) return rc;
+  if (g->tokens == 0 || (!d_y && !d_weights)) return 0;
+  RXMET_CHECK_ARG(g->places && d_out && weights, "places, d_out and weights are needed");
+  RXMET_CHECK_ARG(!d_y || g->offsets, "d_y needs the groups' offsets");
+  RXMET_CHECK_ARG(!d_weights || y, "d_weights needs y");
+  const CombineArgs a{g->offsets, g->places, g->tokens, g->tokens * g->top_k, g->top_k, g->experts, y,
+                      nullptr, d_out, y_stride, 0, d_out_stride, weights, nullptr, d_y, d_weights, N, 0};
+  auto st = static_cast<hipStream_t>(stream);
+  prof::Scope scope("experts_combine_backward", st);
+  with_type(dtype, [&](auto t) {
+    combine_backward<decltype(t)><<<static_cast<unsigned>(g->tokens), 256, 0, st>>>(a);
+  });
+  RXMET_CHECK_LAUNCH();
+  return 0;
+}

@@ -69,15 +69,31 @@ class KvTable(ctypes.Structure):
                 ("cols", ctypes.c_int32)]
 
 
+class Router(ctypes.Structure):
+    """rxmet_router (include/rxmet_experts.h): how a token's experts are chosen and weighed."""
+    _fields_ = [("experts", ctypes.c_int32), ("top_k", ctypes.c_int32), ("score", ctypes.c_int32),
+                ("renormalize", ctypes.c_int32), ("groups", ctypes.c_int32),
+                ("top_groups", ctypes.c_int32), ("group_best", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class ExpertGroups(ctypes.Structure):
+    """rxmet_expert_groups: the entries in the experts' order."""
+    _fields_ = [("offsets", c_ptr), ("entries", c_ptr), ("places", c_ptr), ("tokens", c_i64),
+                ("top_k", ctypes.c_int32), ("experts", ctypes.c_int32)]
+
+
 _LAY = ctypes.POINTER(QdqLayout)
 _MME = ctypes.POINTER(QdqMinMaxEnc)
 _NUM = ctypes.POINTER(QdqNumerics)
 _KVC = ctypes.POINTER(KvCache)
 _KVT = ctypes.POINTER(KvTable)
+_RTR = ctypes.POINTER(Router)
+_GRP = ctypes.POINTER(ExpertGroups)
 _i32 = ctypes.c_int32
 
-# name -> (restype, argtypes); mirrors include/rxmet_qdq.h, include/rxmet_decoder.h and the shared
-# entry points
+# name -> (restype, argtypes); mirrors include/rxmet_qdq.h, include/rxmet_decoder.h,
+# include/rxmet_experts.h and the shared entry points
 _SIGNATURES = {
     "rxmet_last_error": (ctypes.c_char_p, []),
     "rxmet_abi_version": (c_int, []),
@@ -140,6 +156,17 @@ _SIGNATURES = {
     "rxmet_kv_attention_workspace_bytes": (c_i64, [_KVC, _i32, c_i64, _i32, c_i64, c_i64, c_i64]),
     "rxmet_kv_attention": (c_int, [_KVC, _KVT, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_ptr, c_i64,
                                    c_i64, _i32, c_float, _i32, c_i64, c_ptr, _i32, c_ptr, c_ptr]),
+    "rxmet_route_forward": (c_int, [_RTR, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64, _i32, c_ptr]),
+    "rxmet_route_backward": (c_int, [_RTR, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64, _i32, c_ptr]),
+    "rxmet_group_experts_workspace_bytes": (c_i64, [c_i64, _i32]),
+    "rxmet_group_experts": (c_int, [c_ptr, c_i64, _i32, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "rxmet_experts_linear_int8": (c_int, [_GRP, _i32, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i64,
+                                          c_ptr, c_ptr, c_ptr, c_i64, c_i64, _i32, _i32, _i32,
+                                          c_ptr]),
+    "rxmet_experts_combine": (c_int, [_GRP, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_ptr, c_i64, _i32,
+                                      c_ptr]),
+    "rxmet_experts_combine_backward": (c_int, [_GRP, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr,
+                                               c_ptr, c_i64, _i32, c_ptr]),
 }
 
 
