@@ -99,11 +99,12 @@ def build_ort_ops(verbose: bool = True) -> Path | None:
     return ORT_LIB
 
 
-# The autograd node of the learnable min / max path (torch_ext/rxmet_torch.cpp) and the decoder
-# operators' calls (decoder_torch.cpp): host code over PyTorch's C++ headers, without a link to
-# librxmet.so (it is handed the entry points of the loaded one).  Users of the C ABI alone need no
-# PyTorch: without it this module is not built.
-TORCH_SRC = (PKG / "torch_ext" / "rxmet_torch.cpp", PKG / "torch_ext" / "decoder_torch.cpp")
+# The autograd node of the learnable min / max path (torch_ext/rxmet_torch.cpp) and the calls of the
+# decoder's and the experts' operators (decoder_torch.cpp, expert_torch.cpp): host code over PyTorch's
+# C++ headers, without a link to librxmet.so (it is handed the entry points of the loaded one).  Users of
+# the C ABI alone need no PyTorch: without it this module is not built.
+TORCH_SRC = tuple(PKG / "torch_ext" / n for n in ("rxmet_torch.cpp", "decoder_torch.cpp",
+                                                  "expert_torch.cpp"))
 TORCH_LIB = PKG / ("rxmet_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 

@@ -29,6 +29,25 @@ TOP_K_MAX = 64
 GROUPS_MAX = 64
 SCORES = {"softmax": 0, "sigmoid": 1}
 
+_NATIVE = ("rxmet_route_forward", "rxmet_route_backward", "rxmet_group_experts",
+           "rxmet_group_experts_workspace_bytes", "rxmet_experts_linear_int8",
+           "rxmet_experts_combine", "rxmet_experts_combine_backward", "rxmet_last_error")
+_ext = None
+
+
+def _native():
+    """The same calls in C++ (module ``rxmet_torch``, torch_ext/expert_torch.cpp); False where the
+    module cannot be imported.  They return None for what needs a copy or has to be refused: that
+    is done here."""
+    global _ext
+    if _ext is None:
+        ext = _rx.torch_ext()
+        if ext is not None:
+            lib = _rx.load()
+            ext.bind_experts([ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _NATIVE])
+        _ext = ext or False
+    return _ext
+
 
 # ---------------------------------------------------------------------------------
 # Routing
@@ -128,6 +147,12 @@ def route_experts(logits, top_k: int, score: str = "softmax", bias=None, groups:
     logits float32, float16 or bfloat16, E up to 1024, top_k up to 64.  Differentiable in logits; the
     bias and the choice get no gradient.
     """
+    ext = _ext or _native()
+    if ext and score in SCORES and not torch._C._are_functorch_transforms_active():
+        out = ext.route_experts(logits, top_k, SCORES[score], bias, groups, top_groups, group_best,
+                                renormalize, scale)
+        if out is not None:
+            return out
     _not_traced("route_experts")
     _on_gpu(logits, "logits")
     _float_type(logits, "logits")
@@ -158,6 +183,11 @@ def group_experts(experts, num_experts: int) -> ExpertGroups:
     """The order of the entries of experts int32 [..., top_k] by expert; entries of an expert keep
     theirs.  Ids outside 0..num_experts - 1 belong to no expert (experts of another process,
     tokens of a padded batch): such entries are multiplied and added up by nothing."""
+    ext = _ext or _native()
+    if ext:
+        out = ext.group_experts(experts, num_experts)
+        if out is not None:
+            return ExpertGroups(*out)
     _not_traced("group_experts")
     _on_gpu(experts, "experts")
     dev = experts.device
@@ -216,6 +246,12 @@ def experts_linear_int8(codes, scales, weight, weight_scales, groups: ExpertGrou
     The sum over K is exact, the rest float32.  K is at most 131071.  Rows behind the experts' last place are
     not written.  Rows that do not start on 16 bytes (K no multiple of 16) are read more slowly.
     """
+    ext = _ext or _native()
+    if ext and activation in ACTIVATIONS:
+        out = ext.experts_linear_int8(codes, scales, weight, weight_scales, *groups, bias,
+                                      ACTIVATIONS[activation], gated, grouped, dtype)
+        if out is not None:
+            return out
     _not_traced("experts_linear_int8")
     _on_gpu(codes, "codes")
     dev = codes.device
@@ -321,6 +357,11 @@ def experts_combine(y, weights, groups: ExpertGroups, residual=None) -> torch.Te
     order of j, rounded once.  Entries of no expert add nothing; their rows of y are not read.
     Differentiable in y (0 for the rows of no expert), weights and residual.
     """
+    ext = _ext or _native()
+    if ext and not torch._C._are_functorch_transforms_active():
+        out = ext.experts_combine(y, weights, residual, *groups)
+        if out is not None:
+            return out
     _not_traced("experts_combine")
     _on_gpu(y, "y")
     _float_type(y, "y")

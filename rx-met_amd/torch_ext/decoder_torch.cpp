@@ -6,23 +6,16 @@
 // and refuse nothing: they return None for everything else (a wrong type, shape, device or stride, a tensor
 // subclass, a trace, which would record the allocations without the kernels), and decoder_ops.py then
 // goes its own way, which copies or raises.
-#include "rxmet_torch.h"
+#include "operator_calls.h"
 
-#include <ATen/TensorSubclassLikeUtils.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
-#include <optional>
 
 #include "rxmet_decoder.h"
-#include "rxmet_qdq.h"
 
 namespace rxmet_torch {
 namespace {
-
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
 
 // The entry points of the librxmet.so that rxmet_lib.py has loaded (bind_decoder()).
 decltype(&rxmet_rms_quantize_forward) rms_forward = nullptr;
@@ -34,51 +27,6 @@ decltype(&rxmet_kv_append) append = nullptr;
 decltype(&rxmet_kv_read) read = nullptr;
 decltype(&rxmet_kv_attention) attention = nullptr;
 decltype(&rxmet_kv_attention_workspace_bytes) attention_bytes = nullptr;
-const char *(*last_error)(void) = nullptr;
-
-void check(int rc, const char *what) {
-  if (rc != 0)
-    throw LibraryError(std::string(what) + " failed (" + std::to_string(rc) + "): " + last_error());
-}
-
-int type_code(at::ScalarType t) {
-  switch (t) {
-    case at::kFloat: return RXMET_QDQ_F32;
-    case at::kHalf: return RXMET_QDQ_F16;
-    case at::kBFloat16: return RXMET_QDQ_BF16;
-    default: return -1;
-  }
-}
-
-bool plain(const Tensor &t) {
-  return t.is_cuda() && !at::isTensorSubclassLike(t) && !torch::jit::tracer::isTracing();
-}
-
-bool is(const Tensor &t, at::ScalarType type, const Tensor &like) {
-  return t.scalar_type() == type && plain(t) && t.device() == like.device();
-}
-
-// t as rows with a dense last axis; false where that takes a copy.
-bool as_rows(const Tensor &t, int64_t &rows, int64_t &cols, int64_t &stride) {
-  if (t.dim() < 1) return false;
-  cols = t.size(-1);
-  if (cols < 1) return false;
-  if (t.is_contiguous()) {
-    rows = t.numel() / cols;
-    stride = cols;
-    return true;
-  }
-  if (t.dim() != 2 || t.stride(1) != 1) return false;
-  rows = t.size(0);
-  stride = t.stride(0);
-  return true;
-}
-
-bool vector_of(const Tensor &t, int64_t n) {
-  return t.dim() == 1 && t.size(0) == n && t.is_contiguous();
-}
-
-const void *ptr(const OptTensor &t) { return t ? t->const_data_ptr() : nullptr; }
 
 struct Rows {
   Tensor codes, y, scales, rstd, h;

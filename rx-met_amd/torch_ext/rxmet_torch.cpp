@@ -153,4 +153,5 @@ PYBIND11_MODULE(rxmet_torch, m) {
   m.def("make_plan", &make_plan);
   m.def("qdq_minmax", &qdq_minmax);
   rxmet_torch::add_decoder(m);
+  rxmet_torch::add_experts(m);
 }

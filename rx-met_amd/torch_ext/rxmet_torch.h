@@ -22,5 +22,7 @@ inline void *stream_of(const at::Tensor &t) {
 
 // decoder_torch.cpp
 void add_decoder(pybind11::module_ &m);
+// expert_torch.cpp
+void add_experts(pybind11::module_ &m);
 
 }  // namespace rxmet_torch
