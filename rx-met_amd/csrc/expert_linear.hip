@@ -43,14 +43,14 @@ __device__ __forceinline__ int64_t row_of(const ExpertArgs &a, int64_t i) {
 }
 
 // Finishes and writes C consecutive n of place i; v: the sums of the values where gated.
-template <typename T, int C, bool LARGE>
+template <typename T, int C>
 __device__ __forceinline__ void finish(const ExpertArgs &a, int e, int64_t i, float sx, int64_t n0,
                                        const int (&acc)[C], const int (&val)[C]) {
   const int64_t first = static_cast<int64_t>(e) * a.N * (1 + a.gated) + n0;
   const float *sw = a.sw + first;
   const T *bias = a.bias ? static_cast<const T *>(a.bias) + first : nullptr;
   T *y = static_cast<T *>(a.y) + i * a.N + n0;
-  const bool large = LARGE && is_large(sx);
+  const bool large = is_large(sx);
   auto scaled = [&](int acc, float w, T b) {
     const float v = static_cast<float>(acc) * (large ? w : sx) * (large ? sx : w);
     return bias ? v + static_cast<float>(b) : v;
@@ -85,15 +85,15 @@ __device__ __forceinline__ void finish(const ExpertArgs &a, int e, int64_t i, fl
   }
 }
 
-template <int C, bool LARGE = true>
-__device__ __forceinline__ void finish_as(const ExpertArgs &a, int e, int64_t i, float sx, int64_t n0,
-                                          const int (&acc)[C], const int (&val)[C]) {
-  if (a.dtype == RXMET_QDQ_BF16)
-    finish<bf16, C, LARGE>(a, e, i, sx, n0, acc, val);
-  else if (a.dtype == RXMET_QDQ_F16)
-    finish<f16, C, LARGE>(a, e, i, sx, n0, acc, val);
+// f(T{}) for an element type that the host has checked.
+template <typename F>
+__device__ __forceinline__ void with_type_of(int dtype, F &&f) {
+  if (dtype == RXMET_QDQ_BF16)
+    f(bf16{});
+  else if (dtype == RXMET_QDQ_F16)
+    f(f16{});
   else
-    finish<float, C, LARGE>(a, e, i, sx, n0, acc, val);
+    f(float{});
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -157,7 +157,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few(const ExpertArgs a
       const v4i p = sum(c), q = a.gated ? sum(8 + c) : p;
       const int acc4[4] = {p[0], p[1], p[2], p[3]}, val4[4] = {q[0], q[1], q[2], q[3]};
       if (m0 + m < to && n0 + c < a.N)
-        finish_as<4>(a, e, m0 + m, a.sx[row_of(a, m0 + m)], n0 + c, acc4, val4);
+        with_type_of(a.dtype, [&](auto t) {
+          finish<decltype(t), 4>(a, e, m0 + m, a.sx[row_of(a, m0 + m)], n0 + c, acc4, val4);
+        });
     }
     __syncthreads();
   }
@@ -166,25 +168,28 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few(const ExpertArgs a
 // ---------------------------------------------------------------------------------------------
 // Tiles of TN weight rows x TM places of one expert on mfma 32x32x32; WN x WM waves take equal parts.
 // Where gated, a wave's weight rows are gates in their first half and the same columns' values in the
-// second.  K goes through LDS in steps of 64 bytes, memory -> LDS without registers, three steps ahead in
-// a ring of four; pieces of a row and rows of a wave lie as in linear_int8.hip.  Rows that do not start
-// on 16 bytes (ALIGNED false) go through registers, one step ahead.
-template <int TN, int TM, int WN, int WM, bool ALIGNED>
-__global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a) {
+// second, so that a lane holds both.
+//
+// K goes through LDS in steps of 64 bytes, memory -> LDS without registers, two steps ahead in a ring of
+// three; pieces of a row and rows of a wave lie as in linear_int8.hip.  Rows that do not start on 16
+// bytes (ALIGNED false) go through registers, one step ahead.  Scales and bias wait in LDS for the end.
+template <int TN, int TM, int WN, int WM, bool GATED, bool ALIGNED>
+__global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 128 * 64 ? 3 : 4) void experts_tile(const ExpertArgs a) {
   constexpr int threads = 64 * WN * WM;
   constexpr int FN = TN / WN / 32, FM = TM / WM / 32;
   constexpr int bytes = (TN + TM) * kStep;
-  constexpr int ring = 4;
+  constexpr int ring = 3;
   constexpr int loads = bytes / 16 / threads;  // pieces of a thread in a step
-  constexpr int CH = 8 * FN;                   // chunks of four weight rows of a wave (epilogue)
+  constexpr int wide = GATED ? TN / 2 : TN;    // columns of y
   static_assert(loads * 16 * threads == bytes, "a step is whole pieces of all threads");
-  static_assert(WN * WM * 32 * CH * 16 <= ring * bytes, "the epilogue fits the ring");
-  static_assert(RXMET_EXPERTS_MAX * 4 + 64 <= ring * bytes, "the experts' first tiles fit the ring");
+  static_assert(!GATED || FN % 2 == 0, "a wave has gates and values");
+  static_assert(TN * 32 * WM * 4 <= ring * bytes, "the epilogue fits the ring");
+  static_assert(RXMET_EXPERTS_MAX * 4 + 64 <= ring * bytes, "the experts' tiles fit the ring");
   __shared__ __attribute__((aligned(16))) int8_t s[ring][bytes];
+  __shared__ __attribute__((aligned(16))) float s_sw[TN], s_bias[TN], s_sx[TM];
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int col = lane % 32, h = lane / 32;
-  const int wide = a.gated ? TN / 2 : TN;  // columns of y
   const int tiles_n = static_cast<int>((a.N + wide - 1) / wide);
 
   // tiles of the experts before each one
@@ -238,6 +243,12 @@ __global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a)
   const int64_t n0 = static_cast<int64_t>(tn) * wide;
   __syncthreads();
 
+  // the weight row of a tile's row, for one past the columns the last
+  constexpr int part = 32 * FN;  // weight rows of a wave
+  auto weight_row = [&](int row) {
+    const int64_t n = GATED ? n0 + row / part * (part / 2) + row % (part / 2) : n0 + row;
+    return (n < a.N ? n : a.N - 1) + (GATED && row % part >= part / 2 ? a.N : 0);
+  };
   // piece j of a thread lies at place tid + threads * j of the step, which holds this piece of a row
   const int8_t *src[loads];
   auto piece_at = [&](int j) {
@@ -248,17 +259,23 @@ __global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a)
   for (int j = 0; j < loads; ++j) {
     const int row = (tid + threads * j) / 4;
     if (row < TN) {
-      constexpr int part = 32 * FN;  // weight rows of a wave
-      int64_t n = n0 + row, up = 0;
-      if (a.gated) {
-        n = n0 + row / part * (part / 2) + row % (part / 2);
-        up = row % part >= part / 2 ? a.N : 0;
-      }
-      src[j] = a.w + e * a.e_stride + ((n < a.N ? n : a.N - 1) + up) * a.w_stride;
+      src[j] = a.w + e * a.e_stride + weight_row(row) * a.w_stride;
     } else {
       const int64_t i = m0 + row - TN;
       src[j] = a.x + row_of(a, i < end ? i : end - 1) * a.x_stride;
     }
+  }
+  {
+    const int64_t row0 = static_cast<int64_t>(e) * a.N * (GATED ? 2 : 1);
+    for (int r = tid; r < TN; r += threads) {
+      const int64_t n = row0 + weight_row(r);
+      s_sw[r] = a.sw[n];
+      float b = 0;
+      if (a.bias)
+        with_type_of(a.dtype, [&](auto t) { b = static_cast<float>(static_cast<const decltype(t) *>(a.bias)[n]); });
+      s_bias[r] = b;
+    }
+    for (int r = tid; r < TM; r += threads) s_sx[r] = a.sx[row_of(a, m0 + r < end ? m0 + r : end - 1)];
   }
   v16i acc[FN][FM];
 #pragma unroll
@@ -300,10 +317,12 @@ __global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a)
   };
   const int whole = a.K / kStep;
   if constexpr (ALIGNED) {
+#pragma unroll
+    for (int j = 0; j < loads; ++j) src[j] += piece_at(j) * 16;
     auto issue = [&](int step, int slot) {
 #pragma unroll
       for (int j = 0; j < loads; ++j)
-        load_to_lds(src[j] + piece_at(j) * 16 + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
+        load_to_lds(src[j] + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
     };
     if (whole > 0) {
       // past the end a step is read once more, so that the count of loads in flight holds
@@ -314,22 +333,31 @@ __global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a)
       // each half's operands are read from LDS while the half before is multiplied
       Half even, odd;
       load(even, s[0], 0);
+      int slot = 0;
       for (int k = 0; k < whole; ++k) {
-        load(odd, s[k % ring], 1);
+        const int next = slot + 1 == ring ? 0 : slot + 1;
+        load(odd, s[slot], 1);
         multiply(even);
         wait_loads<(ring - 2) * loads>();
         meet();  // step k + 1 is there for all, and step k has been read by all
-        issue(k + ring < whole ? k + ring : k, k % ring);
-        load(even, s[(k + 1) % ring], 0);
+        issue(k + ring < whole ? k + ring : k, slot);
+        load(even, s[next], 0);
         multiply(odd);
+        slot = next;
       }
       wait_loads<0>();
     }
+#pragma unroll
+    for (int j = 0; j < loads; ++j) src[j] -= piece_at(j) * 16;
   } else {
     uint4 piece[loads];
     auto fetch = [&](int step) {
 #pragma unroll
-      for (int j = 0; j < loads; ++j) __builtin_memcpy(&piece[j], src[j] + piece_at(j) * 16 + step * kStep, 16);
+      for (int j = 0; j < loads; ++j) {
+        uint4 v;
+        __builtin_memcpy(&v, src[j] + piece_at(j) * 16 + step * kStep, 16);
+        piece[j] = v;
+      }
     };
     auto put = [&](int slot) {
 #pragma unroll
@@ -368,49 +396,71 @@ __global__ __launch_bounds__(64 * WN * WM) void experts_tile(const ExpertArgs a)
     __syncthreads();
   }
 
-  // 32 places at a time the wave's sums go through its own part of the LDS, from where a lane finishes
-  // eight consecutive n of a place and neighbouring lanes write what lies side by side.  Chunk c of
-  // place m lies at c ^ turn, for the banks.
-  auto turn = [](int m) { return CH >= 16 ? m & 15 : m >> 1 & 7; };
-  v4i *part = reinterpret_cast<v4i *>(&s[0][0]) + wave * 32 * CH;
-  const int chunks = a.gated ? CH / 2 : CH;  // of four columns
-  const int64_t nw = n0 + (a.gated ? wn / 2 : wn);
-  bool large = false;
-  for (int r = lane; r < TM / WM; r += kWave) large |= m0 + wm + r < end && is_large(a.sx[row_of(a, m0 + wm + r)]);
-  large = __any(large);
+  // A lane finishes its 16 consecutive columns of a place; 32 places at a time go through the wave's part of the
+  // LDS, from where neighbouring lanes write what lies side by side.  Chunk c of place m lies at
+  // c ^ m, for the banks.
+  with_type_of(a.dtype, [&](auto type) {
+    using T = decltype(type);
+    constexpr int elems = 16 / sizeof(T);                    // of a chunk
+    constexpr int CH = (GATED ? 16 : 32) * FN / elems;       // chunks of a place
+    uint4 *out = reinterpret_cast<uint4 *>(&s[0][0]) + wave * 32 * CH;
+    const int64_t nw = n0 + (GATED ? wn / 2 : wn);
 #pragma unroll
-  for (int j = 0; j < FM; ++j) {
+    for (int j = 0; j < FM; ++j) {
+      const float sx = s_sx[wm + 32 * j + col];
+      const float lead = is_large(sx) ? 1.0f : sx, rest = is_large(sx) ? sx : 1.0f;
 #pragma unroll
-    for (int i = 0; i < FN; ++i)
+      for (int i = 0; i < (GATED ? FN / 2 : FN); ++i) {
+        T y[16];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        part[col * CH + ((8 * i + 4 * h + k) ^ turn(col))] =
-            v4i{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-#pragma unroll 1
-    for (int at = lane; at < 16 * chunks; at += kWave) {
-      const int r = at / (chunks / 2), c = at % (chunks / 2) * 2;
-      auto eight = [&](int c, int (&v)[8]) {
-        const v4i lo = part[r * CH + (c ^ turn(r))], hi = part[r * CH + ((c + 1) ^ turn(r))];
+        for (int q = 0; q < 4; ++q) {
+          const int r0 = wn + 32 * i + 16 * h + 4 * q;
+          const f4 sw = *reinterpret_cast<const f4 *>(&s_sw[r0]), b = *reinterpret_cast<const f4 *>(&s_bias[r0]);
+          f4 sv, bv;
+          if (GATED) {
+            sv = *reinterpret_cast<const f4 *>(&s_sw[r0 + part / 2]);
+            bv = *reinterpret_cast<const f4 *>(&s_bias[r0 + part / 2]);
+          }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = lo[k], v[4 + k] = hi[k];
-      };
-      int v[8], u[8];
-      eight(c, v);
-      if (a.gated)
-        eight(chunks + c, u);
-      else
-        eight(c, u);
-      const int64_t i = m0 + wm + 32 * j + r, n = nw + 4 * c;
-      if (i >= end || n >= a.N) continue;
-      const float sx = a.sx[row_of(a, i)];
-      if (large)
-        finish_as<8, true>(a, e, i, sx, n, v, u);
-      else
-        finish_as<8, false>(a, e, i, sx, n, v, u);
+          for (int r = 0; r < 4; ++r) {
+            float v = static_cast<float>(acc[i][j][4 * q + r]) * lead * sw[r] * rest;
+            if (a.bias) v += b[r];
+            v = activate(v, a.act);
+            if (GATED) {
+              float u = static_cast<float>(acc[FN / 2 + i][j][4 * q + r]) * lead * sv[r] * rest;
+              if (a.bias) u += bv[r];
+              v *= u;
+            }
+            y[4 * q + r] = static_cast<T>(v);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 16 / elems; ++c) {
+          uint4 w;
+          __builtin_memcpy(&w, &y[c * elems], 16);
+          out[col * CH + (((32 * i + 16 * h) / elems + c) ^ (col & (CH < 16 ? CH - 1 : 15)))] = w;
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      for (int at = lane; at < 32 * CH; at += kWave) {
+        const int m = at / CH, c = at % CH;
+        const uint4 w = out[m * CH + (c ^ (m & (CH < 16 ? CH - 1 : 15)))];
+        const int64_t i = m0 + wm + 32 * j + m, n = nw + c * elems;
+        if (i >= end || n >= a.N) continue;
+        T *y = static_cast<T *>(a.y) + i * a.N + n;
+        if (n + elems <= a.N) {
+          __builtin_memcpy(y, &w, 16);
+        } else {
+          T v[elems];
+          __builtin_memcpy(v, &w, 16);
+#pragma unroll
+          for (int c = 0; c < elems; ++c)
+            if (n + c < a.N) y[c] = v[c];
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before it is written again
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before it is written again
-  }
+  });
 }
 
 // Whether the rows can be read in aligned pieces of 16 bytes.
@@ -420,16 +470,26 @@ bool aligned(const ExpertArgs &a) {
           static_cast<uintptr_t>(a.e_stride)) % 16 == 0;
 }
 
-template <int TN, int TM, int WN, int WM>
+template <int TN, int TM, int WN, int WM, bool GATED>
 void launch_tile(const ExpertArgs &a, hipStream_t st) {
   // an expert's last tile may be partly filled; a run of an XCD is rounded up
   const int64_t tiles_m = a.rows / TM + (a.experts < a.rows ? a.experts : a.rows);
-  const int64_t tiles = cdiv(a.N, a.gated ? TN / 2 : TN) * tiles_m;
+  const int64_t tiles = cdiv(a.N, GATED ? TN / 2 : TN) * tiles_m;
   const unsigned grid = static_cast<unsigned>(cdiv(tiles, 8) * 8);
   if (aligned(a))
-    experts_tile<TN, TM, WN, WM, true><<<grid, 64 * WN * WM, 0, st>>>(a);
+    experts_tile<TN, TM, WN, WM, GATED, true><<<grid, 64 * WN * WM, 0, st>>>(a);
   else
-    experts_tile<TN, TM, WN, WM, false><<<grid, 64 * WN * WM, 0, st>>>(a);
+    experts_tile<TN, TM, WN, WM, GATED, false><<<grid, 64 * WN * WM, 0, st>>>(a);
+}
+
+template <bool GATED>
+void launch_tiles(const ExpertArgs &a, hipStream_t st) {
+  if (a.rows <= 64LL * a.experts)
+    launch_tile<128, 64, 2, 2, GATED>(a, st);
+  else if (a.rows <= 256LL * a.experts)
+    launch_tile<128, 128, 2, 2, GATED>(a, st);
+  else
+    launch_tile<256, 128, 2, 2, GATED>(a, st);
 }
 
 }  // namespace
@@ -465,18 +525,16 @@ extern "C" int rxmet_experts_linear_int8(const rxmet_expert_groups *g, int32_t g
                      bias, y, N, static_cast<int>(K), gated != 0, activation, dtype};
   const int64_t few = cdiv(N, gated ? 8 : 16) * g->experts;
   RXMET_CHECK_ARG(rows < 1 << 26 && few < 1 << 22 &&
-                      cdiv(N, gated ? 32 : 64) * (rows / 64 + g->experts) < 1 << 22,
+                      cdiv(N, gated ? 64 : 128) * (rows / 64 + g->experts) < 1 << 22,
                   "too many outputs for one call");
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_linear_int8", st);
   if (rows <= 16LL * g->experts)
     experts_few<<<static_cast<unsigned>(few), 64 * kFewWaves, 0, st>>>(a);
-  else if (rows <= 64LL * g->experts)
-    launch_tile<64, 64, 2, 2>(a, st);
-  else if (rows <= 256LL * g->experts)
-    launch_tile<128, 128, 2, 2>(a, st);
+  else if (a.gated)
+    launch_tiles<true>(a, st);
   else
-    launch_tile<256, 256, 2, 4>(a, st);
+    launch_tiles<false>(a, st);
   RXMET_CHECK_LAUNCH();
   return 0;
 }
