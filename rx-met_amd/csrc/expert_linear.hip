@@ -178,7 +178,7 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 1
   constexpr int threads = 64 * WN * WM;
   constexpr int FN = TN / WN / 32, FM = TM / WM / 32;
   constexpr int bytes = (TN + TM) * kStep;
-  constexpr int ring = 3;
+  constexpr int ring = TN * TM > 256 * 128 ? 4 : 3;
   constexpr int loads = bytes / 16 / threads;  // pieces of a thread in a step
   constexpr int wide = GATED ? TN / 2 : TN;    // columns of y
   static_assert(loads * 16 * threads == bytes, "a step is whole pieces of all threads");
@@ -398,69 +398,76 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 1
 
   // A lane finishes its 16 consecutive columns of a place; 32 places at a time go through the wave's part of the
   // LDS, from where neighbouring lanes write what lies side by side.  Chunk c of place m lies at
-  // c ^ m, for the banks.
-  with_type_of(a.dtype, [&](auto type) {
+  // c ^ m, for the banks.  The activation is chosen once: asked for at each element, the code that is
+  // jumped over falls out of the instruction cache.
+  const int size = a.dtype == RXMET_QDQ_F32 ? 4 : 2;          // bytes of an element
+  const int CH = (GATED ? 16 : 32) * FN * size / 16;          // chunks of a place
+  const int mask = CH < 16 ? CH - 1 : 15;
+  uint4 *out = reinterpret_cast<uint4 *>(&s[0][0]) + wave * 32 * CH;
+  auto put = [&](auto type, int n, const float (&v)[16]) {
     using T = decltype(type);
-    constexpr int elems = 16 / sizeof(T);                    // of a chunk
-    constexpr int CH = (GATED ? 16 : 32) * FN / elems;       // chunks of a place
-    uint4 *out = reinterpret_cast<uint4 *>(&s[0][0]) + wave * 32 * CH;
-    const int64_t nw = n0 + (GATED ? wn / 2 : wn);
+    T y[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[r] = static_cast<T>(v[r]);
+#pragma unroll
+    for (int c = 0; c < static_cast<int>(sizeof(T)); ++c) {
+      uint4 w;
+      __builtin_memcpy(&w, &y[c * 16 / sizeof(T)], 16);
+      out[col * CH + ((n / (16 / static_cast<int>(sizeof(T))) + c) ^ (col & mask))] = w;
+    }
+  };
+  auto finish_tile = [&](auto act) {
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
       const float sx = s_sx[wm + 32 * j + col];
       const float lead = is_large(sx) ? 1.0f : sx, rest = is_large(sx) ? sx : 1.0f;
 #pragma unroll
       for (int i = 0; i < (GATED ? FN / 2 : FN); ++i) {
-        T y[16];
+        float y[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int r0 = wn + 32 * i + 16 * h + 4 * q;
+          auto scaled = [&](int sum, float w, float b) { return static_cast<float>(sum) * lead * w * rest + b; };
           const f4 sw = *reinterpret_cast<const f4 *>(&s_sw[r0]), b = *reinterpret_cast<const f4 *>(&s_bias[r0]);
-          f4 sv, bv;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            y[4 * q + r] = activate(scaled(acc[i][j][4 * q + r], sw[r], b[r]), decltype(act)::value);
           if (GATED) {
-            sv = *reinterpret_cast<const f4 *>(&s_sw[r0 + part / 2]);
-            bv = *reinterpret_cast<const f4 *>(&s_bias[r0 + part / 2]);
-          }
+            const f4 sv = *reinterpret_cast<const f4 *>(&s_sw[r0 + part / 2]);
+            const f4 bv = *reinterpret_cast<const f4 *>(&s_bias[r0 + part / 2]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = static_cast<float>(acc[i][j][4 * q + r]) * lead * sw[r] * rest;
-            if (a.bias) v += b[r];
-            v = activate(v, a.act);
-            if (GATED) {
-              float u = static_cast<float>(acc[FN / 2 + i][j][4 * q + r]) * lead * sv[r] * rest;
-              if (a.bias) u += bv[r];
-              v *= u;
-            }
-            y[4 * q + r] = static_cast<T>(v);
+            for (int r = 0; r < 4; ++r) y[4 * q + r] *= scaled(acc[FN / 2 + i][j][4 * q + r], sv[r], bv[r]);
           }
         }
-#pragma unroll
-        for (int c = 0; c < 16 / elems; ++c) {
-          uint4 w;
-          __builtin_memcpy(&w, &y[c * elems], 16);
-          out[col * CH + (((32 * i + 16 * h) / elems + c) ^ (col & (CH < 16 ? CH - 1 : 15)))] = w;
-        }
+        with_type_of(a.dtype, [&](auto type) { put(type, 32 * i + 16 * h, y); });
       }
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       for (int at = lane; at < 32 * CH; at += kWave) {
         const int m = at / CH, c = at % CH;
-        const uint4 w = out[m * CH + (c ^ (m & (CH < 16 ? CH - 1 : 15)))];
-        const int64_t i = m0 + wm + 32 * j + m, n = nw + c * elems;
+        const uint4 w = out[m * CH + (c ^ (m & mask))];
+        const int64_t i = m0 + wm + 32 * j + m, n = n0 + (GATED ? wn / 2 : wn) + c * 16 / size;
         if (i >= end || n >= a.N) continue;
-        T *y = static_cast<T *>(a.y) + i * a.N + n;
-        if (n + elems <= a.N) {
+        char *y = static_cast<char *>(a.y) + (i * a.N + n) * size;
+        const int64_t left = (a.N - n) * size;
+        if (left >= 16) {
           __builtin_memcpy(y, &w, 16);
         } else {
-          T v[elems];
-          __builtin_memcpy(v, &w, 16);
+          const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int c = 0; c < elems; ++c)
-            if (n + c < a.N) y[c] = v[c];
+          for (int b = 0; b < 16; b += 2)
+            if (b < left) *reinterpret_cast<unsigned short *>(y + b) = static_cast<unsigned short>(u[b / 4] >> (8 * (b % 4)));
         }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before it is written again
     }
-  });
+  };
+  using std::integral_constant;
+  switch (a.act) {
+    case RXMET_ACT_RELU: finish_tile(integral_constant<int, RXMET_ACT_RELU>{}); break;
+    case RXMET_ACT_SILU: finish_tile(integral_constant<int, RXMET_ACT_SILU>{}); break;
+    case RXMET_ACT_GELU: finish_tile(integral_constant<int, RXMET_ACT_GELU>{}); break;
+    default: finish_tile(integral_constant<int, RXMET_ACT_NONE>{});
+  }
 }
 
 // Whether the rows can be read in aligned pieces of 16 bytes.
