@@ -170,15 +170,23 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few(const ExpertArgs a
 // Where gated, a wave's weight rows are gates in their first half and the same columns' values in the
 // second, so that a lane holds both.
 //
-// K goes through LDS in steps of 64 bytes, memory -> LDS without registers, two steps ahead in a ring of
-// three; pieces of a row and rows of a wave lie as in linear_int8.hip.  Rows that do not start on 16
-// bytes (ALIGNED false) go through registers, one step ahead.  Scales and bias wait in LDS for the end.
+// K goes through LDS in steps of 128 bytes, memory -> LDS without registers, one step ahead.  A row's
+// eight 16-byte pieces lie at the places piece ^ f(row), so that 16 lanes that read one piece of 16 rows meet
+// 16 different bank groups.  Row i of a wave's 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) +
+// i % 4: a lane holds 16 consecutive n of one place.  Rows that do not start on 16 bytes (ALIGNED
+// false) go through registers.  Scales and bias wait in LDS for the end.
+constexpr int kWide = 128;  // bytes of K in a step
+
+// f of a weight row and of a row of codes
+__device__ __forceinline__ int wide_turn_w(int row) { return (row >> 1 & 3) | (row >> 2 & 4); }
+__device__ __forceinline__ int wide_turn_x(int row) { return row >> 1 & 7; }
+
 template <int TN, int TM, int WN, int WM, bool GATED, bool ALIGNED>
-__global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 128 * 64 ? 3 : 4) void experts_tile(const ExpertArgs a) {
+__global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 64 ? 2 : 3) void experts_tile(const ExpertArgs a) {
   constexpr int threads = 64 * WN * WM;
   constexpr int FN = TN / WN / 32, FM = TM / WM / 32;
-  constexpr int bytes = (TN + TM) * kStep;
-  constexpr int ring = TN * TM > 256 * 128 ? 4 : 3;
+  constexpr int bytes = (TN + TM) * kWide;
+  constexpr int ring = 2;
   constexpr int loads = bytes / 16 / threads;  // pieces of a thread in a step
   constexpr int wide = GATED ? TN / 2 : TN;    // columns of y
   static_assert(loads * 16 * threads == bytes, "a step is whole pieces of all threads");
@@ -252,12 +260,12 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 1
   // piece j of a thread lies at place tid + threads * j of the step, which holds this piece of a row
   const int8_t *src[loads];
   auto piece_at = [&](int j) {
-    const int p = tid + threads * j, row = p / 4;
-    return (p % 4) ^ (row < TN ? turn_w(row) : turn_x(row - TN));
+    const int p = tid + threads * j, row = p / 8;
+    return (p % 8) ^ (row < TN ? wide_turn_w(row) : wide_turn_x(row - TN));
   };
 #pragma unroll
   for (int j = 0; j < loads; ++j) {
-    const int row = (tid + threads * j) / 4;
+    const int row = (tid + threads * j) / 8;
     if (row < TN) {
       src[j] = a.w + e * a.e_stride + weight_row(row) * a.w_stride;
     } else {
@@ -285,77 +293,69 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 1
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
   const int wn = wave % WN * (TN / WN), wm = wave / WN * (TM / WM);
-  int wat[FN][2], xat[FM][2];
+  // 32 rows on, a row has the same f: one place for each quarter of a step
+  int wat[4], xat[4];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-#pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      const int row = wn + 32 * i + 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);
-      wat[i][c] = row * kStep + ((2 * c + h) ^ turn_w(row)) * 16;
-    }
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int row = wm + 32 * j + col;
-      xat[j][c] = (TN + row) * kStep + ((2 * c + h) ^ turn_x(row)) * 16;
-    }
+  for (int c = 0; c < 4; ++c) {
+    const int w = wn + 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3), x = wm + col;
+    wat[c] = w * kWide + ((2 * c + h) ^ wide_turn_w(w)) * 16;
+    xat[c] = (TN + x) * kWide + ((2 * c + h) ^ wide_turn_x(x)) * 16;
   }
-  struct Half {  // the operands of half a step
+  struct Quarter {  // the operands of a quarter of a step
     v4i w[FN], x[FM];
   };
-  auto load = [&](Half &f, const int8_t *buf, int c) {
+  auto load = [&](Quarter &f, const int8_t *buf, int c) {
 #pragma unroll
-    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const v4i *>(buf + wat[i][c]);
+    for (int i = 0; i < FN; ++i) f.w[i] = *reinterpret_cast<const v4i *>(buf + wat[c] + 32 * i * kWide);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) f.x[j] = *reinterpret_cast<const v4i *>(buf + xat[j][c]);
+    for (int j = 0; j < FM; ++j) f.x[j] = *reinterpret_cast<const v4i *>(buf + xat[c] + 32 * j * kWide);
   };
-  auto multiply = [&](const Half &f) {
+  auto multiply = [&](const Quarter &f) {
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
       for (int j = 0; j < FM; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
   };
-  const int whole = a.K / kStep;
+  const int whole = a.K / kWide;
   if constexpr (ALIGNED) {
-#pragma unroll
-    for (int j = 0; j < loads; ++j) src[j] += piece_at(j) * 16;
     auto issue = [&](int step, int slot) {
 #pragma unroll
       for (int j = 0; j < loads; ++j)
-        load_to_lds(src[j] + step * kStep, &s[slot][wave * 1024 + j * threads * 16]);
+        load_to_lds(src[j] + piece_at(j) * 16 + step * kWide, &s[slot][wave * 1024 + j * threads * 16]);
     };
     if (whole > 0) {
       // past the end a step is read once more, so that the count of loads in flight holds
-#pragma unroll
-      for (int k = 0; k < ring; ++k) issue(k < whole ? k : 0, k);
-      wait_loads<(ring - 1) * loads>();
+      issue(0, 0);
+      issue(whole > 1 ? 1 : 0, 1);
+      wait_loads<loads>();
       meet();
-      // each half's operands are read from LDS while the half before is multiplied
-      Half even, odd;
+      // each quarter's operands are read from LDS while the quarter before is multiplied
+      Quarter even, odd;
       load(even, s[0], 0);
-      int slot = 0;
       for (int k = 0; k < whole; ++k) {
-        const int next = slot + 1 == ring ? 0 : slot + 1;
+        const int slot = k & 1;
         load(odd, s[slot], 1);
         multiply(even);
-        wait_loads<(ring - 2) * loads>();
-        meet();  // step k + 1 is there for all, and step k has been read by all
-        issue(k + ring < whole ? k + ring : k, slot);
-        load(even, s[next], 0);
+        load(even, s[slot], 2);
         multiply(odd);
-        slot = next;
+        load(odd, s[slot], 3);
+        multiply(even);
+        wait_loads<0>();
+        meet();  // step k + 1 is there for all, and step k has been read by all
+        load(even, s[slot ^ 1], 0);
+        issue(k + 2 < whole ? k + 2 : k, slot);
+        multiply(odd);
       }
       wait_loads<0>();
     }
-#pragma unroll
-    for (int j = 0; j < loads; ++j) src[j] -= piece_at(j) * 16;
   } else {
     uint4 piece[loads];
     auto fetch = [&](int step) {
 #pragma unroll
       for (int j = 0; j < loads; ++j) {
         uint4 v;
-        __builtin_memcpy(&v, src[j] + piece_at(j) * 16 + step * kStep, 16);
+        __builtin_memcpy(&v, src[j] + piece_at(j) * 16 + step * kWide, 16);
         piece[j] = v;
       }
     };
@@ -370,9 +370,9 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 1
     }
     for (int k = 0; k < whole; ++k) {
       if (k + 1 < whole) fetch(k + 1);
-      Half f;
+      Quarter f;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < 4; ++c) {
         load(f, s[k % 2], c);
         multiply(f);
       }
@@ -381,15 +381,15 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 128 ? 2 : TN * TM > 1
     }
   }
   __syncthreads();
-  if (whole * kStep < a.K) {  // the step that K ends in
+  if (whole * kWide < a.K) {  // the step that K ends in
 #pragma unroll
     for (int j = 0; j < loads; ++j)
       *reinterpret_cast<uint4 *>(&s[0][16 * (tid + threads * j)]) =
-          load_piece(src[j], whole * kStep + 16 * piece_at(j), a.K);
+          load_piece(src[j], whole * kWide + 16 * piece_at(j), a.K);
     __syncthreads();
-    Half f;
+    Quarter f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 4; ++c) {
       load(f, s[0], c);
       multiply(f);
     }
@@ -496,7 +496,7 @@ void launch_tiles(const ExpertArgs &a, hipStream_t st) {
   else if (a.rows <= 256LL * a.experts)
     launch_tile<128, 128, 2, 2, GATED>(a, st);
   else
-    launch_tile<256, 128, 2, 2, GATED>(a, st);
+    launch_tile<256, 256, 2, 4, GATED>(a, st);
 }
 
 }  // namespace
