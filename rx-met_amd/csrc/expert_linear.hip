@@ -96,72 +96,132 @@ __device__ __forceinline__ void with_type_of(int dtype, F &&f) {
     f(float{});
 }
 
-// ---------------------------------------------------------------------------------------------
-// Few rows of an expert: a workgroup takes 16 weight rows of one expert (gated: 8 gates and their 8
-// values) and all of K, its eight waves take runs of 128 of K in turn; the weights go from memory
-// into the matrix instruction with no stop in LDS, for 16 rows of codes at a time.  The eight sums meet in LDS.
-constexpr int kFewWaves = 8;
+constexpr int kWide = 128;  // bytes of K in a step: a whole line of each row
 
-__global__ __launch_bounds__(64 * kFewWaves) void experts_few(const ExpertArgs a) {
-  __shared__ int s[kFewWaves][16][20];
-  const int tiles = static_cast<int>((a.N + (a.gated ? 7 : 15)) / (a.gated ? 8 : 16));
+// ---------------------------------------------------------------------------------------------
+// Few rows of an expert: WK waves have 32 weight rows of one expert (gated: 16 gates and their 16
+// values), each every WK-th step of K, and multiply 16 places at a time on mfma 16x16x64.  A wave's steps go memory
+// -> LDS without registers, some steps ahead in a ring of its own, so that waves wait for memory and not
+// for each other; their sums meet in LDS at the end.  Rows that do not start on 16 bytes (ALIGNED
+// false) go from memory into the matrix instruction.
+constexpr int kFewRows = 32, kFewPlaces = 16;
+
+template <int WK, bool ALIGNED>
+__global__ __launch_bounds__(64 * WK) void experts_few(const ExpertArgs a) {
+  constexpr int depth = 4;
+  constexpr int bytes = (kFewRows + kFewPlaces) * kWide, loads = bytes / 1024;
+  __shared__ __attribute__((aligned(16))) int8_t s[WK][ALIGNED ? depth * bytes : 2048];
+  const int width = a.gated ? kFewRows / 2 : kFewRows;
+  const int tiles = static_cast<int>((a.N + width - 1) / width);
   const int e = blockIdx.x / tiles;
   int64_t from, to;
   places_of(a, e, from, to);
   if (from >= to) return;
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int col = lane % 16, g = lane / 16;
-  const int width = a.gated ? 8 : 16;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x % tiles) * width;
-  const int64_t n = n0 + col % width;
-  const int8_t *w = a.w + e * a.e_stride + ((n < a.N ? n : a.N - 1) + (col >= width ? a.N : 0)) * a.w_stride;
-  for (int64_t m0 = from; m0 < to; m0 += 16) {
-    const int8_t *x = a.x + row_of(a, m0 + col < to ? m0 + col : to - 1) * a.x_stride;
-    v4i acc = {0, 0, 0, 0};
-    constexpr int turn = kFewWaves * 128;  // from a wave's run of K to its next
-    auto runs = [&](auto N, int k0) {      // N of them, all their loads before the first product
-      v4i wf[N.value][2], xf[N.value][2];
+  auto weight_row = [&](int row) {
+    const int64_t n = n0 + (a.gated ? row % 16 : row);
+    return a.w + e * a.e_stride + ((n < a.N ? n : a.N - 1) + (a.gated && row >= 16 ? a.N : 0)) * a.w_stride;
+  };
+  const int whole = a.K / kWide;
+  for (int64_t m0 = from; m0 < to; m0 += kFewPlaces) {
+    auto code_row = [&](int row) { return a.x + row_of(a, m0 + row < to ? m0 + row : to - 1) * a.x_stride; };
+    v4i acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if constexpr (ALIGNED) {
+      // a load takes eight rows; piece p of row r lies at p ^ (r / 2 % 8), for the banks
+      const int8_t *src[loads];
 #pragma unroll
-      for (int i = 0; i < N.value; ++i)
+      for (int j = 0; j < loads; ++j) {
+        const int row = 8 * j + lane / 8;
+        src[j] = (8 * j < kFewRows ? weight_row(row) : code_row(row - kFewRows)) + (lane % 8 ^ (row >> 1 & 7)) * 16;
+      }
+      auto issue = [&](int step, int slot) {
+#pragma unroll
+        for (int j = 0; j < loads; ++j) load_to_lds(src[j] + step * kWide, &s[wave][slot * bytes + 1024 * j]);
+      };
+      const int mine = whole > wave ? (whole - wave + WK - 1) / WK : 0;
+#pragma unroll
+      for (int i = 0; i < depth; ++i)
+        if (i < mine) issue(wave + i * WK, i);
+      int slot = 0;
+      for (int i = 0; i < mine; ++i) {
+        if (i + depth <= mine)
+          wait_loads<(depth - 1) * loads>();
+        else
+          wait_loads<0>();
+        const int8_t *buf = &s[wave][slot * bytes];
+        v4i wf[2][2], xf[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int k = k0 + turn * i + 64 * c + 16 * g;
-          __builtin_memcpy(&wf[i][c], w + k, 16);
-          __builtin_memcpy(&xf[i][c], x + k, 16);
+          const int at = col * kWide + ((4 * c + g) ^ (col >> 1 & 7)) * 16;
+          wf[0][c] = *reinterpret_cast<const v4i *>(buf + at);
+          wf[1][c] = *reinterpret_cast<const v4i *>(buf + 16 * kWide + at);
+          xf[c] = *reinterpret_cast<const v4i *>(buf + kFewRows * kWide + at);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // read before it is written again
+        if (i + depth < mine) issue(wave + (i + depth) * WK, slot);
 #pragma unroll
-      for (int i = 0; i < N.value; ++i)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) acc = mfma_i8(wf[i][c], xf[i][c], acc);
-    };
-    int k0 = wave * 128;
-    for (; k0 + turn + 128 <= a.K; k0 += 2 * turn) runs(std::integral_constant<int, 2>{}, k0);
-    for (; k0 + 128 <= a.K; k0 += turn) runs(std::integral_constant<int, 1>{}, k0);
-    if (k0 < a.K) {  // K ends in this run
+          for (int f = 0; f < 2; ++f) acc[f] = mfma_i8(wf[f][c], xf[c], acc[f]);
+        slot = slot + 1 == depth ? 0 : slot + 1;
+      }
+    } else {
+      const int8_t *w[2] = {weight_row(col), weight_row(16 + col)}, *x = code_row(col);
+      auto steps = [&](auto N, int k0) {  // N of them, all their loads before the first product
+        v4i wf[N.value][2][2], xf[N.value][2];
+#pragma unroll
+        for (int i = 0; i < N.value; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int k = (k0 + WK * i) * kWide + 64 * c + 16 * g;
+            __builtin_memcpy(&wf[i][0][c], w[0] + k, 16);
+            __builtin_memcpy(&wf[i][1][c], w[1] + k, 16);
+            __builtin_memcpy(&xf[i][c], x + k, 16);
+          }
+#pragma unroll
+        for (int i = 0; i < N.value; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) acc[f] = mfma_i8(wf[i][f][c], xf[i][c], acc[f]);
+      };
+      int k = wave;
+      for (; k + 3 * WK < whole; k += 4 * WK) steps(std::integral_constant<int, 4>{}, k);
+      for (; k < whole; k += WK) steps(std::integral_constant<int, 1>{}, k);
+    }
+    if (whole * kWide < a.K && whole % WK == wave) {  // the step that K ends in
+      const int8_t *w[2] = {weight_row(col), weight_row(16 + col)}, *x = code_row(col);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int k = k0 + 64 * c + 16 * g;
-        acc = mfma_i8(as_v4i(load_piece(w, k, a.K)), as_v4i(load_piece(x, k, a.K)), acc);
+        const int k = whole * kWide + 64 * c + 16 * g;
+        const v4i xf = as_v4i(load_piece(x, k, a.K));
+#pragma unroll
+        for (int f = 0; f < 2; ++f) acc[f] = mfma_i8(as_v4i(load_piece(w[f], k, a.K)), xf, acc[f]);
       }
     }
-    *reinterpret_cast<v4i *>(&s[wave][col][4 * g]) = acc;
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < 16 * width / 4) {
-      const int m = threadIdx.x / (width / 4), c = threadIdx.x % (width / 4) * 4;
-      auto sum = [&](int at) {
-        v4i t = *reinterpret_cast<const v4i *>(&s[0][m][at]);
+    if (WK > 1) {
+      v4i *sums = reinterpret_cast<v4i *>(&s[wave][0]);
+      sums[lane] = acc[0];
+      sums[kWave + lane] = acc[1];
+      __syncthreads();
+      if (wave == 0)
 #pragma unroll
-        for (int v = 1; v < kFewWaves; ++v) t += *reinterpret_cast<const v4i *>(&s[v][m][at]);
-        return t;
-      };
-      const v4i p = sum(c), q = a.gated ? sum(8 + c) : p;
-      const int acc4[4] = {p[0], p[1], p[2], p[3]}, val4[4] = {q[0], q[1], q[2], q[3]};
-      if (m0 + m < to && n0 + c < a.N)
-        with_type_of(a.dtype, [&](auto t) {
-          finish<decltype(t), 4>(a, e, m0 + m, a.sx[row_of(a, m0 + m)], n0 + c, acc4, val4);
-        });
+        for (int v = 1; v < WK; ++v)
+#pragma unroll
+          for (int f = 0; f < 2; ++f) acc[f] += reinterpret_cast<const v4i *>(&s[v][0])[kWave * f + lane];
     }
-    __syncthreads();
+    if (wave == 0 && m0 + col < to) {
+      const float sx = a.sx[row_of(a, m0 + col)];
+      const int p[4] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3]}, q[4] = {acc[1][0], acc[1][1], acc[1][2], acc[1][3]};
+      with_type_of(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        if (n0 + 4 * g < a.N) finish<T, 4>(a, e, m0 + col, sx, n0 + 4 * g, p, q);
+        if (!a.gated && n0 + 16 + 4 * g < a.N) finish<T, 4>(a, e, m0 + col, sx, n0 + 16 + 4 * g, q, q);
+      });
+    }
+    if (WK > 1) __syncthreads();
   }
 }
 
@@ -175,8 +235,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void experts_few(const ExpertArgs a
 // 16 different bank groups.  Row i of a wave's 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) +
 // i % 4: a lane holds 16 consecutive n of one place.  Rows that do not start on 16 bytes (ALIGNED
 // false) go through registers.  Scales and bias wait in LDS for the end.
-constexpr int kWide = 128;  // bytes of K in a step
-
 // silu by the hardware's exponential and reciprocal (each within a step of fp32): 5 instructions instead of 25.
 __device__ __forceinline__ float quick_activate(float v, int act) {
   if (act != RXMET_ACT_SILU) return activate(v, act);
@@ -538,14 +596,51 @@ void launch_tile(const ExpertArgs &a, hipStream_t st) {
     experts_tile<TN, TM, WN, WM, GATED, false><<<grid, 64 * WN * WM, 0, st>>>(a);
 }
 
-template <bool GATED>
-void launch_tiles(const ExpertArgs &a, hipStream_t st) {
-  if (a.rows <= 64LL * a.experts)
-    launch_tile<128, 64, 2, 2, GATED>(a, st);
-  else if (a.rows <= 256LL * a.experts)
-    launch_tile<128, 128, 2, 2, GATED>(a, st);
+template <int WK>
+void launch_few(const ExpertArgs &a, int64_t grid, hipStream_t st) {
+  const unsigned n = static_cast<unsigned>(grid);
+  if (aligned(a))
+    experts_few<WK, true><<<n, 64 * WK, 0, st>>>(a);
   else
-    launch_tile<256, 256, 2, 4, GATED>(a, st);
+    experts_few<WK, false><<<n, 64 * WK, 0, st>>>(a);
+}
+
+// How a call is run, by how many rows an expert has (R / E) and how much weight there is to stream.
+//
+// Up to 16 rows each: the smallest tiles where there are three for two CUs ([64 x 2048, 2048] gated weights of 64
+// experts, 128 rows: 45.8 us, 5.2 TB/s; experts_few 48.1), else experts_few, whose waves are more (16
+// experts of [2048, 2048], 16 rows: 11.9 us against 16.0), and where those are fewer than 128, four waves
+// for each 32 weight rows (4 experts of [512, 4096]: 8.0 us, one wave 11.0).  Experts that have rows are
+// at most as many as rows.
+//
+// More: a tile size costs its rounds of tiles over the CUs (half a round more, for the last one is not
+// full) times what a round takes; of 32 experts with [2048, 2048], [R / E: 256 x 256, 128 x 128, 128 x 64]
+// 64: 40 28 29 us; 256: 72 67 65; 384: 105 91 97; 512: 108 116 118; 2048: 388 441 481.
+enum Shape { kFewShared, kFewOne, k128x64, k128x128, k256x256 };
+
+Shape shape_for(int64_t rows, int64_t experts, int64_t out_rows) {
+  const int64_t busy = rows < experts ? rows : experts;
+  if (rows <= 16 * experts && busy * cdiv(out_rows, 128) < 384)
+    return busy * cdiv(out_rows, 32) < 128 ? kFewShared : kFewOne;
+  // tiles of an expert's rows, the last one half full; relative time of a round, tiles that a CU holds
+  auto cost = [&](int64_t tn, int64_t tm, double round, int held) {
+    const double tiles = static_cast<double>(cdiv(out_rows, tn)) * (static_cast<double>(rows) / tm + busy / 2.0);
+    return (tiles / (256 * held) + 0.5) * round;
+  };
+  const double small = cost(128, 64, 22, 3), middle = cost(128, 128, 26, 2), large = cost(256, 256, 43, 1);
+  return small <= middle && small <= large ? k128x64 : middle <= large ? k128x128 : k256x256;
+}
+
+template <bool GATED>
+void launch(const ExpertArgs &a, hipStream_t st) {
+  const int64_t few = cdiv(a.N, GATED ? kFewRows / 2 : kFewRows) * a.experts;
+  switch (shape_for(a.rows, a.experts, GATED ? 2 * a.N : a.N)) {
+    case kFewShared: launch_few<4>(a, few, st); break;
+    case kFewOne: launch_few<1>(a, few, st); break;
+    case k128x64: launch_tile<128, 64, 2, 2, GATED>(a, st); break;
+    case k128x128: launch_tile<128, 128, 2, 2, GATED>(a, st); break;
+    case k256x256: launch_tile<256, 256, 2, 4, GATED>(a, st); break;
+  }
 }
 
 }  // namespace
@@ -579,18 +674,16 @@ extern "C" int rxmet_experts_linear_int8(const rxmet_expert_groups *g, int32_t g
   const ExpertArgs a{g->offsets, g->entries, g->tokens, rows, g->top_k, g->experts, grouped != 0,
                      codes, weight, codes_stride, weight_stride, expert_stride, scales, weight_scales,
                      bias, y, N, static_cast<int>(K), gated != 0, activation, dtype};
-  const int64_t few = cdiv(N, gated ? 8 : 16) * g->experts;
+  const int64_t few = cdiv(N, gated ? kFewRows / 2 : kFewRows) * g->experts;
   RXMET_CHECK_ARG(rows < 1 << 26 && few < 1 << 22 &&
                       cdiv(N, gated ? 64 : 128) * (rows / 64 + g->experts) < 1 << 22,
                   "too many outputs for one call");
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_linear_int8", st);
-  if (rows <= 16LL * g->experts)
-    experts_few<<<static_cast<unsigned>(few), 64 * kFewWaves, 0, st>>>(a);
-  else if (a.gated)
-    launch_tiles<true>(a, st);
+  if (a.gated)
+    launch<true>(a, st);
   else
-    launch_tiles<false>(a, st);
+    launch<false>(a, st);
   RXMET_CHECK_LAUNCH();
   return 0;
 }
