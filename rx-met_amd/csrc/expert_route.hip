@@ -17,6 +17,32 @@ namespace rxmet {
 namespace dec {
 namespace {
 
+
+// exp(v) for v in [-700, 700], a value outside taken for the nearest: v = n ln 2 + r, and the series of exp(r),
+// |r| <= ln(2) / 2, up to r^11 (what follows is below 2^-46 of it).  The powers' factors come as
+// scalars: as literals each of them costs two moves where it is used.
+struct Series {
+  double c[10];  // 1 / 2! .. 1 / 11!
+};
+__device__ __forceinline__ double exp_series(double v, const Series &s) {
+  v = fmin(fmax(v, -700.0), 700.0);
+  const double n = __builtin_rint(v * 1.4426950408889634);
+  // ln 2 in two parts, the first of few bits
+  const double r = __builtin_fma(n, -1.9082149292705877e-10, __builtin_fma(n, -0.693147180369123816490, v));
+  double p = s.c[9];
+#pragma unroll
+  for (int i = 8; i >= 0; --i) p = __builtin_fma(p, r, s.c[i]);
+  p = __builtin_fma(__builtin_fma(p, r, 1.0), r, 1.0);
+  return __builtin_ldexp(p, static_cast<int>(n));
+}
+
+// 1 / v for v in [1, 2^1020]: the hardware's estimate and two steps of Newton's rule.
+__device__ __forceinline__ double inverse(double v) {
+  double q = __builtin_amdgcn_rcp(v);
+  q = __builtin_fma(__builtin_fma(-v, q, 1.0), q, q);
+  return __builtin_fma(__builtin_fma(-v, q, 1.0), q, q);
+}
+
 struct RouteArgs {
   rxmet_router r;
   const void *logits;
@@ -26,6 +52,7 @@ struct RouteArgs {
   float *weights;
   const float *d_weights;
   void *d_logits;
+  Series series;
 };
 
 // Sums and maxima over the L lanes of a token, in all of them.
@@ -103,20 +130,23 @@ __device__ __forceinline__ void load_logits(const T *p, int left, float (&x)[V])
 
 constexpr double kNan = __builtin_nan("");
 
-// exp(x - top) of a row's logit, top its largest; rows of -infinity have no scores.
-__device__ __forceinline__ double above(float x, float top) {
-  const double d = x;
-  return top == -INFINITY ? (x != x ? kNan : 0.0) : exp(d - top);
+// exp(x - top) of a row's logit, top its largest and a number; rows of -infinity have no scores.
+__device__ __forceinline__ double above(float x, float top, const Series &s) {
+  return top == -INFINITY ? 0.0 : exp_series(static_cast<double>(x) - top, s);
+}
+__device__ __forceinline__ double sigmoid(float x, const Series &s) {
+  return inverse(1.0 + exp_series(-static_cast<double>(x), s));
 }
 
-// Weight of a chosen logit x over `total` where all weights over the sum of the chosen are asked for:
-// each up to the factor that the sum takes out.  top: the largest chosen logit.
-__device__ __forceinline__ double share(int score, float x, float top) {
-  if (top == -INFINITY) return x != x ? kNan : 0.0;
+// Weight of a chosen logit x where all weights over the sum of the chosen are asked for: each up to the
+// factor that the sum takes out.  top: the largest chosen logit.
+__device__ __forceinline__ double share(int score, float x, float top, const Series &s) {
+  if (x != x) return kNan;
+  if (top == -INFINITY) return 0.0;
   const double d = x, t = top;
-  if (score == RXMET_SCORE_SOFTMAX) return exp(d - t);
+  if (score == RXMET_SCORE_SOFTMAX) return exp_series(d - t, s);
   // 1 / (1 + exp(-x)) = exp(min(x, 0)) / (1 + exp(-|x|)): relative to the largest none underflows
-  return exp((d < 0 ? d : 0.0) - (t < 0 ? t : 0.0)) / (1 + exp(-fabs(d)));
+  return exp_series((d < 0 ? d : 0.0) - (t < 0 ? t : 0.0), s) * inverse(1.0 + exp_series(-fabs(d), s));
 }
 
 template <typename T, int L, int V>
@@ -152,18 +182,18 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
     double s[V], sum = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const double d = x[v];
-      s[v] = softmax ? above(x[v], top) : 1 / (1 + exp(-d));
+      s[v] = softmax ? above(x[v], top, a.series) : sigmoid(x[v], a.series);
       sum += s[v];
     }
     if (softmax) {
       total = over_lanes<L>(sum, [](double p, double q) { return p + q; });
+      const double part = total != 0 ? inverse(total) : 0.0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[v] = total != 0 ? s[v] / total : 0.0;
+      for (int v = 0; v < V; ++v) s[v] *= part;
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      c[v] = static_cast<float>(s[v]);
+      c[v] = bad || x[v] != x[v] ? static_cast<float>(kNan) : static_cast<float>(s[v]);
       if (a.bias && e0 + v < E) c[v] += a.bias[e0 + v];
     }
   } else {
@@ -172,7 +202,7 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
     if (softmax && !a.r.renormalize) {
       double sum = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) sum += above(x[v], top);
+      for (int v = 0; v < V; ++v) sum += above(x[v], top, a.series);
       total = over_lanes<L>(sum, [](double p, double q) { return p + q; });
     }
   }
@@ -184,10 +214,11 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
     __syncthreads();
     for (int g = lane; g < G; g += L) {
       float one = -INFINITY, two = -INFINITY;
+      int at = lane % size;  // lanes start apart, for the banks
+#pragma unroll 4
       for (int i = 0; i < size; ++i) {
-        int at = i + lane;  // lanes start apart, for the banks
-        at = g * size + (at < size ? at : at % size);
-        const float q = s_choice[slot][at];
+        const float q = s_choice[slot][g * size + at];
+        at = at + 1 == size ? 0 : at + 1;
         two = fmaxf(two, fminf(one, q));
         one = fmaxf(one, q);
       }
@@ -222,10 +253,10 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
   for (int j = 0; j < k; ++j) {
     const double best = best_of_lanes<L>(head[0]);
     if (head[0] == best) {
+      s_pick[slot][j] = expert_of(best);
 #pragma unroll
       for (int v = 0; v + 1 < V; ++v) head[v] = head[v + 1];
       head[V - 1] = 1.0;
-      s_pick[slot][j] = expert_of(best);
     }
   }
   __syncthreads();
@@ -234,7 +265,7 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
   first = over_lanes<L>(first, [](float p, float q) { return fmaxf(p, q); });
   if (a.r.renormalize) {
     double sum = 0;
-    for (int j = lane; j < k; j += L) sum += share(a.r.score, s_logit[slot][s_pick[slot][j]], first);
+    for (int j = lane; j < k; j += L) sum += share(a.r.score, s_logit[slot][s_pick[slot][j]], first, a.series);
     total = over_lanes<L>(sum, [](double p, double q) { return p + q; });
   }
   if (wanted >= a.tokens) return;
@@ -243,17 +274,17 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
     const float l = s_logit[slot][e];
     double w;
     if (a.r.renormalize)
-      w = total == 0 ? 0.0 : share(a.r.score, l, first) / total;
+      w = total == 0 ? 0.0 : share(a.r.score, l, first, a.series) / total;
     else if (softmax)
-      w = total != 0 ? above(l, top) / total : 0.0;
+      w = total != 0 ? above(l, top, a.series) / total : 0.0;
     else
-      w = 1 / (1 + exp(-static_cast<double>(l)));
+      w = l != l ? kNan : sigmoid(l, a.series);
     a.experts[t * k + j] = e;
     a.weights[t * k + j] = static_cast<float>(bad ? kNan : w * a.r.scale);
   }
 }
 
-// One token of L lanes: the chosen experts' parts in 64 bits, the others' (softmax as it is) in fp32.
+// The chosen experts' parts in 64 bits; where all logits have one (softmax as it is) the row in fp32.
 template <typename T, int L, int V>
 __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
   constexpr int per = kWave / L, most = L * V;
@@ -266,89 +297,132 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
   const int e0 = lane * V;
   float x[V];
   load_logits(static_cast<const T *>(a.logits) + t * a.stride + e0, E - e0, x);
-  float top = -INFINITY;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     s_logit[slot][e0 + v] = x[v];
     s_grad[slot][e0 + v] = 0;
-    top = fmaxf(top, x[v]);
   }
   const int32_t *experts = a.experts + t * k;
   const float *dw = a.d_weights + t * k;
-  const double scale = a.r.scale;
   __syncthreads();
   auto expert = [&](int j) {
     const int e = experts[j];
     return e >= 0 && e < E ? e : -1;
   };
-  auto plus = [](double p, double q) { return p + q; };
+  auto most_of = [](float p, float q) { return fmaxf(p, q); };
   const bool dense = softmax && !a.r.renormalize;
-  double total = 0, inner = 0;
+  float p[V], inner = 0;
   if (dense) {
-    top = over_lanes<L>(top, [](float p, float q) { return fmaxf(p, q); });
+    float top = -INFINITY, total = 0;
+    bool bad = false;
 #pragma unroll
-    for (int v = 0; v < V; ++v) total += above(x[v], top);
-    total = over_lanes<L>(total, plus);
+    for (int v = 0; v < V; ++v) {
+      top = fmaxf(top, x[v]);
+      bad |= !(x[v] < INFINITY);
+    }
+    top = over_lanes<L>(top, most_of);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      p[v] = bad ? static_cast<float>(kNan) : top == -INFINITY ? 0.0f : expf(x[v] - top);
+      total += p[v];
+    }
+    total = over_lanes<L>(total, [](float p, float q) { return p + q; });
+    const float part = total != 0 ? 1.0f / total : 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] *= part;
     for (int j = lane; j < k; j += L) {
       const int e = expert(j);
       if (e < 0) continue;
-      if (total != 0) inner += dw[j] * above(s_logit[slot][e], top) / total;
+      const float l = s_logit[slot][e];
+      inner += dw[j] * (total != total ? total : top == -INFINITY ? 0.0f : expf(l - top) * part);
       s_grad[slot][e] = dw[j];
     }
-  } else if (a.r.renormalize) {
-    top = -INFINITY;
-    for (int j = lane; j < k; j += L)
-      if (expert(j) >= 0) top = fmaxf(top, s_logit[slot][expert(j)]);
-    top = over_lanes<L>(top, [](float p, float q) { return fmaxf(p, q); });
-    for (int j = lane; j < k; j += L)
-      if (expert(j) >= 0) total += share(a.r.score, s_logit[slot][expert(j)], top);
-    total = over_lanes<L>(total, plus);
-    for (int j = lane; j < k; j += L)
-      if (expert(j) >= 0 && total != 0) inner += dw[j] * share(a.r.score, s_logit[slot][expert(j)], top) / total;
-  }
-  inner = over_lanes<L>(inner, plus);
-  if (!dense)
+    inner = over_lanes<L>(inner, [](float p, float q) { return p + q; });
+  } else {
+    auto plus = [](double p, double q) { return p + q; };
+    float top = -INFINITY;
+    double total = 0, mean = 0;
+    if (a.r.renormalize) {
+      for (int j = lane; j < k; j += L)
+        if (expert(j) >= 0) top = fmaxf(top, s_logit[slot][expert(j)]);
+      top = over_lanes<L>(top, most_of);
+      for (int j = lane; j < k; j += L)
+        if (expert(j) >= 0) {
+          const double s = share(a.r.score, s_logit[slot][expert(j)], top, a.series);
+          total += s;
+          mean += s * dw[j];
+        }
+      total = over_lanes<L>(total, plus);
+      mean = over_lanes<L>(mean, plus);
+      if (total != 0) mean /= total;
+    }
     for (int j = lane; j < k; j += L) {
       const int e = expert(j);
       if (e < 0) continue;
-      const double l = s_logit[slot][e], s = 1 / (1 + exp(-l));
-      double g;
-      if (a.r.renormalize) {
-        g = total != 0 ? share(a.r.score, s_logit[slot][e], top) / total * (dw[j] - inner) : 0.0;
-        if (!softmax) g /= 1 + exp(l);
-      } else {
-        g = dw[j] * s / (1 + exp(l));
-      }
-      s_grad[slot][e] = static_cast<float>(g * scale);
+      const float l = s_logit[slot][e];
+      const double rest = l != l ? kNan : sigmoid(-l, a.series);  // 1 - sigmoid(l)
+      double g = 0;
+      if (!a.r.renormalize)
+        g = dw[j] * sigmoid(l, a.series) * rest;
+      else if (total != 0)
+        g = share(a.r.score, l, top, a.series) / total * (dw[j] - mean) * (softmax ? 1.0 : rest);
+      s_grad[slot][e] = static_cast<float>(g * a.r.scale);
     }
+  }
   __syncthreads();
   if (wanted >= a.tokens) return;
   T *out = static_cast<T *>(a.d_logits) + t * E + e0;
+  float g[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    if (e0 + v >= E) break;
-    float g = s_grad[slot][e0 + v];
-    if (dense)
-      g = static_cast<float>(
-          (total != 0 ? above(x[v], top) / total : 0.0) * (g - inner) * scale);
-    out[v] = static_cast<T>(g);
+    g[v] = s_grad[slot][e0 + v];
+    if (dense) g[v] = p[v] * (g[v] - inner) * a.r.scale;
+  }
+  if (e0 + V <= E) {
+    T u[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) u[v] = static_cast<T>(g[v]);
+    __builtin_memcpy(out, u, sizeof(u));
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (e0 + v < E) out[v] = static_cast<T>(g[v]);
   }
 }
 
-// Lanes and experts of a lane by the number of experts.
-template <typename T, typename F>
-void by_experts(int E, F &&f) {
+// Lanes of a token and experts of a lane.  Few lanes with many experts each spend least on a token, for
+// the maxima over lanes are taken for 64 / L tokens at once ([16384, 256] with groups: 16 lanes 22 us, 64 lanes
+// 38); where tokens are few, a whole wave for each is done sooner ([16, 256]: 7.7 us and 11.1).
+template <typename F>
+void by_experts(int64_t tokens, int E, F &&f) {
   using std::integral_constant;
-  if (E <= 64)
-    f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  auto as = [&](auto L, auto V) { f(L, V); };
+  constexpr integral_constant<int, 64> whole{};
+  if (tokens <= 1024 && E <= 64)
+    as(whole, integral_constant<int, 1>{});
+  else if (tokens <= 1024 && E <= 128)
+    as(whole, integral_constant<int, 2>{});
+  else if (tokens <= 1024 && E <= 256)
+    as(whole, integral_constant<int, 4>{});
+  else if (tokens <= 1024 && E <= 512)
+    as(whole, integral_constant<int, 8>{});
+  else if (E <= 64)
+    as(integral_constant<int, 16>{}, integral_constant<int, 4>{});
   else if (E <= 128)
-    f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    as(integral_constant<int, 16>{}, integral_constant<int, 8>{});
   else if (E <= 256)
-    f(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+    as(integral_constant<int, 16>{}, integral_constant<int, 16>{});
   else if (E <= 512)
-    f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    as(integral_constant<int, 32>{}, integral_constant<int, 16>{});
   else
-    f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    as(whole, integral_constant<int, 16>{});
+}
+
+Series series() {
+  Series s;
+  double f = 1;
+  for (int i = 0; i < 10; ++i) s.c[i] = 1 / (f *= i + 2);
+  return s;
 }
 
 int check_router(const rxmet_router *r, int64_t stride, int64_t tokens, int32_t dtype) {
@@ -384,10 +458,10 @@ extern "C" int rxmet_route_forward(const rxmet_router *r, const void *logits, in
   RXMET_CHECK_ARG(logits && experts && weights, "logits, experts and weights are needed");
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("route_forward", st);
-  const RouteArgs a{*r, logits, stride, tokens, bias, experts, weights, nullptr, nullptr};
+  const RouteArgs a{*r, logits, stride, tokens, bias, experts, weights, nullptr, nullptr, series()};
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    by_experts<T>(r->experts, [&](auto L, auto V) {
+    by_experts(tokens, r->experts, [&](auto L, auto V) {
       route_forward<T, L.value, V.value><<<static_cast<unsigned>(cdiv(tokens, kWave / L.value)), kWave, 0, st>>>(a);
     });
   });
@@ -405,10 +479,10 @@ extern "C" int rxmet_route_backward(const rxmet_router *r, const void *logits, i
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("route_backward", st);
   const RouteArgs a{*r, logits, stride, tokens, nullptr, const_cast<int32_t *>(experts), nullptr,
-                    d_weights, d_logits};
+                    d_weights, d_logits, series()};
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    by_experts<T>(r->experts, [&](auto L, auto V) {
+    by_experts(tokens, r->experts, [&](auto L, auto V) {
       route_backward<T, L.value, V.value><<<static_cast<unsigned>(cdiv(tokens, kWave / L.value)), kWave, 0, st>>>(a);
     });
   });

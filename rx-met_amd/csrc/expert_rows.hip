@@ -55,8 +55,9 @@ __global__ __launch_bounds__(kChunk) void group_place(const GroupArgs a) {
     if (tid < columns * share)
       for (int b = tid % columns; b < bins; b += columns) {
         int all = 0, mine = 0;
+#pragma unroll 8
         for (int c = tid / columns; c < a.chunks; c += share) {
-          const int n = a.counts[static_cast<int64_t>(c) * bins + b];
+          const int n = a.counts[c * bins + b];
           all += n;
           mine += c < static_cast<int>(blockIdx.x) ? n : 0;
         }
@@ -105,10 +106,13 @@ __global__ __launch_bounds__(kChunk) void group_place(const GroupArgs a) {
     __syncthreads();
     for (int b = tid; b < bins; b += kChunk) {  // counts of the waves before; the bin moves on
       int n = 0;
+      int c[kGroupWaves];
+#pragma unroll
+      for (int v = 0; v < kGroupWaves; ++v) c[v] = s_wave[v][b];
+#pragma unroll
       for (int v = 0; v < kGroupWaves; ++v) {
-        const int c = s_wave[v][b];
         s_wave[v][b] = static_cast<unsigned short>(n);
-        n += c;
+        n += c[v];
       }
       s_all[b] = s_at[b];
       s_at[b] += n;
@@ -183,32 +187,34 @@ __global__ __launch_bounds__(256) void combine_rows(const CombineArgs a) {
   }
 }
 
-// The gradient: a workgroup has a token, reads its gradient once for up to kTogether of its rows,
-// writes theirs and adds up their products with y.  Rows of no expert are cleared by all workgroups.
-constexpr int kTogether = 4;
-
-template <typename T>
+// The gradient: the threads of a token read its gradient once for up to TOGETHER of its rows, write theirs
+// and add up their products with y.  Rows of no expert are cleared by all.  Bound: the rows' bytes, read
+// and written.
+template <typename T, int TOGETHER>
 __global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
-  __shared__ float s_dot[4][kTogether];
-  const int64_t t = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  __shared__ float s_dot[4][TOGETHER];
+  const int width = 1 << a.shift, at = threadIdx.x & (width - 1), wave = threadIdx.x / kWave;
+  const int64_t wanted = static_cast<int64_t>(blockIdx.x) * (256 >> a.shift) + (threadIdx.x >> a.shift);
+  const int64_t t = wanted < a.tokens ? wanted : a.tokens - 1;  // (all threads meet below)
   const int32_t *place = a.places + t * a.top_k;
-  for (int j0 = 0; j0 < a.top_k; j0 += kTogether) {
-    int64_t p[kTogether];
-    float w[kTogether], dot[kTogether];
+  // written past the caches only where rows start on 16 bytes ([65536, 2041]: 273 us so, 257 otherwise)
+  const bool whole = (a.N * sizeof(T) | reinterpret_cast<uintptr_t>(a.d_y)) % 16 == 0;
+  for (int j0 = 0; j0 < a.top_k; j0 += TOGETHER) {
+    int64_t p[TOGETHER];
+    float w[TOGETHER], dot[TOGETHER];
 #pragma unroll
-    for (int j = 0; j < kTogether; ++j) {
-      p[j] = j0 + j < a.top_k ? place[j0 + j] : -1;
+    for (int j = 0; j < TOGETHER; ++j) {
+      p[j] = j0 + j < a.top_k && wanted < a.tokens ? place[j0 + j] : -1;
       if (p[j] >= a.rows) p[j] = -1;
       w[j] = j0 + j < a.top_k ? a.weights[t * a.top_k + j0 + j] : 0.0f;
       dot[j] = 0;
     }
-    for (int64_t n = 8 * tid; n < a.N; n += 8 * 256) {
+    for (int64_t n = 8 * at; n < a.N; n += 8 * width) {
       const int64_t left = a.N - n;
       float g[8];
       load_any(static_cast<const T *>(a.d_out) + t * a.d_stride + n, left, g);
 #pragma unroll
-      for (int j = 0; j < kTogether; ++j) {
+      for (int j = 0; j < TOGETHER; ++j) {
         if (p[j] < 0) continue;
         if (a.d_weights) {
           float v[8];
@@ -220,29 +226,50 @@ __global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
           float d[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) d[e] = w[j] * g[e];
-          store_any(static_cast<T *>(a.d_y) + p[j] * a.N + n, left, d);
+          T *out = static_cast<T *>(a.d_y) + p[j] * a.N + n;
+          if (left < 8)
+            store8_part(out, static_cast<int>(left), d);
+          else if (whole)
+            stream_out8(out, d);
+          else
+            store8(out, d);
         }
       }
     }
-    if (a.d_weights) {
+    if (!a.d_weights) continue;
 #pragma unroll
-      for (int j = 0; j < kTogether; ++j) {
+    for (int j = 0; j < TOGETHER; ++j)
+      for (int d = (width < kWave ? width : kWave) / 2; d > 0; d >>= 1) dot[j] += __shfl_xor(dot[j], d, kWave);
+    if (width > kWave) {  // a token's waves
+      __syncthreads();
+      if (threadIdx.x % kWave == 0)
 #pragma unroll
-        for (int d = kWave / 2; d > 0; d >>= 1) dot[j] += __shfl_xor(dot[j], d, kWave);
-        if (lane == 0) s_dot[wave][j] = dot[j];
+        for (int j = 0; j < TOGETHER; ++j) s_dot[wave][j] = dot[j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < TOGETHER; ++j) {
+        dot[j] = 0;
+        for (int v = wave & ~(width / kWave - 1), n = 0; n < width / kWave; ++n) dot[j] += s_dot[v + n][j];
       }
-      __syncthreads();
-      if (tid < kTogether && j0 + tid < a.top_k)
-        a.d_weights[t * a.top_k + j0 + tid] = s_dot[0][tid] + s_dot[1][tid] + s_dot[2][tid] + s_dot[3][tid];
-      __syncthreads();
     }
+    if (at == 0 && wanted < a.tokens)
+#pragma unroll
+      for (int j = 0; j < TOGETHER; ++j)
+        if (j0 + j < a.top_k) a.d_weights[t * a.top_k + j0 + j] = dot[j];
   }
-  if (!a.d_y) return;
+  if (!a.d_y || wanted >= a.tokens) return;
   const int64_t held = a.offsets[a.experts];
   const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   for (int64_t i = (held < 0 ? 0 : held) + t; i < a.rows; i += a.tokens)
-    for (int64_t n = 8 * tid; n < a.N; n += 8 * 256)
+    for (int64_t n = 8 * at; n < a.N; n += 8 * width)
       store_any(static_cast<T *>(a.d_y) + i * a.N + n, a.N - n, zero);
+}
+
+// Threads of a row, as a power of two: eight columns each, at most `most`.
+int shift_for(int64_t N, int most) {
+  int shift = 0;
+  while (shift < most && (8LL << shift) < N) ++shift;
+  return shift;
 }
 
 int check_groups(const rxmet_expert_groups *g, int64_t N, int32_t dtype) {
@@ -298,8 +325,7 @@ extern "C" int rxmet_experts_combine(const rxmet_expert_groups *g, const void *y
   if (const int rc = check_groups(g, N, dtype)) return rc;
   if (g->tokens == 0) return 0;
   RXMET_CHECK_ARG(g->places && y && weights && out, "places, y, weights and out are needed");
-  int shift = 0;
-  while (shift < 8 && (8LL << shift) < N) ++shift;
+  const int shift = shift_for(N, 8);
   const CombineArgs a{g->offsets, g->places, g->tokens, g->tokens * g->top_k, g->top_k, g->experts, y,
                       residual, nullptr, y_stride, residual_stride, 0, weights, out, nullptr, nullptr, N, shift};
   auto st = static_cast<hipStream_t>(stream);
@@ -320,12 +346,22 @@ extern "C" int rxmet_experts_combine_backward(const rxmet_expert_groups *g, cons
   RXMET_CHECK_ARG(g->places && d_out && weights, "places, d_out and weights are needed");
   RXMET_CHECK_ARG(!d_y || g->offsets, "d_y needs the groups' offsets");
   RXMET_CHECK_ARG(!d_weights || y, "d_weights needs y");
+  // a wave has a token, so that its sums over N meet without a barrier ([8192, 2041] x 8: 225 us, a workgroup
+  // 271); a workgroup where tokens are few ([2048, 8192] x 8: 167 us, a wave 217)
+  const int shift = shift_for(N, g->tokens >= 4096 ? 6 : 8);
   const CombineArgs a{g->offsets, g->places, g->tokens, g->tokens * g->top_k, g->top_k, g->experts, y,
-                      nullptr, d_out, y_stride, 0, d_out_stride, weights, nullptr, d_y, d_weights, N, 0};
+                      nullptr, d_out, y_stride, 0, d_out_stride, weights, nullptr, d_y, d_weights, N, shift};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_combine_backward", st);
   with_type(dtype, [&](auto t) {
-    combine_backward<decltype(t)><<<static_cast<unsigned>(g->tokens), 256, 0, st>>>(a);
+    using T = decltype(t);
+    const unsigned grid = static_cast<unsigned>(cdiv(g->tokens, 256 >> shift));
+    if (g->top_k <= 2)
+      combine_backward<T, 2><<<grid, 256, 0, st>>>(a);
+    else if (g->top_k <= 4)
+      combine_backward<T, 4><<<grid, 256, 0, st>>>(a);
+    else
+      combine_backward<T, 8><<<grid, 256, 0, st>>>(a);
   });
   RXMET_CHECK_LAUNCH();
   return 0;
