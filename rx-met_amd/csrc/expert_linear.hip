@@ -42,6 +42,17 @@ __device__ __forceinline__ int64_t row_of(const ExpertArgs &a, int64_t i) {
   return t < 0 ? 0 : t < a.tokens ? t : a.tokens - 1;
 }
 
+// silu by the hardware's exponential and reciprocal (each within a step of fp32): 5 instructions instead of 25, in
+// both kernels, so that a row's result does not go by how many there are.
+__device__ __forceinline__ float quick_activate(float v, int act) {
+  if (act != RXMET_ACT_SILU) return activate(v, act);
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
+}
+
+// f of a weight row and of a row of codes
+__device__ __forceinline__ int wide_turn_w(int row) { return (row >> 1 & 3) | (row >> 2 & 4); }
+__device__ __forceinline__ int wide_turn_x(int row) { return row >> 1 & 7; }
+
 // Finishes and writes C consecutive n of place i; v: the sums of the values where gated.
 template <typename T, int C>
 __device__ __forceinline__ void finish(const ExpertArgs &a, int e, int64_t i, float sx, int64_t n0,
@@ -69,7 +80,7 @@ __device__ __forceinline__ void finish(const ExpertArgs &a, int e, int64_t i, fl
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      float v = activate(scaled(acc[c], w[c], b.v[c]), a.act);
+      float v = quick_activate(scaled(acc[c], w[c], b.v[c]), a.act);
       if (a.gated) v *= scaled(val[c], wv[c], bv.v[c]);
       out.v[c] = static_cast<T>(v);
     }
@@ -78,7 +89,7 @@ __device__ __forceinline__ void finish(const ExpertArgs &a, int e, int64_t i, fl
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (n0 + c < a.N) {
-        float v = activate(scaled(acc[c], sw[c], bias ? bias[c] : static_cast<T>(0.0f)), a.act);
+        float v = quick_activate(scaled(acc[c], sw[c], bias ? bias[c] : static_cast<T>(0.0f)), a.act);
         if (a.gated) v *= scaled(val[c], sw[a.N + c], bias ? bias[a.N + c] : static_cast<T>(0.0f));
         y[c] = static_cast<T>(v);
       }
@@ -235,16 +246,6 @@ __global__ __launch_bounds__(64 * WK) void experts_few(const ExpertArgs a) {
 // 16 different bank groups.  Row i of a wave's 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) +
 // i % 4: a lane holds 16 consecutive n of one place.  Rows that do not start on 16 bytes (ALIGNED
 // false) go through registers.  Scales and bias wait in LDS for the end.
-// silu by the hardware's exponential and reciprocal (each within a step of fp32): 5 instructions instead of 25.
-__device__ __forceinline__ float quick_activate(float v, int act) {
-  if (act != RXMET_ACT_SILU) return activate(v, act);
-  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f));
-}
-
-// f of a weight row and of a row of codes
-__device__ __forceinline__ int wide_turn_w(int row) { return (row >> 1 & 3) | (row >> 2 & 4); }
-__device__ __forceinline__ int wide_turn_x(int row) { return row >> 1 & 7; }
-
 template <int TN, int TM, int WN, int WM, bool GATED, bool ALIGNED>
 __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 64 ? 2 : 3) void experts_tile(const ExpertArgs a) {
   constexpr int threads = 64 * WN * WM;
