@@ -311,15 +311,16 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
   };
   auto most_of = [](float p, float q) { return fmaxf(p, q); };
   const bool dense = softmax && !a.r.renormalize;
-  float p[V], inner = 0;
-  if (dense) {
-    float top = -INFINITY, total = 0;
-    bool bad = false;
+  float p[V], inner = 0, top = -INFINITY;
+  bool bad = false;  // as in the forward pass: the weights are NaN, and so are their gradients
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      top = fmaxf(top, x[v]);
-      bad |= !(x[v] < INFINITY);
-    }
+  for (int v = 0; v < V; ++v) {
+    top = fmaxf(top, x[v]);
+    bad |= softmax && !(x[v] < INFINITY);
+  }
+  bad = over_lanes<L>(static_cast<int>(bad), [](int p, int q) { return p | q; });
+  if (dense) {
+    float total = 0;
     top = over_lanes<L>(top, most_of);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
     inner = over_lanes<L>(inner, [](float p, float q) { return p + q; });
   } else {
     auto plus = [](double p, double q) { return p + q; };
-    float top = -INFINITY;
+    top = -INFINITY;
     double total = 0, mean = 0;
     if (a.r.renormalize) {
       for (int j = lane; j < k; j += L)
@@ -366,7 +367,7 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
         g = dw[j] * sigmoid(l, a.series) * rest;
       else if (total != 0)
         g = share(a.r.score, l, top, a.series) / total * (dw[j] - mean) * (softmax ? 1.0 : rest);
-      s_grad[slot][e] = static_cast<float>(g * a.r.scale);
+      s_grad[slot][e] = static_cast<float>(bad ? kNan : g * a.r.scale);
     }
   }
   __syncthreads();

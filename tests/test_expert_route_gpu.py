@@ -141,6 +141,24 @@ def test_masked_logits_have_gradients_that_are_numbers(cuda, score, renormalize)
     np.testing.assert_allclose(f64(dx), want, rtol=1e-6, atol=16 * 15 * 2.0 ** -24)
 
 
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_softmax_rows_without_weights_have_no_gradient(cuda, renormalize):
+    """A NaN or +infinity anywhere in a softmax row makes its weights NaN, and their gradients: of all its
+    logits, or of the chosen ones where the weights go by those alone."""
+    x = logits(5, 20, 11, cuda)
+    x[0, 4], x[1, 7], x[2, 3:] = torch.nan, torch.inf, torch.nan
+    x.requires_grad_()
+    e, w = ops.route_experts(x, 3, renormalize=renormalize)
+    (dx,) = torch.autograd.grad(w, x, torch.ones_like(w))
+    assert w[:3].isnan().all() and not w[3:].isnan().any() and not dx[3:].isnan().any()
+    picked = dx[:3].gather(1, e[:3].long())
+    assert picked.isnan().all()
+    if renormalize:
+        assert int(dx[:3].isnan().sum()) == 9 and int((dx[:3] == 0).sum()) == 51
+    else:
+        assert dx[:3].isnan().all()
+
+
 def test_strides_leading_axes_and_no_tokens(cuda):
     big = logits(24, 50, 9, cuda)
     x = big[:, 5:37]
