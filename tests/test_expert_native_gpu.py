@@ -146,3 +146,34 @@ def test_saved_tensors_may_be_packed_elsewhere(cuda):
     with torch.autograd.graph.save_on_cpu():
         got = run()[1]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_programs(cuda, backend):
+    """Operators between the graphs of a compiled program give what they give without it."""
+    ids, g = sample(cuda)
+    x = torch.randn(50, 8, device=cuda, requires_grad=True)
+    y = torch.randn(150, 32, device=cuda, requires_grad=True)
+
+    def train(x, y):
+        e, w = ops.route_experts(x * 2, 3, renormalize=False)
+        return (ops.experts_combine(y * 2, w, ops.group_experts(e, 8)) ** 2).sum()
+
+    torch._dynamo.reset()
+    got, want = torch.compile(train, backend=backend)(x, y), train(x, y)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, (x, y)), torch.autograd.grad(want, (x, y))):
+        assert torch.equal(a, b)
+    torch._dynamo.reset()
+
+
+def test_transforms_are_refused(cuda):
+    _, g = sample(cuda)
+    y, w = torch.randn(150, 32, device=cuda), torch.rand(50, 3, device=cuda)
+    x = torch.randn(50, 8, device=cuda)
+    for f, v in ((lambda v: ops.route_experts(v, 3)[1].sum(), x),
+                 (lambda v: ops.experts_combine(v, w, g).sum(), y),
+                 (lambda v: ops.experts_combine(y, w * v.sum(), g).sum(), x)):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(f)(v)
