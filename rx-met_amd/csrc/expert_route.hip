@@ -191,10 +191,12 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
 #pragma unroll
       for (int v = 0; v < V; ++v) s[v] *= part;
     }
+    float b[V];
+    if (a.bias) load_logits(a.bias + e0, E - e0, b);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       c[v] = bad || x[v] != x[v] ? static_cast<float>(kNan) : static_cast<float>(s[v]);
-      if (a.bias && e0 + v < E) c[v] += a.bias[e0 + v];
+      if (a.bias) c[v] += b[v];
     }
   } else {
 #pragma unroll
