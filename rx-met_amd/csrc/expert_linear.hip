@@ -6,6 +6,14 @@
 //
 // The experts' rows are known on the device alone: a launch is sized for the most tiles that the entries
 // can need, and each workgroup finds its tile in the offsets.
+//
+// Bound and measured.  Few rows: the weights' bytes (16 tokens of 8 of 64 experts, gated [2048, 2048]: 268 MB
+// of which 56 experts' are read, 46 us warm, 5.1 TB/s; 57 with other inputs in between).  Many: [65536, 2048] of 32
+// experts' [2048, 2048] 327 us warm, 1.68 POP/s, gated [4096, 2048] 628 us, 1.75 POP/s; the matrix unit is
+// busy for 35 to 39 % of that.  Over K alone (2048 to 4096) the loop runs at 2.0 POP/s, where the library's
+// product of 8192^3 without an epilogue reaches 2.1: without its loads it would at 2.9, and they are 64 KB a step and
+// CU on their way while one step is multiplied, which LDS has no room to do further ahead.  The rest is
+// the tiles' start and end, when the outputs' bytes (268 MB) are written with little to multiply.
 #include <type_traits>
 
 #include "../../include/rxmet_experts.h"
@@ -241,7 +249,8 @@ __global__ __launch_bounds__(64 * WK) void experts_few(const ExpertArgs a) {
 // Where gated, a wave's weight rows are gates in their first half and the same columns' values in the
 // second, so that a lane holds both.
 //
-// K goes through LDS in steps of 128 bytes, memory -> LDS without registers, one step ahead.  A row's
+// K goes through LDS in steps of 128 bytes, whole lines of memory (of 64 bytes: 306 us for each 2048 of K
+// against 260), memory -> LDS without registers, one step ahead.  A row's
 // eight 16-byte pieces lie at the places piece ^ f(row), so that 16 lanes that read one piece of 16 rows meet
 // 16 different bank groups.  Row i of a wave's 32 weight rows stands for n = 16 * (i / 4 % 2) + 4 * (i / 8) +
 // i % 4: a lane holds 16 consecutive n of one place.  Rows that do not start on 16 bytes (ALIGNED

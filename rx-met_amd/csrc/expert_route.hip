@@ -10,6 +10,10 @@
 // one double in [1, 2) whose 52 bits hold the ordered bits of c_e and, below them, 1023 - e: one maximum
 // compares both, and ties go to the lowest index.  Lanes sort theirs, then the best of the lanes'
 // heads is taken k times.
+//
+// Bound: instructions, half of them for the scores and the sort ([16384, 256] fp32, bias, 8 groups, k = 8:
+// 21 us, 17 MB; without groups 17, without bias and groups 11).  A few tokens: one wave's way through all
+// steps (7.4 us).  Backward ([16384, 128] bf16, softmax as it is): 5.5 us.
 #include "../../include/rxmet_experts.h"
 #include "decoder_common.h"
 

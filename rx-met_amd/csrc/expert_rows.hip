@@ -10,6 +10,8 @@ namespace {
 // Order by expert: a counting sort that keeps the entries' order.  A workgroup has kChunk entries; its
 // counts go to memory, and a second launch adds up the counts of the chunks before, ranks the entries of
 // its chunk and writes both directions.  Up to kAlone entries one workgroup does it all in one launch.
+// Bound: launches and trips to memory behind each other ([16384, 8] of 256 experts: 11 us, 1.5 + 9 of kernels, 1.6
+// MB; [16, 8]: 3.6 us of kernel).
 struct GroupArgs {
   const int32_t *experts;
   int64_t count;
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(256) void combine_rows(const CombineArgs a) {
 
 // The gradient: the threads of a token read its gradient once for up to TOGETHER of its rows, write theirs
 // and add up their products with y.  Rows of no expert are cleared by all.  Bound: the rows' bytes, read
-// and written.
+// and written ([65536, 2041] bf16, a tenth of no expert: 128 us, 541 MB, 4.2 TB/s).
 template <typename T, int TOGETHER>
 __global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
   __shared__ float s_dot[4][TOGETHER];
