@@ -71,7 +71,7 @@ int rxmet_route_backward(const rxmet_router *router, const void *logits, int64_t
  *   offsets  [num_experts + 1] out: expert e's places are offsets[e]..offsets[e + 1]
  *   entries  [count] out: the entry of each place; behind offsets[num_experts] stand those of no expert
  *   places   [count] out: the place of each entry, -1 for those of no expert
- * The workspace may be NULL where its size is 0.
+ * The workspace (aligned to 4 bytes) may be NULL where its size is 0.
  */
 int64_t rxmet_group_experts_workspace_bytes(int64_t count, int32_t num_experts);
 int rxmet_group_experts(const int32_t *experts, int64_t count, int32_t num_experts,

@@ -9,19 +9,21 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // Order by expert: a counting sort that keeps the entries' order.  A workgroup has kChunk entries; its
 // counts go to memory, and a second launch adds up the counts of the chunks before, ranks the entries of
-// its chunk and writes both directions.  Up to kAlone entries one workgroup does it all in one launch.
-// Bound: launches and trips to memory behind each other ([16384, 8] of 256 experts: 11 us, 1.5 + 9 of kernels, 1.6
-// MB; [16, 8]: 3.6 us of kernel).
+// its chunk and writes both directions.  Up to kAlone entries one workgroup does it all in one launch;
+// above kFewChunks chunks, whose counts every chunk would read, a launch in between adds them up once.
+// Bound: launches and trips to memory behind each other ([16384, 8] of 256 experts: 11 us, 2.4 + 9.2 of kernels,
+// 1.6 MB; [16, 8]: 3.6 us of kernel; 2^26 entries 1.8 ms).
 struct GroupArgs {
   const int32_t *experts;
   int64_t count;
   int E, chunks;
   int32_t *offsets, *entries, *places;
-  int32_t *counts;  // [chunks, E + 1]
+  int32_t *counts;  // [chunks + 1, E + 1]; added up: of the chunks before, and of all in the last row
 };
 
 constexpr int kChunk = 1024, kGroupWaves = kChunk / kWave;
 constexpr int64_t kAlone = 4096;
+constexpr int64_t kFewChunks = 128;
 constexpr int kBins = RXMET_EXPERTS_MAX + 1;  // the last one: entries of no expert
 
 __device__ __forceinline__ int bin_of(const GroupArgs &a, int64_t i) {
@@ -40,8 +42,32 @@ __global__ __launch_bounds__(kChunk) void group_count(const GroupArgs a) {
     a.counts[static_cast<int64_t>(blockIdx.x) * (a.E + 1) + b] = s_count[b];
 }
 
-// ALONE: one workgroup has all entries and counts them first.
-template <bool ALONE>
+// The counts of each bin's chunks before every chunk: 64 bins a workgroup, 16 threads a bin, each with
+// a run of the chunks.
+__global__ __launch_bounds__(1024) void group_sum(const GroupArgs a) {
+  __shared__ int s_run[16][64];
+  const int bins = a.E + 1, b = blockIdx.x * 64 + threadIdx.x % 64, r = threadIdx.x / 64;
+  const int share = (a.chunks + 15) / 16, from = r * share, to = from + share < a.chunks ? from + share : a.chunks;
+  int n = 0;
+  if (b < bins)
+#pragma unroll 8
+    for (int c = from; c < to; ++c) n += a.counts[c * bins + b];
+  s_run[r][threadIdx.x % 64] = n;
+  __syncthreads();
+  int before = 0;
+  for (int v = 0; v < r; ++v) before += s_run[v][threadIdx.x % 64];
+  if (b >= bins) return;
+#pragma unroll 8
+  for (int c = from; c < to; ++c) {
+    const int m = a.counts[c * bins + b];
+    a.counts[c * bins + b] = before;
+    before += m;
+  }
+  if (r == 15) a.counts[a.chunks * bins + b] = before;
+}
+
+// ALONE: one workgroup has all entries and counts them first.  SUMMED: the chunks' counts are added up.
+template <bool ALONE, bool SUMMED>
 __global__ __launch_bounds__(kChunk) void group_place(const GroupArgs a) {
   __shared__ int s_all[kBins], s_at[kBins];  // entries of a bin; where its next one goes
   __shared__ unsigned short s_wave[kGroupWaves][kBins];
@@ -51,6 +77,11 @@ __global__ __launch_bounds__(kChunk) void group_place(const GroupArgs a) {
   __syncthreads();
   if (ALONE) {
     for (int64_t i = tid; i < a.count; i += kChunk) atomicAdd(&s_all[bin_of(a, i)], 1);
+  } else if (SUMMED) {
+    for (int b = tid; b < bins; b += kChunk) {
+      s_all[b] = a.counts[a.chunks * bins + b];
+      s_at[b] = a.counts[static_cast<int>(blockIdx.x) * bins + b];
+    }
   } else {
     // each bin's column of counts by as many threads as there are
     const int columns = bins < kChunk ? bins : kChunk, share = kChunk / columns;
@@ -311,7 +342,7 @@ using namespace rxmet::dec;
 
 extern "C" int64_t rxmet_group_experts_workspace_bytes(int64_t count, int32_t num_experts) {
   if (count <= kAlone || num_experts < 1) return 0;
-  return cdiv(count, kChunk) * (num_experts + 1) * 4;
+  return (cdiv(count, kChunk) + 1) * (num_experts + 1) * 4;
 }
 
 extern "C" int rxmet_group_experts(const int32_t *experts, int64_t count, int32_t num_experts,
@@ -322,16 +353,22 @@ extern "C" int rxmet_group_experts(const int32_t *experts, int64_t count, int32_
   RXMET_CHECK_ARG(offsets != nullptr, "offsets are needed");
   RXMET_CHECK_ARG(count == 0 || (experts && entries && places), "experts, entries and places are needed");
   RXMET_CHECK_ARG(count <= kAlone || workspace, "this call needs a workspace");
+  RXMET_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "the workspace must be aligned to 4 bytes");
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("group_experts", st);
   const int chunks = static_cast<int>(cdiv(count, kChunk));
   const GroupArgs a{experts, count, num_experts, chunks, offsets, entries, places,
                     static_cast<int32_t *>(workspace)};
   if (count <= kAlone) {
-    group_place<true><<<1, kChunk, 0, st>>>(a);
+    group_place<true, false><<<1, kChunk, 0, st>>>(a);
   } else {
     group_count<<<chunks, kChunk, 0, st>>>(a);
-    group_place<false><<<chunks, kChunk, 0, st>>>(a);
+    if (chunks <= kFewChunks) {
+      group_place<false, false><<<chunks, kChunk, 0, st>>>(a);
+    } else {
+      group_sum<<<static_cast<unsigned>(cdiv(num_experts + 1, 64)), 1024, 0, st>>>(a);
+      group_place<false, true><<<chunks, kChunk, 0, st>>>(a);
+    }
   }
   RXMET_CHECK_LAUNCH();
   return 0;

@@ -38,6 +38,21 @@ def test_order(cuda, T, k, E):
     check_groups(chosen(T, k, E, T + E), E, cuda)
 
 
+# the last number of chunks that each adds up the others' counts, the first that are added up in between
+@pytest.mark.parametrize("n", [128 * 1024, 128 * 1024 + 1, 1500 * 1024 + 77])
+@pytest.mark.parametrize("E", [3, 64, 1024])
+def test_many_entries(cuda, n, E):
+    ids = torch.randint(-1, E + 1, (n,), dtype=torch.int32, generator=torch.Generator().manual_seed(n))
+    got = ops.group_experts(ids.view(-1, 1).to(cuda), E)
+    bins = torch.where((ids < 0) | (ids >= E), E, ids)
+    ordered, entries = bins.sort(stable=True)
+    places = torch.empty(n, dtype=torch.int32)
+    places[entries] = torch.arange(n, dtype=torch.int32)
+    places[bins == E] = -1
+    assert torch.equal(got.entries.cpu(), entries.int()) and torch.equal(got.places.cpu().view(-1), places)
+    assert torch.equal(got.offsets.cpu(), torch.searchsorted(ordered, torch.arange(E + 1, dtype=torch.int32)).int())
+
+
 @pytest.mark.parametrize("T", [7, 3000])
 def test_uneven_choices(cuda, T):
     check_groups(np.zeros((T, 4), np.int32), 9, cuda)              # all to one
