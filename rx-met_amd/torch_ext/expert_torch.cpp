@@ -112,7 +112,7 @@ py::object route_experts(const Tensor &logits, int64_t top_k, int score, const O
                          int64_t groups, std::optional<int64_t> top_groups, int64_t group_best,
                          bool renormalize, double scale) {
   int64_t tokens, E, stride;
-  if (!route_forward || type_code(logits.scalar_type()) < 0 || !plain(logits) ||
+  if (!route_forward || type_code(logits.scalar_type()) < 0 || !plain(logits) || dual(logits) ||
       !as_rows(logits, tokens, E, stride) || E > RXMET_EXPERTS_MAX || groups < 1 ||
       groups > RXMET_EXPERT_GROUPS_MAX || E % groups != 0 || top_k < 1 || top_k > RXMET_TOP_K_MAX ||
       (group_best != 1 && group_best != 2))
@@ -280,13 +280,13 @@ py::object experts_combine(const Tensor &y, const Tensor &weights, const OptTens
   if (!combine || type_code(y.scalar_type()) < 0 || !plain(y) || y.dim() != 2 ||
       !as_rows(y, rows, N, ys) || !groups_of(offsets, entries, places, y, g) ||
       rows != places.numel() || !is(weights, at::kFloat, y) || !weights.is_contiguous() ||
-      weights.sizes() != places.sizes())
+      weights.sizes() != places.sizes() || dual(y) || dual(weights))
     return py::none();
   if (residual) {
     auto shape = places.sizes().vec();
     shape.back() = N;
     if (!is(*residual, y.scalar_type(), y) || residual->sizes() != at::IntArrayRef(shape) ||
-        !as_rows(*residual, rr, rc, rs))
+        !as_rows(*residual, rr, rc, rs) || dual(*residual))
       return py::none();
   }
   if (at::GradMode::is_enabled() && (y.requires_grad() || weights.requires_grad() ||

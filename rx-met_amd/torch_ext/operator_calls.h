@@ -40,6 +40,9 @@ inline bool is(const Tensor &t, at::ScalarType type, const Tensor &like) {
   return t.scalar_type() == type && plain(t) && t.device() == like.device();
 }
 
+// Whether forward-mode differentiation goes through t: a tangent that no kernel gives must not go missing.
+inline bool dual(const Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+
 // t as rows with a dense last axis; false where that takes a copy.
 inline bool as_rows(const Tensor &t, int64_t &rows, int64_t &cols, int64_t &stride) {
   if (t.dim() < 1) return false;
