@@ -78,7 +78,10 @@ int rxmet_group_experts(const int32_t *experts, int64_t count, int32_t num_exper
                         int32_t *offsets, int32_t *entries, int32_t *places, void *workspace,
                         void *stream);
 
-/* What rxmet_group_experts gave for tokens * top_k entries. */
+/*
+ * What rxmet_group_experts gave for tokens * top_k entries.  Places may have been set to -1 since: entries without
+ * one add nothing in rxmet_experts_combine (rxmet_experts_linear_int8 goes by offsets and entries).
+ */
 typedef struct rxmet_expert_groups {
   const int32_t *offsets, *entries, *places;
   int64_t tokens;
@@ -113,10 +116,10 @@ int rxmet_experts_combine(const rxmet_expert_groups *groups, const void *y, int6
                           void *out, int64_t N, int32_t dtype, void *stream);
 
 /*
- * Its gradient for d_out [tokens, N]: d_y[places[t, j]] = weights[t, j] * d_out[t], 0 in the rows
- * behind the experts' last, and d_weights[t, j] = sum_n d_out[t, n] * y[places[t, j], n] in a fixed
- * order, 0 without a place.  d_y (dense) or d_weights may be NULL; y is needed for d_weights.  The
- * residual's gradient is d_out.
+ * Its gradient for d_out [tokens, N]: d_y[places[t, j]] = weights[t, j] * d_out[t], 0 in the rows that no entry
+ * has as its place, and d_weights[t, j] = sum_n d_out[t, n] * y[places[t, j], n] in a fixed order, 0 without a
+ * place.  No two entries may have the same place.  d_y (dense) or d_weights may be NULL; d_y needs the groups'
+ * entries, d_weights needs y.  The residual's gradient is d_out.
  */
 int rxmet_experts_combine_backward(const rxmet_expert_groups *groups, const void *d_out,
                                    int64_t d_out_stride, const void *y, int64_t y_stride,

@@ -165,9 +165,9 @@ __global__ __launch_bounds__(kChunk) void group_place(const GroupArgs a) {
 // its entries in fp32 in their order.  Bound: the rows' bytes.  PAST: y is larger than the memory's 256 MB
 // cache and is read past it ([65536, 2048]: 71 us, 76 through the caches; 25.6 us become 31.9 for 67 MB).
 struct CombineArgs {
-  const int32_t *offsets, *places;
+  const int32_t *entries, *places;
   int64_t tokens, rows;
-  int top_k, experts;
+  int top_k;
   const void *y, *res, *d_out;
   int64_t y_stride, res_stride, d_stride;
   const float *weights;
@@ -237,9 +237,38 @@ __global__ __launch_bounds__(256) void combine_rows(const CombineArgs a) {
   }
 }
 
-// The gradient: the threads of a token read its gradient once for up to TOGETHER of its rows, write theirs
-// and add up their products with y.  Rows of no expert are cleared by all.  Bound: the rows' bytes, read
-// and written ([65536, 2041] bf16, a tenth of no expert: 128 us, 541 MB, 4.2 TB/s).
+// The gradient.  First the rows that no entry has as its place are cleared (behind the experts' last, or taken
+// away by the caller): row i may be one where entries[i] is not placed there.  Then the threads of a token read
+// its gradient once for up to TOGETHER of its rows, write theirs and add up their products with y.  Rows that are
+// placed against `entries` are cleared and then written.  Bound: the rows' bytes, read and written ([65536, 2041]
+// bf16, a tenth of no expert: 7 + 127 us, 541 MB, 4.0 TB/s).
+constexpr int kClearRows = 16;  // rows that a wave looks at, far from each other: those to clear lie together
+
+template <typename T>
+__global__ __launch_bounds__(256) void clear_rows(const CombineArgs a) {
+  const int64_t waves = (a.rows + kClearRows - 1) / kClearRows;
+  const int64_t wave = static_cast<int64_t>(blockIdx.x) * (256 / kWave) + threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave;
+  if (wave >= waves) return;
+  const int64_t i = wave + waves * lane;
+  bool clear = false;
+  if (lane < kClearRows && i < a.rows) {
+    const int64_t entry = a.entries[i];
+    clear = entry < 0 || entry >= a.rows || a.places[entry] != i;
+  }
+  for (unsigned long long left = __ballot(clear); left != 0; left &= left - 1) {
+    T *row = static_cast<T *>(a.d_y) + (wave + waves * (__ffsll(left) - 1)) * a.N;
+    // 16 bytes at a time from where memory's lines are cut, the ends by element (from the row's start: 12 us)
+    const int64_t lead = (16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T), first = lead < a.N ? lead : a.N;
+    const int64_t pieces = (a.N - first) * static_cast<int64_t>(sizeof(T)) / 16, last = first + pieces * 16 / sizeof(T);
+    const v4i_any none = {0, 0, 0, 0};
+    for (int64_t n = lane; n < pieces; n += kWave)
+      __builtin_memcpy(reinterpret_cast<char *>(row + first) + 16 * n, &none, 16);
+    if (lane < first) row[lane] = static_cast<T>(0.0f);
+    if (last + lane < a.N) row[last + lane] = static_cast<T>(0.0f);
+  }
+}
+
 template <typename T, int TOGETHER>
 __global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
   __shared__ float s_dot[4][TOGETHER];
@@ -307,12 +336,6 @@ __global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
       for (int j = 0; j < TOGETHER; ++j)
         if (j0 + j < a.top_k) a.d_weights[t * a.top_k + j0 + j] = dot[j];
   }
-  if (!a.d_y || wanted >= a.tokens) return;
-  const int64_t held = a.offsets[a.experts];
-  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int64_t i = (held < 0 ? 0 : held) + t; i < a.rows; i += a.tokens)
-    for (int64_t n = 8 * at; n < a.N; n += 8 * width)
-      store_any(static_cast<T *>(a.d_y) + i * a.N + n, a.N - n, zero);
 }
 
 // Threads of a row, as a power of two: eight columns each, at most `most`.
@@ -382,7 +405,7 @@ extern "C" int rxmet_experts_combine(const rxmet_expert_groups *g, const void *y
   if (g->tokens == 0) return 0;
   RXMET_CHECK_ARG(g->places && y && weights && out, "places, y, weights and out are needed");
   const int shift = shift_for(N, 8);
-  const CombineArgs a{g->offsets, g->places, g->tokens, g->tokens * g->top_k, g->top_k, g->experts, y,
+  const CombineArgs a{g->entries, g->places, g->tokens, g->tokens * g->top_k, g->top_k, y,
                       residual, nullptr, y_stride, residual_stride, 0, weights, out, nullptr, nullptr, N, shift};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_combine", st);
@@ -405,17 +428,19 @@ extern "C" int rxmet_experts_combine_backward(const rxmet_expert_groups *g, cons
   if (const int rc = check_groups(g, N, dtype)) return rc;
   if (g->tokens == 0 || (!d_y && !d_weights)) return 0;
   RXMET_CHECK_ARG(g->places && d_out && weights, "places, d_out and weights are needed");
-  RXMET_CHECK_ARG(!d_y || g->offsets, "d_y needs the groups' offsets");
+  RXMET_CHECK_ARG(!d_y || g->entries, "d_y needs the groups' entries");
   RXMET_CHECK_ARG(!d_weights || y, "d_weights needs y");
   // a wave has a token, so that its sums over N meet without a barrier ([8192, 2041] x 8: 225 us, a workgroup
   // 271); a workgroup where tokens are few ([2048, 8192] x 8: 167 us, a wave 217)
   const int shift = shift_for(N, g->tokens >= 4096 ? 6 : 8);
-  const CombineArgs a{g->offsets, g->places, g->tokens, g->tokens * g->top_k, g->top_k, g->experts, y,
+  const CombineArgs a{g->entries, g->places, g->tokens, g->tokens * g->top_k, g->top_k, y,
                       nullptr, d_out, y_stride, 0, d_out_stride, weights, nullptr, d_y, d_weights, N, shift};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_combine_backward", st);
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
+    if (d_y)
+      clear_rows<T><<<static_cast<unsigned>(cdiv(cdiv(a.rows, kClearRows), 256 / kWave)), 256, 0, st>>>(a);
     const unsigned grid = static_cast<unsigned>(cdiv(g->tokens, 256 >> shift));
     if (g->top_k <= 2)
       combine_backward<T, 2><<<grid, 256, 0, st>>>(a);

@@ -354,8 +354,9 @@ def experts_combine(y, weights, groups: ExpertGroups, residual=None) -> torch.Te
 
     y [entries, N] float32, float16 or bfloat16, a row for each place of ``groups``; weights float32
     [..., top_k], shaped like ``groups.places``; residual [..., N] in y's type.  The sum is float32, in the
-    order of j, rounded once.  Entries of no expert add nothing; their rows of y are not read.
-    Differentiable in y (0 for the rows of no expert), weights and residual.
+    order of j, rounded once.  Entries of no expert add nothing; their rows of y are not read.  A caller may take
+    further entries away by setting their places to -1 (what exceeds an expert's capacity); no two may share a place.
+    Differentiable in y (0 for the rows of entries without a place), weights and residual.
     """
     ext = _ext or _native()
     if ext and not torch._C._are_functorch_transforms_active():
