@@ -13,7 +13,7 @@
 //
 // Bound: instructions, half of them for the scores and the sort ([16384, 256] fp32, bias, 8 groups, k = 8:
 // 21 us, 17 MB; without groups 17, without bias and groups 11).  A few tokens: one wave's way through all
-// steps (7.4 us).  Backward ([16384, 128] bf16, softmax as it is): 5.5 us.
+// steps (7.4 us).  Backward ([16384, 128] bf16, softmax as it is): 7.4 us.
 #include "../../include/rxmet_experts.h"
 #include "decoder_common.h"
 
@@ -290,7 +290,8 @@ __global__ __launch_bounds__(kWave) void route_forward(const RouteArgs a) {
   }
 }
 
-// The chosen experts' parts in 64 bits; where all logits have one (softmax as it is) the row in fp32.
+// In 64 bits, rounded once: where one expert has nearly all of the weight, its gradient is the difference of
+// numbers that are nearly the same (in fp32 that left no digit of it: softmax as it is, logits of deviation 8).
 template <typename T, int L, int V>
 __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
   constexpr int per = kWave / L, most = L * V;
@@ -317,7 +318,8 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
   };
   auto most_of = [](float p, float q) { return fmaxf(p, q); };
   const bool dense = softmax && !a.r.renormalize;
-  float p[V], inner = 0, top = -INFINITY;
+  double p[V], inner = 0;
+  float top = -INFINITY;
   bool bad = false;  // as in the forward pass: the weights are NaN, and so are their gradients
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -325,28 +327,27 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
     bad |= softmax && !(x[v] < INFINITY);
   }
   bad = over_lanes<L>(static_cast<int>(bad), [](int p, int q) { return p | q; });
+  auto plus = [](double p, double q) { return p + q; };
   if (dense) {
-    float total = 0;
+    double total = 0;
     top = over_lanes<L>(top, most_of);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      p[v] = bad ? static_cast<float>(kNan) : top == -INFINITY ? 0.0f : expf(x[v] - top);
+      p[v] = above(x[v], top, a.series);
       total += p[v];
     }
-    total = over_lanes<L>(total, [](float p, float q) { return p + q; });
-    const float part = total != 0 ? 1.0f / total : 0.0f;
+    total = over_lanes<L>(total, plus);
+    const double part = bad ? kNan : total != 0 ? inverse(total) : 0.0;
 #pragma unroll
     for (int v = 0; v < V; ++v) p[v] *= part;
     for (int j = lane; j < k; j += L) {
       const int e = expert(j);
       if (e < 0) continue;
-      const float l = s_logit[slot][e];
-      inner += dw[j] * (total != total ? total : top == -INFINITY ? 0.0f : expf(l - top) * part);
+      inner += dw[j] * (above(s_logit[slot][e], top, a.series) * part);
       s_grad[slot][e] = dw[j];
     }
-    inner = over_lanes<L>(inner, [](float p, float q) { return p + q; });
+    inner = over_lanes<L>(inner, plus);
   } else {
-    auto plus = [](double p, double q) { return p + q; };
     top = -INFINITY;
     double total = 0, mean = 0;
     if (a.r.renormalize) {
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(kWave) void route_backward(const RouteArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     g[v] = s_grad[slot][e0 + v];
-    if (dense) g[v] = p[v] * (g[v] - inner) * a.r.scale;
+    if (dense) g[v] = static_cast<float>(p[v] * (g[v] - inner) * a.r.scale);
   }
   if (e0 + V <= E) {
     T u[V];
