@@ -34,10 +34,10 @@ enum {
 
 /*
  * How a token's experts are chosen.  With a bias the experts are ordered by c_e = fl32(s_e) + bias_e
- * (the score rounded to fp32, one fp32 addition), without one by their logits; NaN counts as
- * -infinity and ties go to the lowest index.  The `experts` fall into `groups` runs of equal length:
- * a group's value is the sum (fp32) of its `group_best` (1 or 2) largest c (without a bias: of
- * fl32(s_e); of the logit alone where group_best is 1), and only the `top_groups` groups of the
+ * (the score, computed in 64 bits to a few 2^-53 and rounded to fp32; one fp32 addition), without one by
+ * their logits; NaN counts as -infinity and ties go to the lowest index.  The `experts` fall into `groups`
+ * runs of equal length: a group's value is the sum (fp32) of its `group_best` (1 or 2) largest c (without a
+ * bias: of fl32(s_e); of the logit alone where group_best is 1), and only the `top_groups` groups of the
  * largest values are chosen from.
  * Weights are the scores without the bias, over their sum (renormalize != 0), times `scale`.
  */

@@ -2,9 +2,11 @@
 //
 // Mathematics.  s_e = exp(l_e - m) / sum_i exp(l_i - m) or 1 / (1 + exp(-l_e)).  The choice goes by
 // c_e = fl32(s_e) + b_e, with the score computed in 64 bits, so that its rounding to fp32 does not go
-// by the order of a sum or the function's last bit, and any evaluation that is good to a few 2^-53
-// chooses the same experts.  Without a bias the logits themselves are the order.  Weights of the chosen
-// are computed in 64 bits too (k of them, against E scores).
+// by the order of a sum or the function's last bit: the score is off by a few 2^-53 of itself (at most one for each
+// of the up to 22 additions that one passes through, and some four of exp and the quotient), which changes the
+// rounding of one in some 2^26 scores.
+// Without a bias the logits themselves are the order.  Weights of the chosen are computed in 64 bits too (k of them,
+// against E scores).
 //
 // Layout.  L lanes have a token, each V consecutive experts, 64 / L tokens a wave.  A candidate is
 // one double in [1, 2) whose 52 bits hold the ordered bits of c_e and, below them, 1023 - e: one maximum
@@ -13,7 +15,7 @@
 //
 // Bound: instructions, half of them for the scores and the sort ([16384, 256] fp32, bias, 8 groups, k = 8:
 // 21 us, 17 MB; without groups 17, without bias and groups 11).  A few tokens: one wave's way through all
-// steps (7.4 us).  Backward ([16384, 128] bf16, softmax as it is): 7.4 us.
+// steps (7.4 us).  Backward ([16384, 128] bf16, softmax as it is): 7.8 us.
 #include "../../include/rxmet_experts.h"
 #include "decoder_common.h"
 
@@ -21,21 +23,22 @@ namespace rxmet {
 namespace dec {
 namespace {
 
-
-// exp(v) for v in [-700, 700], a value outside taken for the nearest: v = n ln 2 + r, and the series of exp(r),
-// |r| <= ln(2) / 2, up to r^11 (what follows is below 2^-46 of it).  The powers' factors come as
-// scalars: as literals each of them costs two moves where it is used.
+// exp(v) for v in [-700, 700], a value outside taken for the nearest: v = n ln 2 + r with ln 2 in two parts, the first
+// of few bits, so that what is taken off is exact (Cody and Waite's reduction), and the series of exp(r),
+// |r| <= ln(2) / 2, up to r^13 (what follows is below 2^-57 of it; up to r^11 it was 2^-46, and scores next to a border
+// of fp32 fell on its other side).  The factors come as scalars: as literals each of them costs two moves where it is
+// used.
 struct Series {
-  double c[10];  // 1 / 2! .. 1 / 11!
+  double ln2, ln2_rest;
+  double c[12];  // 1 / 2! .. 1 / 13!
 };
 __device__ __forceinline__ double exp_series(double v, const Series &s) {
   v = fmin(fmax(v, -700.0), 700.0);
   const double n = __builtin_rint(v * 1.4426950408889634);
-  // ln 2 in two parts, the first of few bits
-  const double r = __builtin_fma(n, -1.9082149292705877e-10, __builtin_fma(n, -0.693147180369123816490, v));
-  double p = s.c[9];
+  const double r = __builtin_fma(-n, s.ln2_rest, __builtin_fma(-n, s.ln2, v));
+  double p = s.c[11];
 #pragma unroll
-  for (int i = 8; i >= 0; --i) p = __builtin_fma(p, r, s.c[i]);
+  for (int i = 10; i >= 0; --i) p = __builtin_fma(p, r, s.c[i]);
   p = __builtin_fma(__builtin_fma(p, r, 1.0), r, 1.0);
   return __builtin_ldexp(p, static_cast<int>(n));
 }
@@ -427,9 +430,12 @@ void by_experts(int64_t tokens, int E, F &&f) {
 }
 
 Series series() {
+  constexpr long double ln2 = 0.693147180559945309417232121458176568L;
   Series s;
+  s.ln2 = std::ldexp(std::floor(std::ldexp(static_cast<double>(ln2), 32)), -32);
+  s.ln2_rest = static_cast<double>(ln2 - s.ln2);
   double f = 1;
-  for (int i = 0; i < 10; ++i) s.c[i] = 1 / (f *= i + 2);
+  for (int i = 0; i < 12; ++i) s.c[i] = 1 / (f *= i + 2);
   return s;
 }
 
