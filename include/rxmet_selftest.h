@@ -1,8 +1,9 @@
 /*
- * rxmet_selftest.h — self-tests of hardware assumptions the kernels rely on.
+ * rxmet_selftest.h — self-tests of what the kernels rely on.
  *
  * No counterpart in the reference: these entry points exist so that tests can check,
- * on the GPU, the MFMA operand/result lane layouts the GRU kernels are written against.
+ * on the GPU, the MFMA operand/result lane layouts the GRU kernels are written against, and, on the
+ * host, which form of a kernel a call takes.
  */
 #ifndef RXMET_SELFTEST_H_
 #define RXMET_SELFTEST_H_
@@ -22,6 +23,13 @@ extern "C" {
  * A row-major [16][K], B row-major [K][16], D row-major [16][16].
  */
 int rxmet_selftest_mfma(int which, const void *A, const void *B, void *D, void *stream);
+
+/*
+ * The form that rxmet_experts_linear_int8 takes for `rows` places of `experts` experts with `weight_rows`
+ * weight rows (N, gated 2 N) each.  0, 1: few rows, four waves or one for 32 weight rows; 2, 3, 4: tiles of
+ * 128 weight rows x 64 places, 128 x 128 and 256 x 256.
+ */
+int rxmet_selftest_experts_form(int64_t rows, int64_t experts, int64_t weight_rows);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "../../include/rxmet_experts.h"
+#include "../../include/rxmet_selftest.h"
 #include "int8_tile.h"
 
 namespace rxmet {
@@ -665,6 +666,11 @@ void launch(const ExpertArgs &a, hipStream_t st) {
 
 using namespace rxmet;
 using namespace rxmet::dec;
+
+extern "C" int rxmet_selftest_experts_form(int64_t rows, int64_t experts, int64_t weight_rows) {
+  RXMET_CHECK_ARG(rows >= 1 && experts >= 1 && weight_rows >= 1, "sizes must be positive");
+  return shape_for(rows, experts, weight_rows);
+}
 
 extern "C" int rxmet_experts_linear_int8(const rxmet_expert_groups *g, int32_t grouped,
                                          const int8_t *codes, int64_t codes_stride,

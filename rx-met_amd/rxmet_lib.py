@@ -129,6 +129,7 @@ _SIGNATURES = {
     "rxmet_dequantize_backward_ex": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, _LAY, _NUM, c_ptr,
                                              c_ptr, c_ptr, c_ptr]),
     "rxmet_selftest_mfma": (c_int, [c_int, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "rxmet_selftest_experts_form": (c_int, [c_i64, c_i64, c_i64]),
     "rxmet_qdq_encoding_forward": (c_int, [c_ptr, c_ptr, c_i64, c_i64, c_i64, ctypes.c_int32,
                                            ctypes.c_float, ctypes.c_float, c_ptr, c_ptr, c_ptr]),
     "rxmet_qdq_encoding_backward": (c_int, [c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64,
