@@ -160,6 +160,8 @@ class QuantDecoderLayer(nn.Module):
         out where ``experts`` are given."""
         if heads is None or kv_heads is None:
             raise TypeError("heads and kv_heads are needed")
+        if (w_up is None) != (w_down is None) or (w_up is not None and kw.get("experts") is not None):
+            raise ValueError("w_up and w_down are needed both, or neither where experts are given")
         width = w_qkv.shape[1]
         layer = cls(width, heads, kv_heads, w_o.shape[1] // heads,
                     None if w_up is None else w_up.shape[0], device=w_qkv.device, **kw)
