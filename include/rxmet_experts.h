@@ -51,7 +51,7 @@ typedef struct rxmet_router {
  * experts, weights [tokens, top_k]: the chosen experts in their order (int32) and their weights
  * (fp32).  logits [tokens, experts] with a row stride; bias [experts] fp32 or NULL.  A softmax row
  * with a NaN or +infinity has NaN weights, a sigmoid one where a NaN is chosen; chosen experts whose
- * logits are all -infinity have the weights 0.
+ * logits are all -infinity have the weights 0.  At most 2^24 tokens.
  */
 int rxmet_route_forward(const rxmet_router *router, const void *logits, int64_t stride,
                         const float *bias, int32_t *experts, float *weights, int64_t tokens,
@@ -66,7 +66,7 @@ int rxmet_route_backward(const rxmet_router *router, const void *logits, int64_t
                          int64_t tokens, int32_t dtype, void *stream);
 
 /*
- * Order of `count` entries by expert, entries of the same expert in their order.  experts [count]
+ * Order of `count` entries (at most 2^26) by expert, entries of the same expert in their order.  experts [count]
  * int32; ids outside 0..num_experts-1 belong to no expert.
  *   offsets  [num_experts + 1] out: expert e's places are offsets[e]..offsets[e + 1]
  *   entries  [count] out: the entry of each place; behind offsets[num_experts] stand those of no expert
@@ -98,6 +98,9 @@ typedef struct rxmet_expert_groups {
  * weight_scales and bias [experts, N or 2 N] dense, bias in dtype or NULL; y [tokens * top_k, N] dense.
  * The sum is exact (int32), the rest fp32, rounded once to dtype.  Rows behind offsets[experts]
  * are not written.  Offsets and entries out of their range lead to no access out of bounds.
+ * At most 2^24 tokens, fewer than 2^26 rows (tokens * top_k), N up to 2^24, K up to 131071; and the grid has to hold
+ * what the rows may need: ceil(N / 128) (gated: / 64) * (rows / 64 + experts) and ceil(N / 32) (gated: / 16) * experts
+ * are below 2^22.
  */
 int rxmet_experts_linear_int8(const rxmet_expert_groups *groups, int32_t grouped,
                               const int8_t *codes, int64_t codes_stride, const float *scales,
@@ -109,7 +112,8 @@ int rxmet_experts_linear_int8(const rxmet_expert_groups *groups, int32_t grouped
 /*
  * out[t] = sum_j weights[t, j] * y[places[t, j]] + residual[t], in fp32 in the order of j, rounded
  * once.  Entries without a place add nothing.  y [tokens * top_k, N] and residual [tokens, N] (or NULL)
- * in dtype with row strides; weights [tokens, top_k] fp32; out [tokens, N] dense.
+ * in dtype with row strides; weights [tokens, top_k] fp32; out [tokens, N] dense.  At most 2^23 tokens, N up to
+ * 2^24, in the gradient too.
  */
 int rxmet_experts_combine(const rxmet_expert_groups *groups, const void *y, int64_t y_stride,
                           const float *weights, const void *residual, int64_t residual_stride,

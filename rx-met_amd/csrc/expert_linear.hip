@@ -10,7 +10,7 @@
 // Bound and measured.  Few rows: the weights' bytes (16 tokens of 8 of 64 experts, gated [2048, 2048]: 268 MB
 // of which 56 experts' are read, 46 us warm, 5.1 TB/s; 57 with other inputs in between).  Many: [65536, 2048] of 32
 // experts' [2048, 2048] 327 us warm, 1.68 POP/s, gated [4096, 2048] 628 us, 1.75 POP/s; the matrix unit is
-// busy for 35 to 39 % of that.  Over K alone (2048 to 4096) the loop runs at 2.0 POP/s, where the library's
+// busy for 35 and 41 % of that.  Over K alone (2048 to 4096) the loop runs at 2.0 POP/s, where the library's
 // product of 8192^3 without an epilogue reaches 2.1: without its loads it would at 2.9, and they are 64 KB a step and
 // CU on their way while one step is multiplied, which LDS has no room to do further ahead.  The rest is
 // the tiles' start and end, when the outputs' bytes (268 MB) are written with little to multiply.
@@ -496,8 +496,8 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM > 128 * 64 ? 2 : 3) void expe
     __syncthreads();
   }
 
-  // A lane finishes its 16 consecutive columns of a place; 128 bytes of 32 places at a time go through the
-  // wave's part of the LDS, from where neighbouring lanes write what lies side by side.
+  // A lane finishes its 16 consecutive columns of a place; 128 bytes of 32 places at a time (64 of gated outputs in
+  // 16 bits) go through the wave's part of the LDS, from where neighbouring lanes write what lies side by side.
   // The activation is chosen once: asked for at each element, the code that is jumped over falls out
   // of the instruction cache.
   uint4 *out = reinterpret_cast<uint4 *>(&s[0][0]) + wave * 256;
@@ -662,6 +662,9 @@ void launch_few(const ExpertArgs &a, int64_t grid, hipStream_t st) {
 // More: a tile size costs its rounds of tiles over the CUs (half a round more, for the last one is not
 // full) times what a round takes; of 32 experts with [2048, 2048], [R / E: 256 x 256, 128 x 128, 128 x 64]
 // 64: 40 28 29 us; 256: 72 67 65; 384: 105 91 97; 512: 108 116 118; 2048: 388 441 481.
+//
+// R counts entries of no expert too, as how many there are stands on the device alone: with nine of ten such, 8192 x 8
+// of them take 61 us (as many rows in a call of their own 84), 2048 x 8 48 us (45).
 enum Shape { kFewShared, kFewOne, k128x64, k128x128, k256x256 };
 
 Shape shape_for(int64_t rows, int64_t experts, int64_t out_rows) {
@@ -723,7 +726,11 @@ extern "C" int rxmet_experts_linear_int8(const rxmet_expert_groups *g, int32_t g
   RXMET_CHECK_ARG(codes && scales && weight && weight_scales && y,
                   "codes, weight, their scales and y are needed");
   // An output of whole 16-byte pieces that would push codes and weights out of the memory's 256 MB cache is
-  // written past it ([65536, 2048] of [2048, 2048] weights: 384 -> 327 us).
+  // written past it, also where the next call reads it (us through the caches and past them, in brackets with
+  // quantize_rows behind: 32 experts' [2048, 2048] weights, bf16, 64 MB of output 122 and 115 [141, 140], 128 MB 204
+  // and 185 [238, 236], 256 MB 364 and 335 [451, 434]; below, 32 MB, 84 and 75 [95, 97]).  Gated ones, with twice the
+  // products to an output, gain and lose up to 2 % (128 MB 374 and 380 [418, 425], 256 MB 688 and 688 [778, 775], other
+  // inputs in turn 690 and 685).
   const int64_t size = dtype == RXMET_QDQ_F32 ? 4 : 2;
   const bool past = rows * N * size >= 64LL << 20 && (N * size | reinterpret_cast<uintptr_t>(y)) % 16 == 0;
   const ExpertArgs a{g->offsets, g->entries, g->tokens, rows, g->top_k, g->experts, grouped != 0,

@@ -14,7 +14,8 @@
 // heads is taken k times.
 //
 // Bound: instructions, half of them for the scores and the sort ([16384, 256] fp32, bias, 8 groups, k = 8:
-// 21 us, 17 MB; without groups 17, without bias and groups 11).  A few tokens: one wave's way through all
+// 21 us, 17 MB; without groups 17, without bias and groups 11).  One lane values a group, so few large ones cost
+// most: [4096, 1024] in 2 groups 52 us, in 8 27, in 64 25, without groups 18.  A few tokens: one wave's way through all
 // steps (7.4 us).  Backward ([16384, 128] bf16, softmax as it is): 7.8 us.
 #include "../../include/rxmet_experts.h"
 #include "decoder_common.h"

@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256) void combine_rows(const CombineArgs a) {
 // away by the caller): row i may be one where entries[i] is not placed there.  Then the threads of a token read
 // its gradient once for up to TOGETHER of its rows, write theirs and add up their products with y.  Rows that are
 // placed against `entries` are cleared and then written.  Bound: the rows' bytes, read and written ([65536, 2041]
-// bf16, a tenth of no expert: 7 + 127 us, 541 MB, 4.0 TB/s).
+// bf16, a tenth of no expert: 7 + 125 us, 541 MB, 4.1 TB/s).
 constexpr int kClearRows = 16;  // rows that a wave looks at, far from each other: those to clear lie together
 
 template <typename T>

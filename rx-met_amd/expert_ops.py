@@ -144,7 +144,7 @@ def route_experts(logits, top_k: int, score: str = "softmax", bias=None, groups:
     ``scale``.  A softmax row with a NaN or +infinity has NaN weights, a sigmoid one where a NaN is chosen;
     chosen experts whose logits are all -infinity have weights 0.
 
-    logits float32, float16 or bfloat16, E up to 1024, top_k up to 64.  Differentiable in logits; the
+    logits float32, float16 or bfloat16, up to 2^24 rows, E up to 1024, top_k up to 64.  Differentiable in logits; the
     bias and the choice get no gradient.
     """
     ext = _ext or _native()
@@ -182,7 +182,8 @@ class ExpertGroups(NamedTuple):
 def group_experts(experts, num_experts: int) -> ExpertGroups:
     """The order of the entries of experts int32 [..., top_k] by expert; entries of an expert keep
     theirs.  Ids outside 0..num_experts - 1 belong to no expert (experts of another process,
-    tokens of a padded batch): such entries are multiplied and added up by nothing."""
+    tokens of a padded batch): such entries are multiplied and added up by nothing.  At most 2^26
+    entries."""
     ext = _ext or _native()
     if ext:
         out = ext.group_experts(experts, num_experts)
@@ -244,7 +245,8 @@ def experts_linear_int8(codes, scales, weight, weight_scales, groups: ExpertGrou
     rows, and a column is ``act(row n) * (row N + n)``.  activation: None, "relu", "silu" or "gelu" (with
     the error function).  For inference: nothing here carries a gradient.
     The sum over K is exact, the rest float32.  K is at most 131071.  Rows behind the experts' last place are
-    not written.  Rows that do not start on 16 bytes (K no multiple of 16) are read more slowly.
+    not written.  Rows that do not start on 16 bytes (K no multiple of 16) are read more slowly.  At most
+    2^24 tokens and fewer than 2^26 entries; ceil(N / 128) (gated: / 64) * (entries / 64 + E) is below 2^22.
     """
     ext = _ext or _native()
     if ext and activation in ACTIVATIONS:
@@ -356,6 +358,7 @@ def experts_combine(y, weights, groups: ExpertGroups, residual=None) -> torch.Te
     [..., top_k], shaped like ``groups.places``; residual [..., N] in y's type.  The sum is float32, in the
     order of j, rounded once.  Entries of no expert add nothing; their rows of y are not read.  A caller may take
     further entries away by setting their places to -1 (what exceeds an expert's capacity); no two may share a place.
+    At most 2^23 tokens.
     Differentiable in y (0 for the rows of entries without a place), weights and residual.
     """
     ext = _ext or _native()

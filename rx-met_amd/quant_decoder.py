@@ -59,7 +59,12 @@ class Step(NamedTuple):
 
 class QuantExperts(nn.Module):
     """A feed-forward of experts on int8 weights (a scale per output): router, the chosen experts' two
-    products, their rows added up.  The logits are float32, from the codes that the experts get."""
+    products, their rows added up.  The logits are float32, from the codes that the experts get.
+
+    The router is in 8 bits like the products, which changes some choices: of random normal tokens and weights
+    of width 2048, 1.0 % of the chosen (8 of 64 experts; of width 4096 and 8 of 256 1.5 %), 0.7 % (1.1 %) of it by the
+    router's own codes and the rest by the tokens'.  A router that stays in float takes the operators of
+    ``expert_ops`` one by one, with its logits for ``route_experts``."""
 
     def __init__(self, width: int, hidden: int, experts: int, top_k: int, activation: str = "silu",
                  gated: bool = True, score: str = "softmax", with_bias: bool = False, groups: int = 1,
