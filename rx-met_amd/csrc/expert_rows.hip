@@ -175,6 +175,7 @@ struct CombineArgs {
   float *d_weights;
   int64_t N;
   int shift;  // 2^shift threads have a row
+  unsigned blocks;  // workgroups of the tokens; those behind them clear rows of the gradient
 };
 
 template <typename T>
@@ -237,12 +238,33 @@ __global__ __launch_bounds__(256) void combine_rows(const CombineArgs a) {
   }
 }
 
-// The gradient.  First the rows that no entry has as its place are cleared (behind the experts' last, or taken
-// away by the caller): row i may be one where entries[i] is not placed there.  Then the threads of a token read
-// its gradient once for up to TOGETHER of its rows, write theirs and add up their products with y.  Rows that are
-// placed against `entries` are cleared and then written.  Bound: the rows' bytes, read and written ([65536, 2041]
-// bf16, a tenth of no expert: 7 + 125 us, 541 MB, 4.1 TB/s).
+// The gradient: the threads of a token read its gradient once for up to TOGETHER of its rows, write theirs
+// and add up their products with y.  Rows that no entry has as its place (behind the experts' last, or taken away by
+// the caller) are cleared.  Such a row's entry of `entries` is not placed there.  Up to kScan rows, where a launch
+// costs most (2 to 4 us of a pass that the host bounds), waves of the same launch clear those that no place names; above,
+// where that would read all places too often, a launch ahead clears all whose entry is placed elsewhere, and what is
+// placed there against `entries` is written after.  Bound: the rows' bytes, read and
+// written ([65536, 2041] bf16, a tenth of no expert: 7 + 125 us, 541 MB, 4.1 TB/s).
+constexpr int kScan = 4096;
 constexpr int kClearRows = 16;  // rows that a wave looks at, far from each other: those to clear lie together
+
+// Whether no entry that `entries` knows of has row i as its place.
+__device__ __forceinline__ bool unplaced(const CombineArgs &a, int64_t i) {
+  const int64_t entry = a.entries[i];
+  return entry < 0 || entry >= a.rows || a.places[entry] != i;
+}
+
+template <typename T>
+__device__ __forceinline__ void clear_row(const CombineArgs &a, int64_t i, int lane) {
+  T *row = static_cast<T *>(a.d_y) + i * a.N;
+  // 16 bytes at a time from where memory's lines are cut, the ends by element (from the row's start: 12 us)
+  const int64_t lead = (16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T), first = lead < a.N ? lead : a.N;
+  const int64_t pieces = (a.N - first) * static_cast<int64_t>(sizeof(T)) / 16, last = first + pieces * 16 / sizeof(T);
+  const v4i_any none = {0, 0, 0, 0};
+  for (int64_t n = lane; n < pieces; n += kWave) __builtin_memcpy(reinterpret_cast<char *>(row + first) + 16 * n, &none, 16);
+  if (lane < first) row[lane] = static_cast<T>(0.0f);
+  if (last + lane < a.N) row[last + lane] = static_cast<T>(0.0f);
+}
 
 template <typename T>
 __global__ __launch_bounds__(256) void clear_rows(const CombineArgs a) {
@@ -251,28 +273,25 @@ __global__ __launch_bounds__(256) void clear_rows(const CombineArgs a) {
   const int lane = threadIdx.x % kWave;
   if (wave >= waves) return;
   const int64_t i = wave + waves * lane;
-  bool clear = false;
-  if (lane < kClearRows && i < a.rows) {
-    const int64_t entry = a.entries[i];
-    clear = entry < 0 || entry >= a.rows || a.places[entry] != i;
-  }
-  for (unsigned long long left = __ballot(clear); left != 0; left &= left - 1) {
-    T *row = static_cast<T *>(a.d_y) + (wave + waves * (__ffsll(left) - 1)) * a.N;
-    // 16 bytes at a time from where memory's lines are cut, the ends by element (from the row's start: 12 us)
-    const int64_t lead = (16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T), first = lead < a.N ? lead : a.N;
-    const int64_t pieces = (a.N - first) * static_cast<int64_t>(sizeof(T)) / 16, last = first + pieces * 16 / sizeof(T);
-    const v4i_any none = {0, 0, 0, 0};
-    for (int64_t n = lane; n < pieces; n += kWave)
-      __builtin_memcpy(reinterpret_cast<char *>(row + first) + 16 * n, &none, 16);
-    if (lane < first) row[lane] = static_cast<T>(0.0f);
-    if (last + lane < a.N) row[last + lane] = static_cast<T>(0.0f);
-  }
+  const bool clear = lane < kClearRows && i < a.rows && unplaced(a, i);
+  for (unsigned long long left = __ballot(clear); left != 0; left &= left - 1)
+    clear_row<T>(a, wave + waves * (__ffsll(left) - 1), lane);
 }
 
 template <typename T, int TOGETHER>
 __global__ __launch_bounds__(256) void combine_backward(const CombineArgs a) {
   __shared__ float s_dot[4][TOGETHER];
   const int width = 1 << a.shift, at = threadIdx.x & (width - 1), wave = threadIdx.x / kWave;
+  if (blockIdx.x >= a.blocks) {  // a wave a row
+    const int64_t i = static_cast<int64_t>(blockIdx.x - a.blocks) * (256 / kWave) + wave;
+    const int lane = threadIdx.x % kWave;
+    if (i >= a.rows || !unplaced(a, i)) return;
+    bool named = false;
+#pragma unroll 8
+    for (int64_t x = lane; x < a.rows; x += kWave) named |= a.places[x] == i;
+    if (!__any(named)) clear_row<T>(a, i, lane);
+    return;
+  }
   const int64_t wanted = static_cast<int64_t>(blockIdx.x) * (256 >> a.shift) + (threadIdx.x >> a.shift);
   const int64_t t = wanted < a.tokens ? wanted : a.tokens - 1;  // (all threads meet below)
   const int32_t *place = a.places + t * a.top_k;
@@ -406,7 +425,7 @@ extern "C" int rxmet_experts_combine(const rxmet_expert_groups *g, const void *y
   RXMET_CHECK_ARG(g->places && y && weights && out, "places, y, weights and out are needed");
   const int shift = shift_for(N, 8);
   const CombineArgs a{g->entries, g->places, g->tokens, g->tokens * g->top_k, g->top_k, y,
-                      residual, nullptr, y_stride, residual_stride, 0, weights, out, nullptr, nullptr, N, shift};
+                      residual, nullptr, y_stride, residual_stride, 0, weights, out, nullptr, nullptr, N, shift, 0};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_combine", st);
   with_type(dtype, [&](auto t) {
@@ -434,14 +453,15 @@ extern "C" int rxmet_experts_combine_backward(const rxmet_expert_groups *g, cons
   // 271); a workgroup where tokens are few ([2048, 8192] x 8: 167 us, a wave 217)
   const int shift = shift_for(N, g->tokens >= 4096 ? 6 : 8);
   const CombineArgs a{g->entries, g->places, g->tokens, g->tokens * g->top_k, g->top_k, y,
-                      nullptr, d_out, y_stride, 0, d_out_stride, weights, nullptr, d_y, d_weights, N, shift};
+                      nullptr, d_out, y_stride, 0, d_out_stride, weights, nullptr, d_y, d_weights, N, shift,
+                      static_cast<unsigned>(cdiv(g->tokens, 256 >> shift))};
   auto st = static_cast<hipStream_t>(stream);
   prof::Scope scope("experts_combine_backward", st);
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    if (d_y)
+    if (d_y && a.rows > kScan)
       clear_rows<T><<<static_cast<unsigned>(cdiv(cdiv(a.rows, kClearRows), 256 / kWave)), 256, 0, st>>>(a);
-    const unsigned grid = static_cast<unsigned>(cdiv(g->tokens, 256 >> shift));
+    const unsigned grid = a.blocks + (d_y && a.rows <= kScan ? static_cast<unsigned>(cdiv(a.rows, 256 / kWave)) : 0);
     if (g->top_k <= 2)
       combine_backward<T, 2><<<grid, 256, 0, st>>>(a);
     else if (g->top_k <= 4)

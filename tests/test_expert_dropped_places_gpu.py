@@ -32,7 +32,8 @@ def named(g):
     return rows
 
 
-@pytest.mark.parametrize("T,k,N", [(1, 3, 5), (40, 2, 33), (30, 8, 1000), (25, 10, 4100), (4100, 2, 40)])
+@pytest.mark.parametrize("T,k,N", [(1, 3, 5), (40, 2, 33), (30, 8, 1000), (25, 10, 4100), (1024, 4, 70), (1366, 3, 33),
+                                   (4100, 2, 40)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_gradient_of_rows_without_an_entry_is_zero(cuda, T, k, N, dtype):
     y, w, g, d = make(cuda, T, k, N, 4, dtype, T + N)
@@ -58,13 +59,14 @@ def test_gradient_of_rows_without_an_entry_is_zero(cuda, T, k, N, dtype):
 
 
 @pytest.mark.parametrize("native", [True, False])
-def test_places_of_another_order(cuda, monkeypatch, native):
+@pytest.mark.parametrize("T", [60, 1200])
+def test_places_of_another_order(cuda, monkeypatch, native, T):
     """Places that `entries` does not know: the sum and its gradient go by the places alone."""
     if not native:
         monkeypatch.setattr(ops, "_ext", False)
-    y, w, g, d = make(cuda, 60, 4, 50, 5, torch.float32, 9)
-    order = torch.randperm(240, device=cuda, generator=torch.Generator(cuda).manual_seed(1)).int()
-    places = torch.where(g.places < 0, -1, order.view(60, 4))
+    y, w, g, d = make(cuda, T, 4, 50, 5, torch.float32, 9)
+    order = torch.randperm(4 * T, device=cuda, generator=torch.Generator(cuda).manual_seed(1)).int()
+    places = torch.where(g.places < 0, -1, order.view(T, 4))
     other = ops.ExpertGroups(g.offsets, g.entries, places)
     y.requires_grad_(), w.requires_grad_()
     out = ops.experts_combine(y, w, other)
